@@ -565,6 +565,83 @@ int qia_sage_attention_noalloc(const void* q, const void* k, const void* v,
                                const int64_t* strides, float sm_scale,
                                void* stream);
 
+/* ---------------------------------------------------------------------------
+ * INT8 prefix cache and the attention that reads it (no counterpart in the
+ * reference, whose KV cache is bf16)
+ *
+ * A cached row is one token of one head: 128 INT8 codes and one f32 scale,
+ *   scale = max|x| / 127, code = rint(x * (127 / max|x|)), value = code * scale
+ * (an all-zero row has scale 0; a row holding NaN or infinity has scale NaN).
+ * codes: int8 [batch, heads, capacity, 128]; scales: f32 [batch, heads,
+ * capacity]; lengths: int32 [batch], tokens held per request (device memory).
+ * ------------------------------------------------------------------------ */
+
+/* Quantizes K and V rows [batch, seq, heads, 128] bf16 (strides: elements, k's
+ * batch, seq, head, then v's; multiples of 8) into tokens [start, start + seq)
+ * of every request and sets lengths[b] = start + seq. start < 0 appends at
+ * lengths[b] instead and adds seq to it: tokens past the capacity are dropped,
+ * the length stops there and QIA_ERR_INVALID is recorded in the device error
+ * word; ticket: one uint32 of device memory, zero before the first append,
+ * which the calls leave at zero (appends that share it must not overlap; NULL
+ * with a fixed start). head_dim = 128. */
+int qia_kv_cache_write(const void* k, const void* v, void* k_codes,
+                       void* v_codes, void* k_scales, void* v_scales,
+                       void* lengths, int64_t batch, int64_t seq, int64_t heads,
+                       int64_t head_dim, int64_t capacity, int64_t start,
+                       const int64_t* strides, void* ticket, void* stream);
+
+/* Cached tokens [first, first + tokens) as bf16 rows k, v [batch, tokens,
+ * heads, 128] (strides as above); rows past a request's length are zeros. */
+int qia_kv_cache_read(const void* k_codes, const void* v_codes,
+                      const void* k_scales, const void* v_scales,
+                      const void* lengths, void* k, void* v, int64_t batch,
+                      int64_t first, int64_t tokens, int64_t heads,
+                      int64_t head_dim, int64_t capacity, const int64_t* strides,
+                      void* stream);
+
+/* out = softmax(sm_scale q.K) V over the request's cached tokens
+ * [0, min(lengths[b], extent)) and seq_k fresh bf16 tokens k, v [batch, seq_k,
+ * kv_heads, 128] (NULL when seq_k is 0). Query head h reads K/V head
+ * h / (heads / kv_heads). key_valid: bytes [batch, extent + seq_k] (batch
+ * stride mask_stride), non-zero where a key takes part (columns [0, extent)
+ * the cached tokens, then the fresh ones), or NULL. Masked keys do not count
+ * whatever they hold; a query without keys writes zeros. strides: elements, of
+ * q, k, v, out (batch, seq, head each; multiples of 8). sm_scale <= 0:
+ * 1/sqrt(128). Products of exact INT8 codes (cached) or bf16 rows (fresh),
+ * fp32 scores, sums and accumulators; softmax weights are rounded once for the
+ * second product. head_dim = 128, heads / kv_heads <= 128. */
+int qia_cached_attention(const void* q, const void* k, const void* v,
+                         const void* k_codes, const void* v_codes,
+                         const void* k_scales, const void* v_scales,
+                         const void* lengths, const void* key_valid, void* out,
+                         int64_t batch, int64_t seq_q, int64_t seq_k,
+                         int64_t heads, int64_t kv_heads, int64_t head_dim,
+                         int64_t capacity, int64_t extent, const int64_t* strides,
+                         int64_t mask_stride, float sm_scale, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Low-rank adapters, one per request, beside a shared projection (no
+ * counterpart in the reference)
+ * ------------------------------------------------------------------------ */
+
+/* y[b, s] = base[b, s] + scales[i] * B_i (A_i x[b, s]) with i = ids[b];
+ * ids[b] < 0: y = base (an id past the table is treated so too and recorded in
+ * the device error word as QIA_ERR_INVALID). x [batch, seq, in], base and y
+ * [batch, seq, out] bf16 (y may be base), strides: elements, (batch, seq) of
+ * x, base, y, multiples of 8, rows contiguous. a: bf16 [adapters, r_pad, in],
+ * b: bf16 [adapters, out, r_pad]; only the first ranks[i] rows of A_i and
+ * columns of B_i count. ranks, ids: int32, scales: f32, device memory. in,
+ * out and r_pad multiples of 8, r_pad <= 128. workspace:
+ * qia_lora_workspace_bytes bytes of device memory, 16-byte aligned (NULL when
+ * that is 0). */
+int qia_lora_add(const void* x, const void* base, void* y, const void* a,
+                 const void* b, const void* ranks, const void* scales,
+                 const void* ids, int64_t batch, int64_t seq,
+                 int64_t in_features, int64_t out_features, int64_t adapters,
+                 int64_t r_pad, const int64_t* strides, void* workspace,
+                 void* stream);
+int64_t qia_lora_workspace_bytes(int64_t batch, int64_t seq, int64_t r_pad);
+
 /* Reads and clears the device-side error word of the current device (set when
  * a bounded wait inside a tensor-core kernel gave up). Synchronises the device. */
 int qia_device_error(int* code);

@@ -1,0 +1,71 @@
+// What the attention kernels over the INT8 prefix cache share: parameters, key
+// enumeration, and the per-key numbers of the softmax.
+//
+//   o_i = sum_j exp(c q_i.k_j) v_j / sum_j exp(c q_i.k_j)
+//
+// over the request's cached tokens j < lengths[b] (k_j = ks_j kc_j, v_j = vs_j
+// vc_j with INT8 codes kc, vc) and its fresh bf16 tokens, each only where
+// key_valid is set. A query with no key writes zeros.
+//
+// The codes are the tensor-core operands (every INT8 value is exact in bf16 and
+// f16), and both scales move into the exponent, so that a key costs one fused
+// multiply-add per score and masks cost nothing:
+//   t_ij = (c log2e ks_j) (q_i.kc_j) + log2 vs_j
+//   w_ij = 2^(t_ij - M_i)               the weight of the code vc_j
+//   o_i  = sum_j w_ij vc_j / sum_j w_ij / vs_j
+// A masked or missing key has (0, -inf, 0) for (c log2e ks, log2 vs, 1/vs) and
+// zero rows, so its w is exactly 0 whatever its memory holds.
+// M_i is a running maximum that may lag the true one by a bounded factor (the
+// weights then exceed 1, which both operand types hold), so the accumulators
+// are rescaled rarely.
+#pragma once
+
+#include "qia_common.cuh"
+
+namespace qia {
+
+constexpr int kCaD = 128;
+
+struct CachedAttn {
+  const __nv_bfloat16* q;       // [B, Sq, H, 128], strides (b, s, h)
+  const __nv_bfloat16* k;       // fresh rows [B, Sk, Hkv, 128]
+  const __nv_bfloat16* v;
+  __nv_bfloat16* out;           // [B, Sq, H, 128]
+  const int8_t* kc;             // [B, Hkv, capacity, 128]
+  const int8_t* vc;
+  const float* ks;              // [B, Hkv, capacity]
+  const float* vs;
+  const int* lengths;           // [B]
+  const uint8_t* key_valid;     // [B, extent + Sk], or null
+  int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh, mask_sb;
+  int sq, sk, heads, kv_heads, share, capacity, extent;   // share = heads / kv_heads
+  float scale_log2;             // c log2(e)
+};
+
+// Cached tokens of request b that the call may read.
+__device__ __forceinline__ int cached_len(const CachedAttn& p, int b) {
+  return max(0, min(__ldg(p.lengths + b), p.extent));
+}
+
+struct KeyScalars {
+  float sk, lsv, rsv;   // c log2e ks, log2 vs, 1 / vs
+};
+
+// vs below 2^-90 is taken as 2^-90: sums of w / vs then stay in range.
+__device__ __forceinline__ KeyScalars key_scalars(const CachedAttn& p, float ks, float vs, bool valid) {
+  KeyScalars r;
+  // a zero row (scale 0) has zero codes: any vs gives the same value
+  const float v = vs == 0.0f ? 1.0f : fmaxf(vs, 8.077935669e-28f);
+  r.sk = valid ? p.scale_log2 * ks : 0.0f;
+  r.lsv = valid ? (vs == vs ? log2f(v) : vs) : -INFINITY;
+  r.rsv = valid ? 1.0f / v : 0.0f;
+  return r;
+}
+
+__device__ __forceinline__ float ex2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace qia

@@ -1,0 +1,205 @@
+"""The INT8 prefix cache of one layer and the attention that reads it.
+
+The reference keeps the prefix's K/V in bf16 (QwenImage21KVLayerCache,
+transformer_qwenimage21.py:56-74). Here a cached row (one token of one head)
+is 128 INT8 codes and an fp32 scale: half the memory, and half the bytes an
+attention over it streams. `cached_attention` multiplies the codes as they are
+(they are exact in the tensor cores' 16-bit types) and applies the scales to
+the scores; `kv_cache_read` gives bf16 rows to an attention of another kind.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .. import _lib
+
+HEAD_DIM = 128
+_Strides6 = ctypes.c_int64 * 6
+_Strides12 = ctypes.c_int64 * 12
+
+
+class QuantizedKV:
+    """K and V of up to `capacity` tokens of each of `batch` requests.
+
+    k_codes, v_codes: int8 [batch, kv_heads, capacity, 128]; k_scales,
+    v_scales: float32 [batch, kv_heads, capacity]; lengths: int32 [batch] on
+    the device, the tokens each request holds. `extent` is the longest
+    request's length as the host knows it (the key columns of a mask); writes
+    through this class keep it up to date."""
+
+    def __init__(self, batch: int, kv_heads: int, capacity: int, device="cuda"):
+        dev = torch.device(device)
+        shape = (batch, kv_heads, capacity)
+        self._bind(torch.zeros(*shape, HEAD_DIM, dtype=torch.int8, device=dev),
+                   torch.zeros(*shape, HEAD_DIM, dtype=torch.int8, device=dev),
+                   torch.zeros(shape, dtype=torch.float32, device=dev),
+                   torch.zeros(shape, dtype=torch.float32, device=dev),
+                   torch.zeros(batch, dtype=torch.int32, device=dev),
+                   torch.zeros(batch, dtype=torch.int32, device=dev), 0, None)
+
+    @classmethod
+    def from_tensors(cls, k_codes, v_codes, k_scales, v_scales, lengths, extent: int) -> "QuantizedKV":
+        """A cache around tensors of the class's layout (contiguous); no
+        entry of `lengths` may exceed `extent`."""
+        self = cls.__new__(cls)
+        self._bind(k_codes, v_codes, k_scales, v_scales, lengths, torch.zeros_like(lengths), int(extent), None)
+        return self
+
+    def _bind(self, k_codes, v_codes, k_scales, v_scales, lengths, tickets, extent, parent):
+        _lib.require_cuda(k_codes, v_codes, k_scales, v_scales, lengths)
+        if k_codes.ndim != 4 or k_codes.shape[-1] != HEAD_DIM:
+            raise ValueError(f"QuantizedKV: codes must be [batch, kv_heads, capacity, 128], got {tuple(k_codes.shape)}")
+        batch, heads, capacity, _ = k_codes.shape
+        for t, shape, dtype in ((k_codes, k_codes.shape, torch.int8), (v_codes, k_codes.shape, torch.int8),
+                                (k_scales, k_codes.shape[:3], torch.float32),
+                                (v_scales, k_codes.shape[:3], torch.float32), (lengths, (batch,), torch.int32)):
+            if t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.device != k_codes.device:
+                raise ValueError(f"QuantizedKV: expected a contiguous {dtype} {tuple(shape)}, got {t.dtype} "
+                                 f"{tuple(t.shape)}")
+        if not 0 <= extent <= capacity:
+            raise ValueError(f"QuantizedKV: extent {extent} of capacity {capacity}")
+        self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
+        self.lengths, self._tickets, self._parent = lengths, tickets, parent
+        self.batch, self.kv_heads, self.capacity, self.extent = batch, heads, capacity, extent
+        self.device = k_codes.device
+        # the buffers' addresses, for the calls below
+        self._buffers = tuple(_lib.ptr(t) for t in (k_codes, v_codes, k_scales, v_scales, lengths))
+        self._ticket = _lib.ptr(tickets)
+
+    def select(self, first: int, count: int = 1) -> "QuantizedKV":
+        """Requests [first, first + count) of this cache, sharing its memory
+        (prefixes of different lengths are written one request at a time)."""
+        if first < 0 or count <= 0 or first + count > self.batch:
+            raise ValueError(f"QuantizedKV.select: requests {first}+{count} of {self.batch}")
+        part = QuantizedKV.__new__(QuantizedKV)
+        s = slice(first, first + count)
+        part._bind(self.k_codes[s], self.v_codes[s], self.k_scales[s], self.v_scales[s], self.lengths[s],
+                   self._tickets[s], self.extent, self)
+        return part
+
+    def _grow(self, extent: int, whole: bool) -> None:
+        """Record that requests hold up to `extent` tokens; `whole`: exactly so."""
+        self.extent = extent if whole else max(self.extent, extent)
+        if self._parent is not None:
+            self._parent._grow(extent, False)
+
+
+def _check_rows(who: str, cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> None:
+    _lib.require_cuda(k, v)
+    shape = k.shape
+    if k.ndim != 4 or shape[0] != cache.batch or shape[2] != cache.kv_heads or shape[3] != HEAD_DIM or v.shape != shape:
+        raise ValueError(f"{who}: k and v must be [{cache.batch}, seq, {cache.kv_heads}, {HEAD_DIM}], got "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.stride(3) != 1 or v.stride(3) != 1:
+        raise NotImplementedError(f"{who}: k and v must be bf16 with contiguous rows")
+    if k.device != cache.device or v.device != cache.device:
+        raise ValueError(f"{who}: k, v and the cache are on different devices")
+
+
+def kv_cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, start: int = 0) -> None:
+    """Quantise k, v [batch, seq, kv_heads, 128] bf16 (any strides that are
+    multiples of 8, rows contiguous) into tokens [start, start + seq) of every
+    request, which then holds start + seq tokens."""
+    _check_rows("kv_cache_write", cache, k, v)
+    seq = k.shape[1]
+    if start < 0 or start + seq > cache.capacity:
+        raise ValueError(f"kv_cache_write: tokens {start}+{seq} of capacity {cache.capacity}")
+    _write(cache, k, v, seq, start)
+    cache._grow(start + seq, True)
+
+
+def kv_cache_append(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> None:
+    """kv_cache_write behind the tokens that each request holds (lengths read
+    on the device, so a captured append replays)."""
+    _check_rows("kv_cache_append", cache, k, v)
+    seq = k.shape[1]
+    if cache.extent + seq > cache.capacity:
+        raise ValueError(f"kv_cache_append: {seq} tokens behind {cache.extent} of capacity {cache.capacity}")
+    _write(cache, k, v, seq, -1)
+    cache._grow(cache.extent + seq, False)
+
+
+def _write(cache, k, v, seq, start):
+    kc, vc, ks, vs, lengths = cache._buffers
+    _lib.call("qia_kv_cache_write", k.data_ptr(), v.data_ptr(), kc, vc, ks, vs, lengths, cache.batch, seq,
+              cache.kv_heads, HEAD_DIM, cache.capacity, start, _Strides6(*k.stride()[:3], *v.stride()[:3]),
+              cache._ticket, _lib.stream(cache.device))
+
+
+def kv_cache_read(cache: QuantizedKV, first: int = 0, tokens: int | None = None, out_k: torch.Tensor | None = None,
+                  out_v: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cached tokens [first, first + tokens) (default: up to the extent) as
+    bf16 rows [batch, tokens, kv_heads, 128], into out_k / out_v when given
+    (e.g. the head of a joint K/V buffer); rows past a request's length are
+    zeros."""
+    if tokens is None:
+        tokens = cache.extent - first
+    if first < 0 or tokens < 0 or first + tokens > cache.capacity:
+        raise ValueError(f"kv_cache_read: tokens {first}+{tokens} of capacity {cache.capacity}")
+    shape = (cache.batch, tokens, cache.kv_heads, HEAD_DIM)
+    if out_k is None:
+        out_k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+    if out_v is None:
+        out_v = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+    _check_rows("kv_cache_read", cache, out_k, out_v)
+    if out_k.shape != shape:
+        raise ValueError(f"kv_cache_read: the outputs must be {shape}, got {tuple(out_k.shape)}")
+    _lib.call("qia_kv_cache_read", *cache._buffers, out_k.data_ptr(), out_v.data_ptr(), cache.batch, first, tokens,
+              cache.kv_heads, HEAD_DIM, cache.capacity, _Strides6(*out_k.stride()[:3], *out_v.stride()[:3]),
+              _lib.stream(cache.device))
+    return out_k, out_v
+
+
+def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None = None,
+                     v: torch.Tensor | None = None, key_valid: torch.Tensor | None = None,
+                     scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(scale q K^T) V over [cached prefix, fresh k / v], unmasked but
+    for key_valid.
+
+    q: bf16 [batch, seq, heads, 128], heads a multiple of the cache's K/V
+    heads (query head h reads K/V head h // (heads // kv_heads)); k, v: bf16
+    [batch, fresh, kv_heads, 128] or None; key_valid: bool [batch, cache.extent
+    + fresh], False where a key takes no part (whatever it holds). Cached
+    tokens past a request's length never take part. A query without any key
+    gives zeros. scale defaults to 1/sqrt(128). Returns bf16 like q."""
+    who = "cached_attention"
+    _lib.require_cuda(q, key_valid)
+    if q.ndim != 4 or q.shape[0] != cache.batch or q.shape[3] != HEAD_DIM or q.shape[2] % cache.kv_heads:
+        raise ValueError(f"{who}: q must be [{cache.batch}, seq, a multiple of {cache.kv_heads}, {HEAD_DIM}], got "
+                         f"{tuple(q.shape)}")
+    if q.dtype != torch.bfloat16 or q.stride(3) != 1:
+        raise NotImplementedError(f"{who}: q must be bf16 with contiguous rows")
+    if q.device != cache.device:
+        raise ValueError(f"{who}: q and the cache are on different devices")
+    if scale is not None and not scale > 0:
+        raise ValueError(f"{who}: scale={scale} must be positive")
+    if (k is None) != (v is None):
+        raise ValueError(f"{who}: k and v come together")
+    fresh = 0
+    if k is not None:
+        _check_rows(who, cache, k, v)
+        fresh = k.shape[1]
+    mask_stride = 0
+    if key_valid is not None:
+        if key_valid.shape != (cache.batch, cache.extent + fresh) or key_valid.dtype != torch.bool:
+            raise ValueError(f"{who}: key_valid must be bool [{cache.batch}, {cache.extent + fresh}], got "
+                             f"{key_valid.dtype} {tuple(key_valid.shape)}")
+        if key_valid.stride(1) != 1 or key_valid.device != cache.device:
+            raise NotImplementedError(f"{who}: key_valid must have contiguous rows on the cache's device")
+        mask_stride = key_valid.stride(0)
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    elif (out.shape != q.shape or out.dtype != torch.bfloat16 or out.stride(3) != 1 or out.device != q.device):
+        raise ValueError(f"{who}: out must be like q")
+    if not out.numel():
+        return out
+    kc, vc, ks, vs, lengths = cache._buffers
+    rows = (*k.stride()[:3], *v.stride()[:3]) if fresh else (0,) * 6
+    _lib.call("qia_cached_attention", q.data_ptr(), k.data_ptr() if fresh else None, v.data_ptr() if fresh else None,
+              kc, vc, ks, vs, lengths, None if key_valid is None else key_valid.data_ptr(), out.data_ptr(),
+              cache.batch, q.shape[1], fresh, q.shape[2], cache.kv_heads, HEAD_DIM, cache.capacity, cache.extent,
+              _Strides12(*q.stride()[:3], *rows, *out.stride()[:3]), mask_stride,
+              0.0 if scale is None else float(scale), _lib.stream(q.device))
+    return out
