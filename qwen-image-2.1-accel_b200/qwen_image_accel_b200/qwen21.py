@@ -29,6 +29,11 @@ epilogue, the gated residuals from the output-projection GEMM epilogues, and
 the gate/value projections as one grouped launch -- each byte-identical to
 the unfused op sequence it replaces.
 
+For serving, a QuantizedKVLayerCache keeps the prefix in INT8 (the bf16
+attention then reads the codes directly, the Sage attention gets them back as
+bf16 rows), and a block with adapters adds each request's low-rank update to
+the outputs of the linears it names (kernels/lora.py), in both modes.
+
 As in the reference (quantize_transformer swaps the linears, the MLP forward
 is replaced for both modes), the prefill uses the same MXFP8 linears and MLP;
 its attention is the reference's per-segment SDPA by default, or, with
@@ -49,7 +54,9 @@ from .kernels.attention import joint_qk_norm_rope
 from .kernels.bf16 import swiglu
 from .kernels.elementwise import residual
 from .kernels.epilogue import layer_norm_scale_quantize, swiglu_quantize
+from .kernels.kv_cache import QuantizedKV, cached_attention, kv_cache_read, kv_cache_write
 from .kernels.layernorm import layer_norm_scale
+from .kernels.lora import LoraWeights, lora_add
 from .kernels.mxfp8 import quantize
 from .optimizations.mxfp8 import MXFP8Linear, matmul_grouped
 from .optimizations.prefill import prefill_attention, segment_prefill_sdpa
@@ -94,13 +101,36 @@ class KVLayerCache:
         return self.k, self.v
 
 
+class QuantizedKVLayerCache:
+    """KVLayerCache in INT8: a prefix is quantised as it is stored and takes
+    half the memory. `quantized` is the cache that the attention reads; get()
+    reads bf16 rows back for anything else."""
+
+    def __init__(self):
+        self.quantized: QuantizedKV | None = None
+
+    def store(self, k: torch.Tensor, v: torch.Tensor):
+        b, n, h, _ = k.shape
+        c = self.quantized
+        if c is None or c.batch != b or c.kv_heads != h or c.capacity < n or c.device != k.device:
+            c = self.quantized = QuantizedKV(b, h, n, device=k.device)
+        kv_cache_write(c, k, v)
+
+    def get(self) -> tuple[torch.Tensor, torch.Tensor]:
+        if self.quantized is None:
+            raise RuntimeError("KV cache has not been populated yet.")
+        return kv_cache_read(self.quantized)
+
+
 class KVCache:
-    """One KVLayerCache per block (QwenImage21KVCache, :77-84)."""
+    """One KVLayerCache per block (QwenImage21KVCache, :77-84), or, with
+    quantized=True, one QuantizedKVLayerCache."""
 
-    def __init__(self, num_layers: int):
-        self.layer_caches = [KVLayerCache() for _ in range(num_layers)]
+    def __init__(self, num_layers: int, quantized: bool = False):
+        layer = QuantizedKVLayerCache if quantized else KVLayerCache
+        self.layer_caches = [layer() for _ in range(num_layers)]
 
-    def get_layer(self, layer_idx: int) -> KVLayerCache:
+    def get_layer(self, layer_idx: int) -> KVLayerCache | QuantizedKVLayerCache:
         return self.layer_caches[layer_idx]
 
 
@@ -189,6 +219,25 @@ class Block21:
         self.out_mx = isinstance(to_out, MXFP8Linear)
         self.gv_mx = isinstance(self.gate_layer, MXFP8Linear) and isinstance(self.proj, MXFP8Linear)
         self.down_mx = isinstance(self.out, MXFP8Linear)
+        self.adapters: dict[str, LoraWeights] = {}
+
+    ADAPTED = ("attn.to_q", "attn.to_k", "attn.to_v", "attn.to_out.0", "img_mlp.gate_layer", "img_mlp.proj",
+               "img_mlp.out")
+
+    def set_adapters(self, adapters: dict[str, LoraWeights]) -> None:
+        """Low-rank adapters by the name of the linear they sit beside (a
+        subset of ADAPTED); forward_cached and forward_prefill apply those that
+        their adapter_ids name, one per sample."""
+        unknown = set(adapters) - set(self.ADAPTED)
+        if unknown:
+            raise ValueError(f"adapters for unknown linears: {sorted(unknown)}")
+        self.adapters = dict(adapters)
+
+    def _adapt(self, name: str, x: torch.Tensor, y: torch.Tensor, ids: torch.Tensor | None) -> None:
+        """Add the requests' adapters of linear `name`, applied to x [B, S, in],
+        to its output y [B, S, out] in place."""
+        if ids is not None and name in self.adapters:
+            lora_add(x, y, self.adapters[name], ids, out=y)
 
     @property
     def quantized(self) -> bool:
@@ -215,14 +264,18 @@ class Block21:
             return lin.matmul(x)
         return F.linear(x, lin.weight)
 
-    def _qkv_into(self, x, b, s, freqs, oq, ok, ov, offset):
+    def _qkv_into(self, x, b, s, freqs, oq, ok, ov, offset, ids=None):
         """q|k|v projection of the LN output x (bf16 tensor, or MXFP8 Quantized
-        when the projections are MXFP8) for s tokens per sample, RMS-normalised
-        and rotated into rows [offset, offset + s) of the joint NHD buffers."""
+        when the projections are MXFP8 and nothing is adapted) for s tokens per
+        sample, RMS-normalised and rotated into rows [offset, offset + s) of the
+        joint NHD buffers."""
         if isinstance(self.qkv, tuple):
             qkv = torch.cat([self._apply(p, x).view(b, s, -1) for p in self.qkv], dim=-1)
         else:
             qkv = self._apply(self.qkv, x).view(b, s, -1)
+        if ids is not None:
+            for name, y in zip(("attn.to_q", "attn.to_k", "attn.to_v"), qkv.chunk(3, dim=-1)):
+                self._adapt(name, x, y, ids)
         joint_qk_norm_rope(qkv, self.norm_q.weight, self.norm_k.weight, torch.view_as_real(freqs).contiguous(),
                            oq, ok, ov, offset, eps=self.cfg.eps)
 
@@ -230,8 +283,11 @@ class Block21:
         shape = (b, total, self.cfg.heads, self.cfg.head_dim)
         return tuple(torch.empty(shape, device=device, dtype=torch.bfloat16) for _ in range(3))
 
-    def _out_proj(self, attn):
-        return self._apply(self.to_out, attn.flatten(2, 3).contiguous()).view(*attn.shape[:2], -1)
+    def _out_proj(self, attn, ids=None):
+        x = attn.flatten(2, 3).contiguous()
+        y = self._apply(self.to_out, x).view(*attn.shape[:2], -1)
+        self._adapt("attn.to_out.0", x, y, ids)
+        return y
 
     def _swiglu_act(self, x):
         """MXFP8 SwiGLU activation of the MLP (gate, value and down projections
@@ -251,9 +307,17 @@ class Block21:
             return matmul_grouped([(self.gate_layer, a), (self.proj, a)])
         return self._apply(self.gate_layer, x), self._apply(self.proj, x)
 
-    def _mlp(self, x, lead):
+    def _mlp(self, x, lead, ids=None):
         """SwiGLU MLP; x is the LN output (bf16, or its MXFP8 quantization when
-        the gate and value projections are MXFP8)."""
+        the gate and value projections are MXFP8 and nothing is adapted)."""
+        if ids is not None:
+            gate, value = (t.view(*lead, -1) for t in self._gate_value(x))
+            self._adapt("img_mlp.gate_layer", x, gate, ids)
+            self._adapt("img_mlp.proj", x, value, ids)
+            act = swiglu(gate.contiguous(), value.contiguous())
+            y = self._apply(self.out, act).view(*lead, -1)
+            self._adapt("img_mlp.out", act, y, ids)
+            return y
         if self.gv_mx and self.down_mx:
             return self.out.matmul(self._swiglu_act(x)).view(*lead, -1)
         gate, value = self._gate_value(x)
@@ -284,39 +348,77 @@ class Block21:
         return out
 
     # ------------------------------------------------------------------ modes
-    def forward_cached(self, h: torch.Tensor, values, freqs: torch.Tensor, layer_cache: KVLayerCache,
-                       key_valid: torch.Tensor | None = None) -> torch.Tensor:
+    def _joint_with_prefix(self, layer_cache, b: int, st: int, device):
+        """Joint q/k/v buffers of p + st tokens with the cached prefix's K/V in
+        rows [0, p), and p."""
+        if isinstance(layer_cache, QuantizedKVLayerCache):
+            cache = layer_cache.quantized
+            if cache is None:
+                raise RuntimeError("KV cache has not been populated yet.")
+            p, batch = cache.extent, cache.batch
+        else:
+            cached_k, cached_v = layer_cache.get()
+            p, batch = cached_k.shape[1], cached_k.shape[0]
+            if cached_v.shape != cached_k.shape:
+                raise ValueError("cached decode: the cache does not match the batch")
+        if batch != b:
+            raise ValueError("cached decode: the cache does not match the batch")
+        oq, ok, ov = self._joint(b, p + st, device)
+        if isinstance(layer_cache, QuantizedKVLayerCache):
+            kv_cache_read(cache, out_k=ok[:, :p], out_v=ov[:, :p])
+        else:
+            ok[:, :p].copy_(cached_k)
+            ov[:, :p].copy_(cached_v)
+        return p, oq, ok, ov
+
+    def _attend_quantized(self, x, b, st, freqs, cache: QuantizedKV | None, key_valid, ids=None):
+        """bf16 attention of the target tokens (LN output x) over [INT8 prefix,
+        target], without a joint K/V copy."""
+        if cache is None:
+            raise RuntimeError("KV cache has not been populated yet.")
+        if cache.batch != b:
+            raise ValueError("cached decode: the cache does not match the batch")
+        q, k, v = self._joint(b, st, freqs.device)
+        self._qkv_into(x, b, st, freqs, q, k, v, 0, ids)
+        return cached_attention(q, cache, k, v, key_valid=key_valid)
+
+    def forward_cached(self, h: torch.Tensor, values, freqs: torch.Tensor,
+                       layer_cache: KVLayerCache | QuantizedKVLayerCache, key_valid: torch.Tensor | None = None,
+                       adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
         """Cached decode of the target tokens h [B, St, D]; values =
         modulation_values(modulation); freqs complex64 [St, 64] (the target's
-        rows of the RoPE table); key_valid bool [B, prefix + St] or None."""
+        rows of the RoPE table); key_valid bool [B, prefix + St] or None;
+        adapter_ids int32 [B] (-1: none) or None."""
         s1, g1, s2, g2 = values
         b, st, _ = h.shape
         h = h.contiguous()
-        cached_k, cached_v = layer_cache.get()
-        p = cached_k.shape[1]
-        if cached_k.shape[0] != b or cached_v.shape != cached_k.shape:
-            raise ValueError("cached decode: the cache does not match the batch")
-        oq, ok, ov = self._joint(b, p + st, h.device)
-        ok[:, :p].copy_(cached_k)
-        ov[:, :p].copy_(cached_v)
-        self._qkv_into(self._normalized(h, s1, self.qkv_mx), b, st, freqs, oq, ok, ov, p)
-        q = oq[:, p:]
-        if self.sage and key_valid is None and self.out_mx:
-            h = self.to_out.matmul_gate_residual(sage_attention_quantized(q, ok, ov), g1, h)
+        ids = adapter_ids if self.adapters else None
+        sage = self.sage and key_valid is None
+        # adapters multiply the bf16 activation: the LN output then stays bf16
+        x = self._normalized(h, s1, self.qkv_mx and ids is None)
+        if isinstance(layer_cache, QuantizedKVLayerCache) and not sage:
+            attn = self._attend_quantized(x, b, st, freqs, layer_cache.quantized, key_valid, ids)
+            h = residual(h, self._out_proj(attn, ids).contiguous(), g1)
         else:
-            if self.sage and key_valid is None:
-                attn = sage_attention(q, ok, ov)
+            p, oq, ok, ov = self._joint_with_prefix(layer_cache, b, st, h.device)
+            self._qkv_into(x, b, st, freqs, oq, ok, ov, p, ids)
+            q = oq[:, p:]
+            if sage and self.out_mx and ids is None:
+                h = self.to_out.matmul_gate_residual(sage_attention_quantized(q, ok, ov), g1, h)
             else:
-                mask = None if key_valid is None else key_valid[:, None, None, :]
-                attn = F.scaled_dot_product_attention(q.transpose(1, 2), ok.transpose(1, 2), ov.transpose(1, 2),
-                                                      attn_mask=mask).transpose(1, 2)
-            h = residual(h, self._out_proj(attn).contiguous(), g1)
-        x = self._normalized(h, s2, self.gv_mx)
-        if self.gv_mx and self.down_mx:
+                if sage:
+                    attn = sage_attention(q, ok, ov)
+                else:
+                    mask = None if key_valid is None else key_valid[:, None, None, :]
+                    attn = F.scaled_dot_product_attention(q.transpose(1, 2), ok.transpose(1, 2), ov.transpose(1, 2),
+                                                          attn_mask=mask).transpose(1, 2)
+                h = residual(h, self._out_proj(attn, ids).contiguous(), g1)
+        x = self._normalized(h, s2, self.gv_mx and ids is None)
+        if self.gv_mx and self.down_mx and ids is None:
             return self.out.matmul_gate_residual(self._swiglu_act(x), g2, h)
-        return residual(h, self._mlp(x, (b, st)).contiguous(), g2)
+        return residual(h, self._mlp(x, (b, st), ids).contiguous(), g2)
 
-    def attention_cached(self, x, freqs: torch.Tensor, layer_cache: KVLayerCache,
+    def attention_cached(self, x, freqs: torch.Tensor, layer_cache: KVLayerCache | QuantizedKVLayerCache,
                          key_valid: torch.Tensor | None = None) -> torch.Tensor:
         """The attention half of the cached decode on an already modulated
         input x [B, St, D] bf16: Q/K/V projections, QK-RMSNorm + RoPE behind the
@@ -324,11 +426,10 @@ class Block21:
         has it and nothing is masked, else SDPA), output projection -> bf16
         [B, St, D]."""
         b, st, _ = x.shape
-        cached_k, cached_v = layer_cache.get()
-        p = cached_k.shape[1]
-        oq, ok, ov = self._joint(b, p + st, x.device)
-        ok[:, :p].copy_(cached_k)
-        ov[:, :p].copy_(cached_v)
+        if isinstance(layer_cache, QuantizedKVLayerCache) and not (self.sage and key_valid is None):
+            return self._out_proj(self._attend_quantized(x.contiguous(), b, st, freqs, layer_cache.quantized,
+                                                         key_valid))
+        p, oq, ok, ov = self._joint_with_prefix(layer_cache, b, st, x.device)
         self._qkv_into(x.contiguous(), b, st, freqs, oq, ok, ov, p)
         q = oq[:, p:]
         if self.sage and key_valid is None:
@@ -340,26 +441,32 @@ class Block21:
         return self._out_proj(attn)
 
     def forward_prefill(self, h: torch.Tensor, modulation: torch.Tensor, freqs: torch.Tensor,
-                        image_ids: torch.Tensor, prefix_len: int, layer_cache: KVLayerCache | None = None,
-                        key_valid: torch.Tensor | None = None) -> torch.Tensor:
+                        image_ids: torch.Tensor, prefix_len: int,
+                        layer_cache: KVLayerCache | QuantizedKVLayerCache | None = None,
+                        key_valid: torch.Tensor | None = None,
+                        adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
         """Prefill of the joint sequence h [B, S, D] (target image = the last
         S - prefix_len tokens); modulation [B + 1, 4D]; freqs complex64
         [S, 64]; image_ids int [S] (-1 at text tokens). Stores the prefix's
-        post-RoPE K/V in layer_cache when given (kv_cache_mode="extract")."""
+        post-RoPE K/V in layer_cache when given (kv_cache_mode="extract").
+        adapter_ids as in forward_cached."""
         b, s, _ = h.shape
         h = h.contiguous()
+        ids = adapter_ids if self.adapters else None
         s1, g1, s2, g2 = modulation.chunk(4, dim=-1)
         one_s1, tanh_g1, one_s2, tanh_g2 = ((1 + s1).contiguous(), g1.tanh().contiguous(),
                                             (1 + s2).contiguous(), g2.tanh().contiguous())
         x = self._rows("ln", h, one_s1, prefix_len)
         q, k, v = self._joint(b, s, h.device)
-        self._qkv_into(x, b, s, freqs, q, k, v, 0)
-        if layer_cache is not None:
+        self._qkv_into(x, b, s, freqs, q, k, v, 0, ids)
+        if isinstance(layer_cache, QuantizedKVLayerCache):
+            layer_cache.store(k[:, :prefix_len], v[:, :prefix_len])
+        elif layer_cache is not None:
             layer_cache.store(k[:, :prefix_len].clone(), v[:, :prefix_len].clone())
         if self.sage_prefill:
             attn = prefill_attention(q, k, v, image_ids, key_valid=key_valid)
         else:
             attn = segment_prefill_sdpa(q, k, v, image_ids, prefix_len, key_valid=key_valid)
-        h = self._rows("res", h, tanh_g1, prefix_len, other=self._out_proj(attn).contiguous())
+        h = self._rows("res", h, tanh_g1, prefix_len, other=self._out_proj(attn, ids).contiguous())
         x = self._rows("ln", h, one_s2, prefix_len)
-        return self._rows("res", h, tanh_g2, prefix_len, other=self._mlp(x, (b, s)).contiguous())
+        return self._rows("res", h, tanh_g2, prefix_len, other=self._mlp(x, (b, s), ids).contiguous())

@@ -25,6 +25,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from .kernels.layernorm import layer_norm_scale
+from .kernels.lora import LoraWeights
 from .optimizations.mxfp8 import skip_block_indices
 from .profiles import get_profile
 from .qwen21 import Block21, Block21Config, KVCache, _Norm, block21_parameter_shapes, modulation_values
@@ -170,6 +171,29 @@ class Qwen21Transformer:
         # QwenImage21TemporalTimesteps(256): frequencies built once in fp32 on the CPU
         self.t_freqs = torch.exp(-math.log(10000) * torch.arange(0, 128, dtype=torch.float32) / 128).to(dev)
 
+    # ---------------------------------------------------------------- adapters
+    def load_adapters(self, adapters) -> None:
+        """Keep low-rank adapters for requests to choose from: each a mapping
+        "transformer_blocks.{i}.{linear}" -> (A [rank, in], B [out, rank],
+        scale) over any of the blocks' linears (Block21.ADAPTED). forward's
+        adapter_ids number them in this order. An adapter that leaves a linear
+        out does nothing there; an empty list removes them all."""
+        known = {f"transformer_blocks.{i}.{n}" for i in range(len(self.blocks)) for n in Block21.ADAPTED}
+        for ad in adapters:
+            if set(ad) - known:
+                raise ValueError(f"adapters for unknown linears: {sorted(set(ad) - known)}")
+        dev = self.t_freqs.device
+        for i, blk in enumerate(self.blocks):
+            per = {}
+            for n in Block21.ADAPTED:
+                held = [ad.get(f"transformer_blocks.{i}.{n}") for ad in adapters]
+                some = next((h for h in held if h is not None), None)
+                if some is None:
+                    continue
+                none = (torch.zeros(1, some[0].shape[1]), torch.zeros(some[1].shape[0], 1), 0.0)
+                per[n] = LoraWeights([none if h is None else h for h in held], device=dev)
+            blk.set_adapters(per)
+
     # ---------------------------------------------------------------- embedders
     def time_embed(self, t: torch.Tensor) -> torch.Tensor:
         """QwenImage21TimestepProjEmbeddings: [cos | sin](1000 t * freqs) in
@@ -214,10 +238,13 @@ class Qwen21Transformer:
     # ---------------------------------------------------------------- forward
     def forward(self, hidden_states: torch.Tensor, encoder_hidden_states: torch.Tensor, timestep: torch.Tensor,
                 img_shapes, img_mask: torch.Tensor, encoder_hidden_states_mask: torch.Tensor | None = None,
-                kv_cache: KVCache | None = None, kv_cache_mode: str | None = None) -> torch.Tensor:
+                kv_cache: KVCache | None = None, kv_cache_mode: str | None = None,
+                adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
         """Same arguments and result as QwenImage21Transformer2DModel.forward
         (return_dict=False, first element): the prefill returns the whole
-        joint sequence's output, the cached decode the target tokens'."""
+        joint sequence's output, the cached decode the target tokens'. kv_cache
+        may be a quantized one; adapter_ids int32 [B] names each sample's
+        adapter of load_adapters (-1: none)."""
         _lib.require_cuda(hidden_states, encoder_hidden_states)
         if kv_cache is not None and kv_cache_mode not in ("extract", "cached"):
             raise ValueError(f"kv_cache_mode must be 'extract' or 'cached' when kv_cache is provided, "
@@ -251,14 +278,15 @@ class Qwen21Transformer:
             vals = modulation_values(modulation)
             freqs = rope[prefix_len:].contiguous()
             for i, blk in enumerate(self.blocks):
-                h = blk.forward_cached(h, vals, freqs, kv_cache.get_layer(i), key_valid=key_valid)
+                h = blk.forward_cached(h, vals, freqs, kv_cache.get_layer(i), key_valid=key_valid,
+                                       adapter_ids=adapter_ids)
             y = layer_norm_scale(h, (1 + scale[:-1])[:, None].contiguous(), self.ln)
         else:
             h = joint.contiguous()
             for i, blk in enumerate(self.blocks):
                 cache = kv_cache.get_layer(i) if kv_cache_mode == "extract" else None
                 h = blk.forward_prefill(h, modulation, rope, image_ids, prefix_len, layer_cache=cache,
-                                        key_valid=key_valid)
+                                        key_valid=key_valid, adapter_ids=adapter_ids)
             # prefix rows scale from the t = 0 row, target rows from their sample's row
             y = self.blocks[0]._rows("ln", h, (1 + scale).contiguous(), prefix_len)
         return F.linear(y, self.w["proj_out.weight"])
