@@ -508,5 +508,7 @@ extern "C" int qia_cached_attention(const void* q, const void* k, const void* v,
   p.capacity = int(capacity);
   p.extent = int(extent);
   p.scale_log2 = (sm_scale > 0.0f ? sm_scale : 0.08838834764831845f) * 1.4426950408889634f;
-  return launch_cached_rows(p, int(batch), as_stream(stream));
+  // rows that share a K/V head fill one 16-row tile, or the tensor-core tiles
+  if (seq_q * p.share <= 16) return launch_cached_rows(p, int(batch), as_stream(stream));
+  return launch_cached_tiles(p, int(batch), as_stream(stream));
 }

@@ -62,6 +62,9 @@ __device__ __forceinline__ KeyScalars key_scalars(const CachedAttn& p, float ks,
   return r;
 }
 
+int launch_cached_rows(const CachedAttn& p, int batch, cudaStream_t st);    // few query rows (cached_attn.cu)
+int launch_cached_tiles(const CachedAttn& p, int batch, cudaStream_t st);   // many (cached_attn_tiles.cu)
+
 __device__ __forceinline__ float ex2_ftz(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
