@@ -629,8 +629,8 @@ int qia_cached_attention(const void* q, const void* k, const void* v,
  * the device error word as QIA_ERR_INVALID). x [batch, seq, in], base and y
  * [batch, seq, out] bf16 (y may be base), strides: elements, (batch, seq) of
  * x, base, y, multiples of 8, rows contiguous. a: bf16 [adapters, r_pad, in],
- * b: bf16 [adapters, out, r_pad]; only the first ranks[i] rows of A_i and
- * columns of B_i count. ranks, ids: int32, scales: f32, device memory. in,
+ * b: bf16 [adapters, out, r_pad]; rows of A_i and columns of B_i past
+ * ranks[i] hold zeros. ranks, ids: int32, scales: f32, device memory. in,
  * out and r_pad multiples of 8, r_pad <= 128. workspace:
  * qia_lora_workspace_bytes bytes of device memory, 16-byte aligned (NULL when
  * that is 0). */
