@@ -4,9 +4,11 @@
 // cached_attn_rows_kernel: a tile of 16 query rows (token-major over the heads
 // that share a K/V head) against a slice of the keys. What bounds it is the
 // cache's bytes (one per element), so everything is arranged around streaming
-// them once: the codes go from global memory straight into the registers of
-// the warp that multiplies them, with no shared-memory pass, by giving each
-// thread contiguous bytes and permuting the contraction instead:
+// them once: every warp keeps a ring of kRowsRing 16-key steps (4 KB of codes
+// each) in flight with cp.async into shared memory of its own -- no barrier
+// between warps -- and reads 16-byte pieces back with no bank conflicts (piece
+// p of row r is stored at p ^ (r & 7)). Each thread takes contiguous bytes and
+// the contraction is permuted instead:
 //   * q.k: thread c = lane % 4 holds channels [32c, 32c + 32) of key lane / 4,
 //     and step j of the eight m16n8k16 products takes channels 32c + 4j .. + 3
 //     of every c (the query fragments are loaded in the same order);
@@ -31,15 +33,22 @@ namespace {
 constexpr int kRowsWarps = 4;
 constexpr int kRowsTile = 16;          // query rows per CTA
 constexpr int kRowsStep = 16;          // keys per warp step
+constexpr int kRowsRing = 4;           // steps in flight per warp
+constexpr int kRowsCodes = 2 * kRowsStep * kCaD;            // K, then V codes of a step
+constexpr int kRowsStage = kRowsCodes + 2 * kRowsStep * 4;  // and their scales
 // f16 weights: w = 2^(t - M + 8) <= 2^15 while t <= M + 7, so the accumulators
 // are rescaled only when a score passes its maximum by more than 7.
 constexpr float kRowsBias = 8.0f, kRowsLag = 7.0f;
 
-struct RowsSmem {
+// The rings are done when the joining begins.
+union RowsSmem {
+  uint8_t ring[kRowsWarps][kRowsRing][kRowsStage];
+  struct {
   float o[kRowsWarps][kRowsTile][kCaD + 4];
   float m[kRowsWarps][kRowsTile], l[kRowsWarps][kRowsTile];
   float om[kRowsTile][kCaD + 4];        // the CTA's joined rows, read by the cluster
   float mm[kRowsTile], lm[kRowsTile];
+  };
 };
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
@@ -69,12 +78,18 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint4 ldg_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+__device__ __forceinline__ void cp_async16(void* smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(smem))), "l"(gmem)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(uint32_t(__cvta_generic_to_shared(smem))), "l"(gmem)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // 2^e with max|x| in [2^e, 2^(e+1)), e clamped to [-90, 126], and its inverse:
@@ -93,13 +108,6 @@ __device__ __forceinline__ uint32_t absmax8(const uint4& v, uint32_t m) {
   return m;
 }
 
-// A step's operands: the K codes of two 8-key groups and the V codes of the
-// thread's four keys.
-struct StepCodes {
-  uint4 k[2][2];
-  uint4 v[4];
-};
-
 __global__ void __launch_bounds__(kRowsWarps * 32, 3) cached_attn_rows_kernel(const __grid_constant__ CachedAttn p) {
   extern __shared__ __align__(16) uint8_t rows_smem[];
   RowsSmem& sm = *reinterpret_cast<RowsSmem*>(rows_smem);
@@ -113,6 +121,41 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 3) cached_attn_rows_kernel(co
   const int steps = cached_steps + (p.sk + kRowsStep - 1) / kRowsStep;
   const int per = (steps + splits - 1) / splits;
   const int step_end = min(steps, (split + 1) * per);
+
+  const int64_t head_row = (int64_t(b) * p.kv_heads + kvh) * p.capacity;
+  const int8_t* kc = p.kc + head_row * kCaD;
+  const int8_t* vc = p.vc + head_row * kCaD;
+  const uint8_t* mask = p.key_valid ? p.key_valid + b * p.mask_sb : nullptr;
+  // key of this thread's V row i (of four), and of its score columns
+  const auto vkey = [&](int i) { return 2 * c + (i & 1) + (i >> 1) * 8; };
+
+  // ---- the warp's ring of cached steps: step0, step0 + kRowsWarps, ...
+  const int cached_end = min(step_end, cached_steps);
+  const int step0 = split * per + warp;
+  const int mine_n = step0 < cached_end ? (cached_end - step0 + kRowsWarps - 1) / kRowsWarps : 0;
+  const auto issue = [&](int i) {
+    if (i < mine_n) {
+      uint8_t* st = sm.ring[warp][i % kRowsRing];
+      const int k0 = (step0 + i * kRowsWarps) * kRowsStep;
+      // (keys past the length: any held row, weight 0)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int row = r4 * 4 + (lane >> 3), piece = lane & 7, at = row * kCaD + ((piece ^ (row & 7)) << 4);
+        const int64_t src = int64_t(min(k0 + row, len - 1)) * kCaD + piece * 16;
+        cp_async16(st + at, kc + src);
+        cp_async16(st + kRowsCodes / 2 + at, vc + src);
+      }
+      cp_async4(st + kRowsCodes + lane * 4, (lane < 16 ? p.ks : p.vs) + head_row + min(k0 + (lane & 15), len - 1));
+    }
+    cp_async_commit();      // (an empty group keeps the count)
+  };
+  const auto mask_of = [&](int i) {   // of key lane % 16 of step i
+    const int key = (step0 + i * kRowsWarps) * kRowsStep + (lane & 15);
+    return i < mine_n && key < len && (!mask || __ldg(mask + key) != 0);
+  };
+#pragma unroll
+  for (int i = 0; i < kRowsRing - 1; ++i) issue(i);
+  bool valid = mask_of(0);
 
   // ---- query fragments, normalised per row by a power of two (f16 operands)
   uint32_t qa[8][4];
@@ -154,35 +197,6 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 3) cached_attn_rows_kernel(co
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[t][e] = 0.0f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-
-  const int64_t head_row = (int64_t(b) * p.kv_heads + kvh) * p.capacity;
-  const int8_t* kc = p.kc + head_row * kCaD;
-  const int8_t* vc = p.vc + head_row * kCaD;
-  const uint8_t* mask = p.key_valid ? p.key_valid + b * p.mask_sb : nullptr;
-
-  // key of this thread's V row i (of four), and of its score columns
-  const auto vkey = [&](int i) { return 2 * c + (i & 1) + (i >> 1) * 8; };
-  const auto load_codes = [&](int step, StepCodes& s) {
-    const int k0 = step * kRowsStep;
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      const int key = min(k0 + nt * 8 + g, len - 1);      // (rows past the length: any held row, weight 0)
-      const uint4* src = reinterpret_cast<const uint4*>(kc + int64_t(key) * kCaD + 32 * c);
-      s.k[nt][0] = ldg_stream(src);
-      s.k[nt][1] = ldg_stream(src + 1);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      s.v[i] = ldg_stream(vc + int64_t(min(k0 + vkey(i), len - 1)) * kCaD + 16 * g);
-  };
-  // scalars of key lane % 16 of a cached step
-  const auto load_scalars = [&](int step, float& ks, float& vs, bool& valid) {
-    const int key = step * kRowsStep + (lane & 15);
-    valid = key < len;
-    ks = valid ? __ldg(p.ks + head_row + key) : 0.0f;
-    vs = valid ? __ldg(p.vs + head_row + key) : 0.0f;
-    if (mask && valid) valid = mask[key] != 0;
-  };
 
   // softmax of one step's scores s[nt][..] and p.v over four V rows given as
   // f16 pair producers
@@ -239,53 +253,49 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 3) cached_attn_rows_kernel(co
   };
 
   // ---- cached keys
-  const int cached_end = min(step_end, cached_steps);
-  int step = split * per + warp;
-  if (step < cached_end) {
-    StepCodes cur;
-    float ks, vs;
-    bool valid;
-    load_codes(step, cur);
-    load_scalars(step, ks, vs, valid);
-    while (true) {
-      const int next = step + kRowsWarps;
-      const KeyScalars mine = key_scalars(p, ks, vs, valid);
-      float s[2][4];
+  for (int i = 0; i < mine_n; ++i) {
+    cp_async_wait<kRowsRing - 2>();
+    __syncwarp();
+    issue(i + kRowsRing - 1);              // into the slot of step i - 1, which every lane has read
+    const bool next_valid = mask_of(i + 1);
+    const uint8_t* st = sm.ring[warp][i % kRowsRing];
+    const float* scales = reinterpret_cast<const float*>(st + kRowsCodes);
+    const KeyScalars mine = key_scalars(p, scales[lane & 15], scales[16 + (lane & 15)], valid);
+    float s[2][4];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
+    for (int nt = 0; nt < 2; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
-        const uint32_t w[8] = {cur.k[nt][0].x, cur.k[nt][0].y, cur.k[nt][0].z, cur.k[nt][0].w,
-                               cur.k[nt][1].x, cur.k[nt][1].y, cur.k[nt][1].z, cur.k[nt][1].w};
+      for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+      for (int h = 0; h < 2; ++h) {
+        const uint4 x = *reinterpret_cast<const uint4*>(st + (nt * 8 + g) * kCaD + (((2 * c + h) ^ g) << 4));
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
           const uint32_t u = w[j] ^ 0x80808080u;
-          mma_f16(s[nt], qa[j], code_pair(u, 0x4140), code_pair(u, 0x4342));
+          mma_f16(s[nt], qa[4 * h + j], code_pair(u, 0x4140), code_pair(u, 0x4342));
         }
       }
-      const StepCodes now = cur;
-      if (next < cached_end) {
-        load_codes(next, cur);
-        load_scalars(next, ks, vs, valid);
-      }
-      // channel t of two V rows: interleave the rows' bytes, then widen
-      uint32_t il[2][8];
-#pragma unroll
-      for (int pr = 0; pr < 2; ++pr) {
-        const uint4 &x = now.v[2 * pr], &y = now.v[2 * pr + 1];
-        const uint32_t xa[4] = {x.x, x.y, x.z, x.w}, ya[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          il[pr][2 * i] = prmt(xa[i], ya[i], 0x5140) ^ 0x80808080u;
-          il[pr][2 * i + 1] = prmt(xa[i], ya[i], 0x7362) ^ 0x80808080u;
-        }
-      }
-      absorb(s, mine, [&](int pr, int tt) { return code_pair(il[pr][tt >> 1], (tt & 1) ? 0x4342 : 0x4140); });
-      if (next >= cached_end) break;
-      step = next;
     }
-    step += kRowsWarps;
+    // channel t of two V rows: interleave the rows' bytes, then widen
+    uint32_t il[2][8];
+#pragma unroll
+    for (int pr = 0; pr < 2; ++pr) {
+      const uint8_t* v0 = st + kRowsCodes / 2 + vkey(2 * pr) * kCaD + ((g ^ (2 * c)) << 4);
+      const uint8_t* v1 = st + kRowsCodes / 2 + vkey(2 * pr + 1) * kCaD + ((g ^ (2 * c + 1)) << 4);
+      const uint4 x = *reinterpret_cast<const uint4*>(v0), y = *reinterpret_cast<const uint4*>(v1);
+      const uint32_t xa[4] = {x.x, x.y, x.z, x.w}, ya[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        il[pr][2 * k] = prmt(xa[k], ya[k], 0x5140) ^ 0x80808080u;
+        il[pr][2 * k + 1] = prmt(xa[k], ya[k], 0x7362) ^ 0x80808080u;
+      }
+    }
+    absorb(s, mine, [&](int pr, int tt) { return code_pair(il[pr][tt >> 1], (tt & 1) ? 0x4342 : 0x4140); });
+    valid = next_valid;
   }
+  cp_async_wait<0>();
+  int step = step0 + mine_n * kRowsWarps;
 
   // ---- fresh keys: rows normalised by a power of two each, then as above
   for (; step < step_end; step += kRowsWarps) {
@@ -358,6 +368,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 3) cached_attn_rows_kernel(co
   }
 
   // ---- join the warps
+  __syncthreads();          // (every ring is done)
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -439,10 +450,15 @@ int launch_cached_rows(const CachedAttn& p, int batch, cudaStream_t st) {
   const int64_t tiles = (int64_t(p.sq) * p.share + kRowsTile - 1) / kRowsTile;
   const int64_t groups = tiles * p.kv_heads * batch;
   const int steps = (p.extent + kRowsStep - 1) / kRowsStep + (p.sk + kRowsStep - 1) / kRowsStep;
-  // keys are split until the CTAs fill the device (three per SM), as long as
-  // every warp keeps two steps of its own
+  // The keys are split as finely as leaves every warp two steps, up to a cluster
+  // of eight, but not into a second wave that would be nearly empty: past one
+  // wave (three CTAs per SM) only where that leaves several.
+  const int64_t slots = 3 * int64_t(sm_count());
   int splits = 1;
-  while (splits < 8 && groups * splits < 3 * sm_count() && steps >= 2 * splits * 2 * kRowsWarps) splits *= 2;
+  for (int s = 2; s <= 8; ++s) {
+    if (steps < 2 * s * kRowsWarps) break;
+    if (groups * s <= slots || groups * s >= 2 * slots || groups * (s - 1) > slots) splits = s;
+  }
   const int64_t gx = tiles * splits;
   if (gx > 0x7fffffff) return set_error(QIA_ERR_UNSUPPORTED, "qia_cached_attention: too many query rows");
   return launch_cluster("qia_cached_attention", cached_attn_rows_kernel,
@@ -454,12 +470,23 @@ int launch_cached_rows(const CachedAttn& p, int batch, cudaStream_t st) {
 
 using namespace qia;
 
+// The rows that share a K/V head fill one 16-row tile.
+static bool use_rows(int64_t seq_q, int64_t share) { return seq_q * share <= 16; }
+
+extern "C" int64_t qia_cached_attention_workspace_bytes(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t heads,
+                                                        int64_t kv_heads, int64_t extent, int masked) {
+  if (batch <= 0 || seq_q <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || heads / kv_heads > 128 ||
+      use_rows(seq_q, heads / kv_heads))
+    return 0;
+  return cached_tiles_workspace(batch, seq_q, seq_k, heads / kv_heads, kv_heads, extent, masked != 0);
+}
+
 extern "C" int qia_cached_attention(const void* q, const void* k, const void* v, const void* k_codes,
                                     const void* v_codes, const void* k_scales, const void* v_scales,
                                     const void* lengths, const void* key_valid, void* out, int64_t batch,
                                     int64_t seq_q, int64_t seq_k, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                     int64_t capacity, int64_t extent, const int64_t* strides, int64_t mask_stride,
-                                    float sm_scale, void* stream) {
+                                    float sm_scale, void* workspace, void* stream) {
   const char* who = "qia_cached_attention";
   if (!q || !k_codes || !v_codes || !k_scales || !v_scales || !lengths || !out || !strides)
     return set_error(QIA_ERR_INVALID, "%s: null pointer", who);
@@ -509,6 +536,13 @@ extern "C" int qia_cached_attention(const void* q, const void* k, const void* v,
   p.extent = int(extent);
   p.scale_log2 = (sm_scale > 0.0f ? sm_scale : 0.08838834764831845f) * 1.4426950408889634f;
   // rows that share a K/V head fill one 16-row tile, or the tensor-core tiles
-  if (seq_q * p.share <= 16) return launch_cached_rows(p, int(batch), as_stream(stream));
-  return launch_cached_tiles(p, int(batch), as_stream(stream));
+  if (use_rows(seq_q, p.share)) return launch_cached_rows(p, int(batch), as_stream(stream));
+  // a zero stride (broadcast k or v) is not a tensor map's: such rows are given another stride where
+  // it does not matter, and refused where it does
+  if (batch == 1) p.k_sb = p.v_sb = kCaD;
+  if (kv_heads == 1) p.k_sh = p.v_sh = kCaD;
+  if (seq_k == 1) p.k_ss = p.v_ss = kCaD;
+  if (seq_k > 0 && (p.k_sb <= 0 || p.v_sb <= 0 || p.k_sh <= 0 || p.v_sh <= 0 || p.k_ss <= 0 || p.v_ss <= 0))
+    return set_error(QIA_ERR_UNSUPPORTED, "%s: k and v may not be broadcast views", who);
+  return launch_cached_tiles(p, int(batch), workspace, as_stream(stream));
 }

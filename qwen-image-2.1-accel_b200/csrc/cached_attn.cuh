@@ -63,7 +63,9 @@ __device__ __forceinline__ KeyScalars key_scalars(const CachedAttn& p, float ks,
 }
 
 int launch_cached_rows(const CachedAttn& p, int batch, cudaStream_t st);    // few query rows (cached_attn.cu)
-int launch_cached_tiles(const CachedAttn& p, int batch, cudaStream_t st);   // many (cached_attn_tiles.cu)
+int launch_cached_tiles(const CachedAttn& p, int batch, void* workspace, cudaStream_t st);   // many (cached_attn_tiles.cu)
+int64_t cached_tiles_workspace(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t share, int64_t kv_heads,
+                               int64_t extent, bool masked);
 
 __device__ __forceinline__ float ex2_ftz(float x) {
   float y;

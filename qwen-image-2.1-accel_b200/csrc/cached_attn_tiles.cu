@@ -1,28 +1,30 @@
 // Attention of many query rows over the INT8 prefix cache: 256 query rows per
 // CTA on tcgen05.
 //
-// Roles (512 threads, one CTA per SM; warps 13-15 only fill the warpgroup):
-//   warps 0-3, 4-7  softmax of query tile 0 / 1 (128 rows each, a row per
-//                   thread): scores from TMEM, weights back into TMEM;
-//   warps 8-11      operand writers: INT8 codes -> bf16 (exact), fresh bf16 rows
+// Roles (384 threads, one CTA per SM):
+//   warps 0-3, 4-7  softmax groups 0 and 1 (a query row per thread): scores from
+//                   TMEM, weights back into TMEM;
+//   warp 8          issues the MMAs;
+//   warps 9-11      operand writers: INT8 codes -> bf16 (exact), fresh bf16 rows
 //                   copied, into the swizzled shared-memory tiles, and the
-//                   three per-key numbers of the softmax;
-//   warp 12         issues the MMAs.
+//                   per-key numbers of the softmax.
 // A key tile is 128 keys. K and V tiles (32 KB each) have two stages. TMEM:
-// scores of tile i at columns [128 i, +128), its bf16 weights over the first 64
-// of them (the A operand of P.V), accumulators at 256 + 128 i.
+// scores of group i at columns [128 i, +128), its bf16 weights over the first 64
+// of them (the A operand of P.V), accumulators at 256 + 128 i. The groups own
+// the two query tiles of the CTA and see every key tile, or, when there is only
+// one query tile, both work on it with the even and the odd key tiles.
 //
-// The issuer runs, for key tile j and query tile i:  P_i(j).V(j), then
-// Q_i.K(j+1), so while one tile's products run, the other tile's softmax works.
-// MMAs of one thread complete in order: Q_i.K(j+1) may overwrite the scores that
-// hold P_i(j), and once the scores of j+1 are there, the accumulators hold all
-// of P.V up to j and the softmax may rescale them (only when a row's maximum
-// grew by more than 2^8, see cached_attn.cuh).
+// The issuer runs, per softmax group: P(j).V(j), as each half of P(j) is stored,
+// then Q.K of the group's next key tile, so while one group's products run, the
+// other group's softmax works. MMAs of one thread complete in order: the next
+// Q.K may overwrite the scores that hold P(j), and once its scores are there,
+// the accumulators hold all of P.V up to j and the softmax may rescale them
+// (only when a row's maximum grew by more than 2^8, see cached_attn.cuh).
 //
-// What bounds it: per key tile and query tile 2 x 512 tensor cycles and 1024
-// cycles of exponentials per SM, with 4.5 instructions per score on four
-// schedulers close behind; INT8 -> bf16 costs two instructions per code, spread
-// over the 256 rows of the CTA.
+// Both products take the codes themselves; the softmax multiplies scores by
+// c log2e ks_j and weights by vs_j in fp32. Tiles whose keys all take part skip
+// the mask; fresh ones have no scales and touch no per-key number at all (the
+// broadcast reads of those share the shared-memory port with the operands).
 //
 // INT8 -> bf16: byte b under exponent byte 0x43; x = 128 + (b & 0x7f) and
 // c = 128 (b >= 0) or 256 (b < 0, exponent + 1) are bf16 patterns, x - c = b.
@@ -30,6 +32,10 @@
 // Keys may be split over a cluster, which joins through distributed shared
 // memory in rank order (no workspace, fixed order). Every wait is bounded (1 s)
 // and reports QIA_ERR_TIMEOUT through the device error word.
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
 #include "cached_attn.cuh"
 #include "cluster.cuh"
 #include "sm100.cuh"
@@ -43,14 +49,24 @@ constexpr int kPanel = kTileBytes / 2;
 constexpr int kSmemQ = 0;
 constexpr int kSmemKV = 2 * kTileBytes;        // stage s: K at 2 s, V at 2 s + 1
 constexpr int kScalarRing = 4;
-constexpr int kSmemScal = kSmemKV + 4 * kTileBytes;                   // [ring][sk | lsv | rsv][128] f32
-constexpr int kSmemML = kSmemScal + kScalarRing * 3 * 128 * 4;        // m, l of 256 rows (cluster join)
+constexpr int kScalarBytes = 3 * 128 * 4;      // [sk | vs | bias][128] f32
+constexpr int kSmemScal = kSmemKV + 4 * kTileBytes;
+constexpr int kSmemML = kSmemScal + kScalarRing * kScalarBytes;       // m, l of 256 rows (joining)
 constexpr int kSmemBars = kSmemML + 2 * 256 * 4;
 constexpr int kTilesSmem = kSmemBars + 256 + 1024;
-constexpr int kTilesThreads = 512;   // (a multiple of four warps: the register split below is per warpgroup)
+// Warps, and the registers of a softmax and of any other thread: the shares add
+// up to what the block starts with (384 x 168, 512 x 128).
+template <bool WIDE>
+struct Roles {
+  static constexpr int threads = WIDE ? 384 : 512;
+  static constexpr int writers = WIDE ? 1 : 7;         // arrivals of a written operand tile
+  static constexpr int softmax_regs = WIDE ? 208 : 160, other_regs = WIDE ? 88 : 96;
+};
 constexpr float kTilesLag = 8.0f;
 constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 constexpr uint32_t kIdescO = kIdescS | (1u << 16);   // B (V) is MN-major
+// kinds of a key tile, in the order of what the softmax has to read
+constexpr int kFreshFull = 0, kCachedFull = 1, kMasked = 2;
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t smem, const void* gmem, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(valid ? 16 : 0) : "memory");
@@ -60,10 +76,10 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_al
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-  return v;
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // bf16 pair of two codes of `w` (bytes picked by `sel`)
@@ -79,14 +95,170 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int piece) {
   return uint32_t((piece >> 3) * kPanel + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
 }
 
-struct TilesParams {
-  CachedAttn a;
-  int tokens_per_tile;   // query tokens in a tile of 128 rows: 128 / share
-  int q_tiles;           // tiles of the request
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+  uint32_t out;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
+  return out;
+}
+
+// Operands widened ahead of the products, per (request, K/V head): the cached
+// tiles (cached_cap of them) and, when keys are masked, the fresh tiles behind
+// them as bf16 rows (masked and missing ones zeros), and the per-key numbers of
+// all tiles.
+struct Widened {
+  __nv_bfloat16* k;      // [B Hkv, kv_tiles * 128, 128]
+  __nv_bfloat16* v;
+  float* scalars;        // [B Hkv, cached_cap + fresh_cap, 3, 128]
+  int cached_cap, fresh_cap, kv_tiles;
 };
 
-__global__ void __launch_bounds__(kTilesThreads, 1)
-cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, int* err) {
+struct TilesParams {
+  CachedAttn a;
+  Widened wide;
+  int tokens_per_tile;   // query tokens in a tile of 128 rows: 128 / share
+  int q_tiles, pairs;    // tiles of a request, and pairs of them
+  int first_group;       // group = (request, K/V head, pair), pairs fastest
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// One CTA per (key tile, K/V head, request): fills Widened. Bytes only: one in
+// and two out per code.
+__global__ void __launch_bounds__(256) cached_widen_kernel(const __grid_constant__ CachedAttn p,
+                                                           const __grid_constant__ Widened w) {
+  const int tile = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  grid_launch_dependents();
+  const bool cached = tile < w.cached_cap;
+  const int len = cached_len(p, b), end = cached ? len : p.sk, k0 = (cached ? tile : tile - w.cached_cap) * 128;
+  if (k0 >= end) return;
+  const int group = b * p.kv_heads + kvh;
+  const int64_t head_row = int64_t(group) * p.capacity;
+  const uint8_t* mask = p.key_valid ? p.key_valid + b * p.mask_sb + (cached ? 0 : p.extent) : nullptr;
+  if (threadIdx.x < 128) {
+    const int key = k0 + threadIdx.x;
+    const bool held = key < end, valid = held && (!mask || __ldg(mask + key) != 0);
+    float* dst = w.scalars + (int64_t(group) * (w.cached_cap + w.fresh_cap) + tile) * 384 + threadIdx.x;
+    const float ks = valid && cached ? __ldg(p.ks + head_row + key) : 1.0f;
+    dst[0] = valid ? p.scale_log2 * ks : 0.0f;
+    dst[128] = !valid ? 0.0f : cached ? __ldg(p.vs + head_row + key) : 1.0f;
+    dst[256] = valid ? 0.0f : -INFINITY;
+  }
+  if (tile >= w.kv_tiles) return;
+  const int64_t row0 = (int64_t(group) * w.kv_tiles + tile) * 128;
+  if (cached) {
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const int8_t* src = (z ? p.vc : p.kc) + head_row * kCaD;
+      __nv_bfloat16* dst = (z ? w.v : w.k) + row0 * kCaD;
+      uint4 c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = i * 32 + (threadIdx.x >> 3), key = k0 + row;
+        c[i] = key < end ? __ldg(reinterpret_cast<const uint4*>(src + int64_t(key) * kCaD) + (threadIdx.x & 7))
+                         : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = i * 32 + (threadIdx.x >> 3);
+        uint4* out = reinterpret_cast<uint4*>(dst + int64_t(row) * kCaD) + 2 * (threadIdx.x & 7);
+        st_global_v8(out,
+                     make_uint4(codes_bf16x2(c[i].x, 0x4140), codes_bf16x2(c[i].x, 0x4342),
+                                codes_bf16x2(c[i].y, 0x4140), codes_bf16x2(c[i].y, 0x4342)),
+                     make_uint4(codes_bf16x2(c[i].z, 0x4140), codes_bf16x2(c[i].z, 0x4342),
+                                codes_bf16x2(c[i].w, 0x4140), codes_bf16x2(c[i].w, 0x4342)));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const __nv_bfloat16* src = z ? p.v + b * p.v_sb + kvh * p.v_sh : p.k + b * p.k_sb + kvh * p.k_sh;
+      const int64_t ss = z ? p.v_ss : p.k_ss;
+      __nv_bfloat16* dst = (z ? w.v : w.k) + row0 * kCaD;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = i * 16 + (threadIdx.x >> 4), key = k0 + row;
+        const bool valid = key < end && (!mask || __ldg(mask + key) != 0);
+        reinterpret_cast<uint4*>(dst + int64_t(row) * kCaD)[threadIdx.x & 15] =
+            valid ? __ldg(reinterpret_cast<const uint4*>(src + int64_t(key) * ss) + (threadIdx.x & 15))
+                  : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  }
+}
+
+// The 128 scores of a row in registers -> their maximum, and for tiles with
+// per-key numbers also t = s * sk (+ bias) in place.
+template <int KIND>
+__device__ __forceinline__ float row_scores(uint32_t (&s)[128], const float* scal, float c) {
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < 128; i += 4) {
+    if (KIND != kFreshFull) {
+      const float4 sk = *reinterpret_cast<const float4*>(scal + i);
+      uint64_t t0 = f2_pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+      uint64_t t1 = f2_pack(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+      if (KIND == kMasked) {
+        const float4 bias = *reinterpret_cast<const float4*>(scal + 256 + i);
+        t0 = f2_fma(t0, f2_pack(sk.x, sk.y), f2_pack(bias.x, bias.y));
+        t1 = f2_fma(t1, f2_pack(sk.z, sk.w), f2_pack(bias.z, bias.w));
+      } else {
+        t0 = f2_mul(t0, f2_pack(sk.x, sk.y));
+        t1 = f2_mul(t1, f2_pack(sk.z, sk.w));
+      }
+      float a, b;
+      f2_unpack(t0, a, b);
+      s[i] = __float_as_uint(a);
+      s[i + 1] = __float_as_uint(b);
+      f2_unpack(t1, a, b);
+      s[i + 2] = __float_as_uint(a);
+      s[i + 3] = __float_as_uint(b);
+    }
+    mx[(i / 4) & 3] = max3(mx[(i / 4) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+    mx[(i / 4 + 2) & 3] = max3(mx[(i / 4 + 2) & 3], __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+  }
+  const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+  return KIND == kFreshFull ? top * c : top;
+}
+
+// Weights of 64 keys (half h): w = 2^(t - m), their sum into l, and w (times vs
+// of cached keys) as bf16 pairs.
+template <int KIND>
+__device__ __forceinline__ void row_weights(const uint32_t (&s)[128], int h, const float* scal, float c, float neg_m,
+                                            uint64_t (&l)[2], uint32_t (&w)[32]) {
+  const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(neg_m, neg_m);
+#pragma unroll
+  for (int k = 0; k < 64; k += 4) {
+    const int i = h * 64 + k;
+    float4 vs;
+    if (KIND != kFreshFull) vs = *reinterpret_cast<const float4*>(scal + 128 + i);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint64_t x = f2_pack(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
+      float a, b;
+      f2_unpack(KIND == kFreshFull ? f2_fma(x, c2, n2) : f2_add(x, n2), a, b);
+      a = ex2_ftz(a);
+      b = ex2_ftz(b);
+      l[e] = f2_add(l[e], f2_pack(a, b));
+      if (KIND != kFreshFull) f2_unpack(f2_mul(f2_pack(a, b), e ? f2_pack(vs.z, vs.w) : f2_pack(vs.x, vs.y)), a, b);
+      w[k / 2 + e] = cvt_bf16x2(a, b);
+    }
+  }
+}
+
+// WIDE: operands come by TMA, cached ones (and masked fresh ones) from Widened,
+// fresh ones straight from k and v; else seven warps write them from the codes.
+template <bool WIDE>
+__global__ void __launch_bounds__(Roles<WIDE>::threads, 1)
+cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, const __grid_constant__ CUtensorMap tm_wk,
+                         const __grid_constant__ CUtensorMap tm_wv, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v, int* err) {
+  constexpr int kTilesThreads = Roles<WIDE>::threads, kWriters = Roles<WIDE>::writers;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const CachedAttn& p = tp.a;
@@ -97,16 +269,18 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, int* err) {
   uint64_t* k_empty = bars + 4;       // [2] issuer -> operand writers
   uint64_t* v_empty = bars + 6;       // [2]
   uint64_t* scal_full = bars + 8;     // [4] operand writers -> softmax
-  uint64_t* s_full = bars + 12;       // [2] scores of query tile i
-  uint64_t* p_full = bars + 14;       // [2] weights of query tile i stored
-  uint64_t* o_full = bars + 16;
-  uint64_t* drain = bars + 17;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  uint64_t* s_full = bars + 12;       // [2] scores of group i
+  uint64_t* p_full = bars + 14;       // [2][2] weights of group i, half h, stored
+  uint64_t* o_full = bars + 18;
+  uint64_t* drain = bars + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = int(cluster_size()), split = int(cluster_rank());
-  const int pair = blockIdx.x / splits, kvh = blockIdx.y, b = blockIdx.z;
+  const int group = tp.first_group + int(blockIdx.x) / splits;
+  const int pair = group % tp.pairs, kvh = group / tp.pairs % p.kv_heads, b = group / tp.pairs / p.kv_heads;
   const int n_tiles = min(2, tp.q_tiles - 2 * pair);   // query tiles of this CTA
+  const bool duo = n_tiles == 1;                       // the groups share one: even and odd key tiles
   const int len = cached_len(p, b);
   const int cached_tiles = (len + 127) / 128;
   const int all_tiles = cached_tiles + (p.sk + 127) / 128;
@@ -115,26 +289,26 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, int* err) {
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&k_full[i]), 4);
-      mbar_init(smem_u32(&v_full[i]), 4);
+      mbar_init(smem_u32(&k_full[i]), kWriters);
+      mbar_init(smem_u32(&v_full[i]), kWriters);
       mbar_init(smem_u32(&k_empty[i]), 1);
       mbar_init(smem_u32(&v_empty[i]), 1);
       mbar_init(smem_u32(&s_full[i]), 1);
-      mbar_init(smem_u32(&p_full[i]), 4);
     }
-    for (int i = 0; i < kScalarRing; ++i) mbar_init(smem_u32(&scal_full[i]), 4);
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&p_full[i]), 4);
+    for (int i = 0; i < kScalarRing; ++i) mbar_init(smem_u32(&scal_full[i]), kWriters);
     mbar_init(smem_u32(o_full), 1);
     mbar_init(smem_u32(drain), 1);
     fence_barrier_init();
   }
-  if (warp == 12) tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == 8) tmem_alloc(smem_u32(tmem_slot), 512);
   // ---- query tiles (rows past the end are zeros)
   const int tile_rows = tp.tokens_per_tile * p.share;
-  for (int i = threadIdx.x; i < 2 * kTileRows * 16; i += kTilesThreads) {
+  for (int i = threadIdx.x; i < n_tiles * kTileRows * 16; i += kTilesThreads) {
     const int tile = i >> 11, row = (i >> 4) & 127, piece = i & 15;
     const int token = (2 * pair + tile) * tp.tokens_per_tile + row / p.share;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (tile < n_tiles && row < tile_rows && token < p.sq)
+    if (row < tile_rows && token < p.sq)
       v = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_sb + int64_t(token) * p.q_ss +
                                                int64_t(kvh * p.share + row % p.share) * p.q_sh) + piece);
     st_shared_v4(sbase + kSmemQ + tile * kTileBytes + tile_offset(row, piece), v.x, v.y, v.z, v.w);
@@ -144,275 +318,333 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, int* err) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // key tiles of softmax group w: the it-th is it (both groups), or 2 it + w
+  const auto tiles_of = [&](int w) { return duo ? (n - w + 1) / 2 : n; };
 
-  float m = -INFINITY, l = 0.0f;
-  bool have = false;               // the accumulators hold something
-  if (warp >= 12) {
-    // -------------------------------------------------------------- MMA issuer
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 12 && lane == 0 && n > 0) {
-      bool ok = true;
-      const auto qk = [&](int i, int j) {
-        const uint64_t qd = smem_desc_k_sw128(sbase + kSmemQ + i * kTileBytes);
-        const uint64_t kd = smem_desc_k_sw128(sbase + kSmemKV + (j & 1) * 2 * kTileBytes);
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Roles<WIDE>::other_regs));
+    if (warp == 8) {
+      // ------------------------------------------------------------ MMA issuer
+      if (lane == 0 && n > 0) {
+        bool ok = true;
+        const auto qk = [&](int w, int j) {
+          const uint64_t qd = smem_desc_k_sw128(sbase + kSmemQ + (duo ? 0 : w) * kTileBytes);
+          const uint64_t kd = smem_desc_k_sw128(sbase + kSmemKV + (j & 1) * 2 * kTileBytes);
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const uint64_t off = uint64_t(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
-          tc_mma_f16_ss(tmem + uint32_t(128 * i), qd + off, kd + off, kIdescS, kk > 0);
-        }
-        tc_commit(smem_u32(&s_full[i]));
-      };
-      const auto pv = [&](int i, int j) {
-        const uint64_t vd = smem_desc_mn_sw128(sbase + kSmemKV + ((j & 1) * 2 + 1) * kTileBytes, kPanel);
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint64_t off = uint64_t(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
+            tc_mma_f16_ss(tmem + uint32_t(128 * w), qd + off, kd + off, kIdescS, kk > 0);
+          }
+          tc_commit(smem_u32(&s_full[w]));
+        };
+        const auto wait_k = [&](int j) { return mbar_wait(smem_u32(&k_full[j & 1]), (j >> 1) & 1, err); };
+        // P.V of group w's it-th key tile j, in halves of 64 keys as they are stored
+        const auto pv = [&](int w, int it, int j) {
+          const uint64_t vd = smem_desc_mn_sw128(sbase + kSmemKV + ((j & 1) * 2 + 1) * kTileBytes, kPanel);
+          for (int h = 0; h < 2; ++h) {
+            if (!mbar_wait(smem_u32(&p_full[2 * w + h]), it & 1, err)) return false;
+            tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)   // 16 keys: two 8-key groups of 1 KB
-          tc_mma_f16_ts(tmem + uint32_t(256 + 128 * i), tmem + uint32_t(128 * i + 8 * kk), vd + uint64_t(128 * kk),
-                        kIdescO, (j | kk) != 0);
-      };
-      ok = mbar_wait(smem_u32(&k_full[0]), 0, err);
-      tc_fence_after();
-      if (ok) {
-        for (int i = 0; i < n_tiles; ++i) qk(i, 0);
-        tc_commit(smem_u32(&k_empty[0]));
-      }
-      for (int j = 0; j < n && ok; ++j) {
-        ok = mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, err);
-        for (int i = 0; i < n_tiles && ok; ++i) {
-          ok = mbar_wait(smem_u32(&p_full[i]), j & 1, err);
-          if (ok && i == 0 && j + 1 < n) ok = mbar_wait(smem_u32(&k_full[(j + 1) & 1]), ((j + 1) >> 1) & 1, err);
-          if (!ok) break;
-          tc_fence_after();
-          pv(i, j);
-          if (j + 1 < n) qk(i, j + 1);
-        }
-        if (!ok) break;
-        tc_commit(smem_u32(&v_empty[j & 1]));
-        if (j + 1 < n) tc_commit(smem_u32(&k_empty[(j + 1) & 1]));
-      }
-      if (ok) tc_commit(smem_u32(o_full));
-      tc_commit(smem_u32(drain));
-      mbar_wait(smem_u32(drain), 0, ok ? err : nullptr, 100000000ull);
-    }
-    __syncwarp();
-  } else if (warp >= 8) {
-    // --------------------------------------------------------- operand writers
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    const int t = threadIdx.x - 256;
-    const int64_t head_row = (int64_t(b) * p.kv_heads + kvh) * p.capacity;
-    const uint8_t* mask = p.key_valid ? p.key_valid + b * p.mask_sb : nullptr;
-    const int cached_n = max(0, min(n, cached_tiles - first));   // cached tiles of this CTA
-    // codes of half tile u (2 j: K of tile j, 2 j + 1: V): eight 16-byte pieces, eight threads per row
-    const auto load_codes = [&](int u, uint4 (&c)[8]) {
-      const int k0 = (first + (u >> 1)) * 128;
-      const int8_t* src = ((u & 1) ? p.vc : p.kc) + head_row * kCaD + (t & 7) * 16;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = min(k0 + i * 16 + (t >> 3), len - 1);   // (past the length: any held row, weight 0)
-        c[i] = __ldg(reinterpret_cast<const uint4*>(src + int64_t(key) * kCaD));
-      }
-    };
-    const auto load_scalars = [&](int j, float& ks, float& vs, bool& valid) {
-      const int tile = first + j;
-      ks = vs = 1.0f;
-      if (tile < cached_tiles) {
-        const int key = tile * 128 + t;
-        valid = key < len && (!mask || mask[key] != 0);
-        if (key < len) {
-          ks = __ldg(p.ks + head_row + key);
-          vs = __ldg(p.vs + head_row + key);
-        }
-      } else {
-        const int key = (tile - cached_tiles) * 128 + t;
-        valid = key < p.sk && (!mask || mask[p.extent + key] != 0);
-      }
-    };
-    const auto store_scalars = [&](int j, float ks, float vs, bool valid) {
-      const KeyScalars k = key_scalars(p, ks, vs, valid);
-      float* dst = reinterpret_cast<float*>(smem + kSmemScal) + (j % kScalarRing) * 384 + t;
-      dst[0] = k.sk;
-      dst[128] = k.lsv;
-      dst[256] = k.rsv;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&scal_full[j % kScalarRing]));
-    };
-    const auto publish = [&](int u) {
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32((u & 1) ? &v_full[(u >> 1) & 1] : &k_full[(u >> 1) & 1]));
-    };
-    const auto wait_slot = [&](int u) {
-      const int j = u >> 1;
-      return __all_sync(0xffffffffu, mbar_wait(smem_u32((u & 1) ? &v_empty[j & 1] : &k_empty[j & 1]),
-                                               ((j >> 1) & 1) ^ 1, err));
-    };
-    uint4 cur[8];
-    float ks = 1.0f, vs = 1.0f;
-    bool valid = false, ok = true;
-    if (n > 0) load_scalars(0, ks, vs, valid);
-    if (cached_n > 0) load_codes(0, cur);
-    int u = 0;
-    for (; u < 2 * cached_n && ok; ++u) {
-      uint4 next[8];
-      if (u + 1 < 2 * cached_n) load_codes(u + 1, next);
-      const int j = u >> 1;
-      ok = wait_slot(u);
-      if (!ok) break;
-      const uint32_t slot = sbase + kSmemKV + uint32_t((j & 1) * 2 + (u & 1)) * kTileBytes;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = i * 16 + (t >> 3), piece = (t & 7) * 2;
-        const uint32_t a0 = codes_bf16x2(cur[i].x, 0x4140), a1 = codes_bf16x2(cur[i].x, 0x4342);
-        const uint32_t a2 = codes_bf16x2(cur[i].y, 0x4140), a3 = codes_bf16x2(cur[i].y, 0x4342);
-        const uint32_t b0 = codes_bf16x2(cur[i].z, 0x4140), b1 = codes_bf16x2(cur[i].z, 0x4342);
-        const uint32_t b2 = codes_bf16x2(cur[i].w, 0x4140), b3 = codes_bf16x2(cur[i].w, 0x4342);
-        // the upper four lanes of a row write their second piece first: the
-        // eight lanes of a store phase then hit eight different bank groups
-        if (t & 4) {
-          st_shared_v4(slot + tile_offset(row, piece + 1), b0, b1, b2, b3);
-          st_shared_v4(slot + tile_offset(row, piece), a0, a1, a2, a3);
+            for (int k = 0; k < 4; ++k) {   // 16 keys: two 8-key groups of 1 KB
+              const int kk = 4 * h + k;
+              tc_mma_f16_ts(tmem + uint32_t(256 + 128 * w), tmem + uint32_t(128 * w + 8 * kk), vd + uint64_t(128 * kk),
+                            kIdescO, (it | kk) != 0);
+            }
+          }
+          return true;
+        };
+        if (duo) {
+          for (int j = 0; j < 2 && j < n && ok; ++j) {
+            ok = wait_k(j);
+            tc_fence_after();
+            if (ok) qk(j, j);
+            if (ok) tc_commit(smem_u32(&k_empty[j]));
+          }
+          for (int j = 0; j < n && ok; ++j) {
+            ok = mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, err) && pv(j & 1, j >> 1, j);
+            if (!ok) break;
+            tc_commit(smem_u32(&v_empty[j & 1]));
+            if (j + 2 < n) {
+              ok = wait_k(j + 2);
+              if (!ok) break;
+              tc_fence_after();
+              qk(j & 1, j + 2);
+              tc_commit(smem_u32(&k_empty[j & 1]));
+            }
+          }
         } else {
-          st_shared_v4(slot + tile_offset(row, piece), a0, a1, a2, a3);
-          st_shared_v4(slot + tile_offset(row, piece + 1), b0, b1, b2, b3);
+          ok = wait_k(0);
+          tc_fence_after();
+          if (ok) {
+            qk(0, 0);
+            qk(1, 0);
+            tc_commit(smem_u32(&k_empty[0]));
+          }
+          for (int j = 0; j < n && ok; ++j) {
+            ok = mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, err);
+            for (int w = 0; w < 2 && ok; ++w) {
+              ok = pv(w, j, j);
+              if (ok && j + 1 < n) {
+                ok = w > 0 || wait_k(j + 1);
+                if (!ok) break;
+                tc_fence_after();
+                qk(w, j + 1);
+              }
+            }
+            if (!ok) break;
+            tc_commit(smem_u32(&v_empty[j & 1]));
+            if (j + 1 < n) tc_commit(smem_u32(&k_empty[(j + 1) & 1]));
+          }
+        }
+        if (ok) tc_commit(smem_u32(o_full));
+        tc_commit(smem_u32(drain));
+        mbar_wait(smem_u32(drain), 0, ok ? err : nullptr, 100000000ull);
+      }
+      __syncwarp();
+    } else if constexpr (WIDE) {
+      // ---------------------------------------------------------- TMA producer
+      if (warp == 9 && lane == 0 && n > 0) {
+        const int bh = b * p.kv_heads + kvh;
+        bool ok = true;
+        grid_wait();                           // the operands are widened
+        int issued = 0;
+        for (int u = 0; u < 2 * n && ok; ++u) {
+          const int j = u >> 1, tile = first + j, st = j & 1;
+          if (!(u & 1)) {                      // (ring slot j % 4: tile j - 4 was done before V of j - 3 left)
+            const uint32_t bar = smem_u32(&scal_full[j % kScalarRing]);
+            const int at = tile < cached_tiles ? tile : tp.wide.cached_cap + tile - cached_tiles;
+            mbar_arrive_expect_tx(bar, kScalarBytes);
+            bulk_load(sbase + kSmemScal + uint32_t(j % kScalarRing) * kScalarBytes,
+                      tp.wide.scalars + (int64_t(bh) * (tp.wide.cached_cap + tp.wide.fresh_cap) + at) * 384,
+                      kScalarBytes, bar);
+          }
+          ok = mbar_wait(smem_u32((u & 1) ? &v_empty[st] : &k_empty[st]), ((j >> 1) & 1) ^ 1, err);
+          if (!ok) break;
+          const uint32_t bar = smem_u32((u & 1) ? &v_full[st] : &k_full[st]);
+          const uint32_t slot = sbase + kSmemKV + uint32_t(st * 2 + (u & 1)) * kTileBytes;
+          mbar_arrive_expect_tx(bar, kTileBytes);
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t dst = slot + uint32_t(h * kPanel);
+            if (tile < cached_tiles || p.key_valid) {
+              const int at = tile < cached_tiles ? tile : tp.wide.cached_cap + tile - cached_tiles;
+              tma_load_2d(dst, (u & 1) ? &tm_wv : &tm_wk, bar, h * 64, (bh * tp.wide.kv_tiles + at) * 128);
+            } else {
+              tma_load_4d(dst, (u & 1) ? &tm_v : &tm_k, bar, h * 64, (tile - cached_tiles) * 128, kvh, b);
+            }
+          }
+          issued = u + 1;
+        }
+        if (!ok) {   // let queued copies land before the shared memory is released
+          for (int u = max(0, issued - 4); u < issued; ++u)
+            mbar_wait(smem_u32((u & 1) ? &v_full[(u >> 1) & 1] : &k_full[(u >> 1) & 1]), (u >> 2) & 1, nullptr,
+                      100000000ull);
+          for (int j = max(0, (issued + 1) / 2 - kScalarRing); j <= issued / 2; ++j)
+            mbar_wait(smem_u32(&scal_full[j % kScalarRing]), (j / kScalarRing) & 1, nullptr, 100000000ull);
         }
       }
-      if (!(u & 1)) {
-        store_scalars(j, ks, vs, valid);
-      } else if (j + 1 < n) {
-        load_scalars(j + 1, ks, vs, valid);
-      }
-      publish(u);
+      __syncwarp();
+    } else {
+      // ------------------------------------------------------- operand writers
+      const int t = threadIdx.x - 32 * 9;
+      const int64_t head_row = (int64_t(b) * p.kv_heads + kvh) * p.capacity;
+      const uint8_t* mask = p.key_valid ? p.key_valid + b * p.mask_sb : nullptr;
+      const int cached_n = max(0, min(n, cached_tiles - first));   // cached tiles of this CTA
+      // codes of half tile u (2 j: K of tile j, 2 j + 1: V): eight threads per
+      // row, 28 rows per step
+      constexpr int kSteps = 5;
+      const int trow = t >> 3;
+      const auto load_codes = [&](int u, uint4 (&c)[kSteps]) {
+        const int k0 = (first + (u >> 1)) * 128;
+        const int8_t* src = ((u & 1) ? p.vc : p.kc) + head_row * kCaD + (t & 7) * 16;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) cur[i] = next[i];
-    }
-    // fresh tiles: bf16 rows copied as they are (masked and missing rows as
-    // zeros); a tile is published one step later, when its copies have landed
-    bool pending = false;
-    for (; u < 2 * n && ok; ++u) {
-      const int j = u >> 1, k0 = (first + j - cached_tiles) * 128;
-      ok = wait_slot(u);
-      if (!ok) break;
-      if (pending) {
-        cp_async_wait();
-        publish(u - 1);
-      }
-      const uint32_t slot = sbase + kSmemKV + uint32_t((j & 1) * 2 + (u & 1)) * kTileBytes;
-      const __nv_bfloat16* src = (u & 1) ? p.v + b * p.v_sb + kvh * p.v_sh : p.k + b * p.k_sb + kvh * p.k_sh;
-      const int64_t ss = (u & 1) ? p.v_ss : p.k_ss;
+        for (int i = 0; i < kSteps; ++i) {
+          const int key = min(k0 + i * 28 + trow, len - 1);   // (past the length: any held row, weight 0)
+          c[i] = __ldg(reinterpret_cast<const uint4*>(src + int64_t(key) * kCaD));
+        }
+      };
+      const auto store_codes = [&](uint32_t slot, const uint4 (&c)[kSteps]) {
+        const int piece = (t & 7) * 2;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int row = i * 8 + (t >> 4), piece = t & 15, key = k0 + row;
-        const bool held = key < p.sk && (!mask || mask[p.extent + key] != 0);
-        cp_async16_zfill(slot + tile_offset(row, piece), src + int64_t(held ? key : 0) * ss + piece * 8, held);
+        for (int i = 0; i < kSteps; ++i) {
+          const int row = i * 28 + trow;
+          if (row >= kTileRows) break;
+          const uint32_t a0 = codes_bf16x2(c[i].x, 0x4140), a1 = codes_bf16x2(c[i].x, 0x4342);
+          const uint32_t a2 = codes_bf16x2(c[i].y, 0x4140), a3 = codes_bf16x2(c[i].y, 0x4342);
+          const uint32_t b0 = codes_bf16x2(c[i].z, 0x4140), b1 = codes_bf16x2(c[i].z, 0x4342);
+          const uint32_t b2 = codes_bf16x2(c[i].w, 0x4140), b3 = codes_bf16x2(c[i].w, 0x4342);
+          // the upper four lanes of a row write their second piece first: the
+          // eight lanes of a store phase then hit eight different bank groups
+          const bool up = t & 4;
+          st_shared_v4(slot + tile_offset(row, piece + up), up ? b0 : a0, up ? b1 : a1, up ? b2 : a2, up ? b3 : a3);
+          st_shared_v4(slot + tile_offset(row, piece + !up), up ? a0 : b0, up ? a1 : b1, up ? a2 : b2, up ? a3 : b3);
+        }
+      };
+      // the softmax's numbers of key tile j, one key per thread
+      float ks = 1.0f, vs = 1.0f;
+      bool valid = false;
+      const auto load_scalars = [&](int j) {
+        const int tile = first + j;
+        ks = vs = 1.0f;
+        if (tile < cached_tiles) {
+          const int key = tile * 128 + t;
+          valid = key < len && t < 128;
+          if (valid) {
+            ks = __ldg(p.ks + head_row + key);
+            vs = __ldg(p.vs + head_row + key);
+            valid = !mask || __ldg(mask + key) != 0;
+          }
+        } else {
+          const int key = (tile - cached_tiles) * 128 + t;
+          valid = key < p.sk && t < 128 && (!mask || __ldg(mask + p.extent + key) != 0);
+        }
+      };
+      const auto store_scalars = [&](int j) {
+        if (t < 128) {
+          float* dst = reinterpret_cast<float*>(smem + kSmemScal + (j % kScalarRing) * kScalarBytes) + t;
+          dst[0] = valid ? p.scale_log2 * ks : 0.0f;
+          dst[128] = valid ? vs : 0.0f;
+          dst[256] = valid ? 0.0f : -INFINITY;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&scal_full[j % kScalarRing]));
+      };
+      const auto publish = [&](int u) {
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32((u & 1) ? &v_full[(u >> 1) & 1] : &k_full[(u >> 1) & 1]));
+      };
+      const auto wait_slot = [&](int u) {
+        const int j = u >> 1;
+        return __all_sync(0xffffffffu, mbar_wait(smem_u32((u & 1) ? &v_empty[j & 1] : &k_empty[j & 1]),
+                                                 ((j >> 1) & 1) ^ 1, err));
+      };
+      uint4 cur[kSteps];
+      bool ok = true;
+      if (n > 0) load_scalars(0);
+      if (cached_n > 0) load_codes(0, cur);
+      int u = 0;
+      for (; u < 2 * cached_n && ok; ++u) {
+        uint4 next[kSteps];
+        if (u + 1 < 2 * cached_n) load_codes(u + 1, next);
+        const int j = u >> 1;
+        ok = wait_slot(u);
+        if (!ok) break;
+        store_codes(sbase + kSmemKV + uint32_t((j & 1) * 2 + (u & 1)) * kTileBytes, cur);
+        publish(u);
+        if (!(u & 1)) {
+          store_scalars(j);
+        } else if (j + 1 < n) {
+          load_scalars(j + 1);
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) cur[i] = next[i];
       }
-      pending = true;
-      if (!(u & 1)) {
-        store_scalars(j, ks, vs, valid);
-        if (j + 1 < n) load_scalars(j + 1, ks, vs, valid);
+      // fresh tiles: bf16 rows copied as they are (masked and missing rows as
+      // zeros); a tile is published one step later, when its copies have landed
+      bool pending = false;
+      for (; u < 2 * n && ok; ++u) {
+        const int j = u >> 1, k0 = (first + j - cached_tiles) * 128;
+        ok = wait_slot(u);
+        if (!ok) break;
+        if (pending) {
+          cp_async_wait();
+          publish(u - 1);
+        }
+        const uint32_t slot = sbase + kSmemKV + uint32_t((j & 1) * 2 + (u & 1)) * kTileBytes;
+        const __nv_bfloat16* src = (u & 1) ? p.v + b * p.v_sb + kvh * p.v_sh : p.k + b * p.k_sb + kvh * p.k_sh;
+        const int64_t ss = (u & 1) ? p.v_ss : p.k_ss;
+        for (int row = t >> 4; row < kTileRows; row += 14) {
+          const int piece = t & 15, key = k0 + row;
+          const bool held = key < p.sk && (!mask || __ldg(mask + p.extent + key) != 0);
+          cp_async16_zfill(slot + tile_offset(row, piece), src + int64_t(held ? key : 0) * ss + piece * 8, held);
+        }
+        pending = true;
+        if (!(u & 1)) {
+          store_scalars(j);
+          if (j + 1 < n) load_scalars(j + 1);
+        }
       }
+      cp_async_wait();
+      if (pending && ok) publish(u - 1);
     }
-    cp_async_wait();
-    if (pending && ok) publish(u - 1);
   } else {
     // ----------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-    const int tile = warp >> 2;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Roles<WIDE>::softmax_regs));
+    const int w = warp >> 2;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + t_lane + uint32_t(128 * tile), t_o = tmem + t_lane + uint32_t(256 + 128 * tile);
-    bool ok = tile < n_tiles;
-    uint64_t l0 = f2_pack(0.0f, 0.0f), l1 = l0;
-    for (int j = 0; j < n && ok; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[tile]), j & 1, err) &&
+    const uint32_t t_s = tmem + t_lane + uint32_t(128 * w), t_o = tmem + t_lane + uint32_t(256 + 128 * w);
+    const float c = p.scale_log2;
+    const int count = tiles_of(w);
+    bool ok = true;
+    float m = -INFINITY;
+    uint64_t l2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+    for (int it = 0; it < count; ++it) {
+      const int j = duo ? 2 * it + w : it;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[w]), it & 1, err) &&
                                        mbar_wait(smem_u32(&scal_full[j % kScalarRing]), (j / kScalarRing) & 1, err));
       if (!ok) break;
       tc_fence_after();
       uint32_t s[128];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        tc_ld_32x32b_x32(t_s + uint32_t(c * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+      for (int q = 0; q < 4; ++q)
+        tc_ld_32x32b_x32(t_s + uint32_t(q * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[q * 32]));
+      const float* scal = reinterpret_cast<const float*>(smem + kSmemScal + (j % kScalarRing) * kScalarBytes);
+      const int tile = first + j, tail = tile < cached_tiles ? len - tile * 128 : p.sk - (tile - cached_tiles) * 128;
+      const int kind = p.key_valid || tail < 128 ? kMasked : tile < cached_tiles ? kCachedFull : kFreshFull;
       tc_wait_ld();
-      const uint32_t scal = sbase + kSmemScal + uint32_t((j % kScalarRing) * 384 * 4);
-      float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 128; c += 4) {
-        const float4 sk = ld_shared_f4(scal + c * 4), lv = ld_shared_f4(scal + 512 + c * 4);
-        float t0, t1, t2, t3;
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), f2_pack(sk.x, sk.y),
-                         f2_pack(lv.x, lv.y)), t0, t1);
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), f2_pack(sk.z, sk.w),
-                         f2_pack(lv.z, lv.w)), t2, t3);
-        mx0 = fmaxf(mx0, fmaxf(t0, t1));
-        mx1 = fmaxf(mx1, fmaxf(t2, t3));
-        s[c] = __float_as_uint(t0);
-        s[c + 1] = __float_as_uint(t1);
-        s[c + 2] = __float_as_uint(t2);
-        s[c + 3] = __float_as_uint(t3);
-      }
-      const float top = fmaxf(mx0, mx1);
+      const float top = kind == kFreshFull    ? row_scores<kFreshFull>(s, scal, c)
+                        : kind == kCachedFull ? row_scores<kCachedFull>(s, scal, c)
+                                              : row_scores<kMasked>(s, scal, c);
       const bool grow = top > m + kTilesLag;
       if (__any_sync(0xffffffffu, grow)) {
         const float f = grow ? ex2_ftz(m - top) : 1.0f;   // (m = -inf: 0)
         if (grow) m = top;
-        l0 = f2_mul(l0, f2_pack(f, f));
-        l1 = f2_mul(l1, f2_pack(f, f));
-        if (j > 0) {
+        l2[0] = f2_mul(l2[0], f2_pack(f, f));
+        l2[1] = f2_mul(l2[1], f2_pack(f, f));
+        if (it > 0) {
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tc_ld_32x32b_x32(t_o + uint32_t(c * 32), o);
+          for (int q = 0; q < 8; ++q) {
+            uint32_t o[16];
+            tc_ld_32x32b_x16(t_o + uint32_t(q * 16), o);
             tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tc_st_32x32b_x32(t_o + uint32_t(c * 32), o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tc_st_32x32b_x16(t_o + uint32_t(q * 16), o);
           }
         }
       }
-      const float base = m == -INFINITY ? 0.0f : -m;
-      const uint64_t base2 = f2_pack(base, base);
+      const float neg_m = m == -INFINITY ? 0.0f : -m;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t w[32];
-#pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          const int i = h * 64 + c;
-          const float4 rv = ld_shared_f4(scal + 1024 + i * 4);
-          float w0, w1, w2, w3;
-          f2_unpack(f2_add(f2_pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), base2), w0, w1);
-          f2_unpack(f2_add(f2_pack(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), base2), w2, w3);
-          w0 = ex2_ftz(w0);
-          w1 = ex2_ftz(w1);
-          w2 = ex2_ftz(w2);
-          w3 = ex2_ftz(w3);
-          l0 = f2_fma(f2_pack(w0, w1), f2_pack(rv.x, rv.y), l0);
-          l1 = f2_fma(f2_pack(w2, w3), f2_pack(rv.z, rv.w), l1);
-          w[c / 2] = cvt_bf16x2(w0, w1);
-          w[c / 2 + 1] = cvt_bf16x2(w2, w3);
-        }
-        tc_st_32x32b_x32(t_s + uint32_t(32 * h), w);
+        uint32_t x[32];
+        if (kind == kFreshFull) row_weights<kFreshFull>(s, h, scal, c, neg_m, l2, x);
+        else row_weights<kCachedFull>(s, h, scal, c, neg_m, l2, x);
+        tc_st_32x32b_x32(t_s + uint32_t(32 * h), x);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&p_full[2 * w + h]));
       }
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&p_full[tile]));
     }
-    float a, c;
-    f2_unpack(f2_add(l0, l1), a, c);
-    l = a + c;
-    have = ok && n > 0;
-    if (have) have = __all_sync(0xffffffffu, mbar_wait(smem_u32(o_full), 0, err));
+    float la, lb;
+    f2_unpack(f2_add(l2[0], l2[1]), la, lb);
+    const float l = la + lb;
+    bool have = ok && count > 0;       // the accumulators hold something
+    if (ok && n > 0) have = __all_sync(0xffffffffu, mbar_wait(smem_u32(o_full), 0, err)) && have;
     tc_fence_after();
     // ------------------------------------------------------------------ output
     const int row = (warp & 3) * 32 + lane;
-    const int token = (2 * pair + tile) * tp.tokens_per_tile + row / p.share;
-    const bool live = tile < n_tiles && row < tile_rows && token < p.sq;
-    if (splits == 1) {
+    if (splits == 1 && !duo) {
+      const int token = (2 * pair + w) * tp.tokens_per_tile + row / p.share;
+      const bool live = row < tile_rows && token < p.sq;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       uint4* dst = reinterpret_cast<uint4*>(p.out + b * p.o_sb + int64_t(token) * p.o_ss +
                                             int64_t(kvh * p.share + row % p.share) * p.o_sh);
 #pragma unroll 1
-      for (int c4 = 0; c4 < 4; ++c4) {
+      for (int q = 0; q < 4; ++q) {
         uint32_t o[32];
         if (have) {
-          tc_ld_32x32b_x32(t_o + uint32_t(c4 * 32), o);
+          tc_ld_32x32b_x32(t_o + uint32_t(q * 32), o);
           tc_wait_ld();
         } else {
 #pragma unroll
@@ -420,71 +652,66 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, int* err) {
         }
         if (live) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int h = 0; h < 4; ++h) {
             float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[q * 8 + e]) * inv;
-            dst[c4 * 4 + q] = pack8(f);
+            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[h * 8 + e]) * inv;
+            dst[q * 4 + h] = pack8(f);
           }
         }
       }
-    } else if (tile < n_tiles) {
-      // this CTA's rows into the K/V stages (every MMA that read them is done),
+    } else {
+      // this group's rows into the K/V stages (every MMA that read them is done),
       // 16-byte pieces swizzled by the row so that a warp's stores spread
-      const int r = tile * kTileRows + row;
+      const int r = w * kTileRows + row;
       float* ml = reinterpret_cast<float*>(smem + kSmemML);
-      ml[r] = m;
-      ml[256 + r] = l;
+      ml[r] = have ? m : -INFINITY;
+      ml[256 + r] = have ? l : 0.0f;
 #pragma unroll 1
-      for (int c4 = 0; c4 < 4; ++c4) {
+      for (int q = 0; q < 4; ++q) {
         uint32_t o[32];
         if (have) {
-          tc_ld_32x32b_x32(t_o + uint32_t(c4 * 32), o);
+          tc_ld_32x32b_x32(t_o + uint32_t(q * 32), o);
           tc_wait_ld();
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0u;
         }
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-          st_shared_v4(sbase + kSmemKV + r * 512 + (((c4 * 8 + q) ^ (r & 31)) << 4), o[4 * q], o[4 * q + 1],
-                       o[4 * q + 2], o[4 * q + 3]);
+        for (int h = 0; h < 8; ++h)
+          st_shared_v4(sbase + kSmemKV + r * 512 + (((q * 8 + h) ^ (r & 31)) << 4), o[4 * h], o[4 * h + 1],
+                       o[4 * h + 2], o[4 * h + 3]);
       }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (splits == 1) return;
+  if (splits == 1 && !duo) return;      // (the same in every CTA of a cluster)
   cluster_sync();
-  // ---- join the splits: (row, four channels) pieces shared out over the CTAs
-  const int pieces = n_tiles * kTileRows * 32;
-  const uint32_t ml0 = sbase + kSmemML;
+  // ---- join the splits and, of a shared query tile, the groups: (row, four
+  // channels) pieces shared out over the CTAs
+  const int sets = duo ? 2 : 1, pieces = n_tiles * kTileRows * 32;
   for (int i = split * kTilesThreads + int(threadIdx.x); i < pieces; i += splits * kTilesThreads) {
     const int r = i >> 5, q = i & 31, tile = r >> 7, row = r & 127;
     const int token = (2 * pair + tile) * tp.tokens_per_tile + row / p.share;
     if (row >= tile_rows || token >= p.sq) continue;
     float mx = -INFINITY;
-    for (int k = 0; k < splits; ++k) {
-      uint32_t peer;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(ml0 + uint32_t(r * 4)), "r"(k));
-      mx = fmaxf(mx, ld_cluster_f32(peer));
-    }
+    for (int k = 0; k < splits * sets; ++k)
+      mx = fmaxf(mx, ld_cluster_f32(cluster_addr(sbase + kSmemML + uint32_t((r + k % sets * kTileRows) * 4), k / sets)));
     float sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = 0; k < splits; ++k) {
-      uint32_t peer, data;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(ml0 + uint32_t(r * 4)), "r"(k));
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                   : "=r"(data)
-                   : "r"(sbase + kSmemKV + uint32_t(r * 512 + ((q ^ (r & 31)) << 4))), "r"(k));
-      const float mk = ld_cluster_f32(peer);
+    for (int k = 0; k < splits * sets; ++k) {
+      const int rk = r + k % sets * kTileRows;
+      const uint32_t ml = cluster_addr(sbase + kSmemML + uint32_t(rk * 4), k / sets);
+      const float mk = ld_cluster_f32(ml);
       const float f = mk == -INFINITY ? 0.0f : ex2_ftz(mk - mx);
-      sum = fmaf(ld_cluster_f32(peer + 1024), f, sum);
-      const float4 x = ld_cluster_f32x4(data);
+      sum = fmaf(ld_cluster_f32(ml + 1024), f, sum);
+      const float4 x = ld_cluster_f32x4(
+          cluster_addr(sbase + kSmemKV + uint32_t(rk * 512 + ((q ^ (rk & 31)) << 4)), k / sets));
       acc.x = fmaf(x.x, f, acc.x);
       acc.y = fmaf(x.y, f, acc.y);
       acc.z = fmaf(x.z, f, acc.z);
@@ -498,36 +725,182 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, int* err) {
   cluster_sync();
 }
 
+// Clusters of `size` CTAs that the device holds at once (one CTA per SM; a
+// cluster stays within a GPU processing cluster, so this is less than SMs / size).
+template <bool WIDE>
+int resident_clusters(int size) {
+  static int cached[9] = {0};
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  if (cached[size] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(size));
+    cfg.blockDim = dim3(Roles<WIDE>::threads);
+    cfg.dynamicSmemBytes = kTilesSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(size);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, cached_attn_tiles_kernel<WIDE>, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = sm_count() / size > 0 ? sm_count() / size : 1;
+    }
+    cached[size] = n;
+  }
+  return cached[size];
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 tiles_encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* q = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) == cudaSuccess &&
+        r == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(q);
+  });
+  return fn;
+}
+
+// bf16 rows of 128 channels, boxes of 128 rows x 64 channels: [rows, 128] (d2 =
+// d3 = 0), or rows of (d3 requests, d2 heads) with element strides s1, s2, s3.
+int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t s1, int64_t d2 = 0, int64_t s2 = 0,
+             int64_t d3 = 0, int64_t s3 = 0) {
+  auto fn = tiles_encode_fn();
+  if (!fn) return set_error(QIA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[4] = {cuuint64_t(kCaD), cuuint64_t(rows), cuuint64_t(d2), cuuint64_t(d3)};
+  cuuint64_t strides[3] = {cuuint64_t(s1 * 2), cuuint64_t(s2 * 2), cuuint64_t(s3 * 2)};
+  cuuint32_t box[4] = {64u, 128u, 1u, 1u};
+  cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d2 ? 4 : 2, const_cast<void*>(base), dims, strides, box,
+                        estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(QIA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+  return QIA_OK;
+}
+
+// The kernel over groups [first, first + count), keys split over `splits`.
+template <bool WIDE>
+int launch_groups(TilesParams tp, const CUtensorMap (&tm)[4], int64_t first, int64_t count, int splits, bool after_widen,
+                  cudaStream_t st) {
+  tp.first_group = int(first);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(count * splits));
+  cfg.blockDim = dim3(Roles<WIDE>::threads);
+  cfg.dynamicSmemBytes = kTilesSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(splits);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_widen ? 2 : 1;
+  const cudaError_t e =
+      cudaLaunchKernelEx(&cfg, cached_attn_tiles_kernel<WIDE>, tp, tm[0], tm[1], tm[2], tm[3], device_error_word());
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(QIA_ERR_CUDA, "cached_attn_tiles_kernel: %s", cudaGetErrorString(e));
+  }
+  return QIA_OK;
+}
+
+// Whole waves of one CTA per SM run unsplit; what is left over splits its keys
+// so that it fills the device, when that is shorter (in key tiles, with the
+// fixed part of a CTA -- prologue and output -- as two, joining as two more).
+template <bool WIDE>
+int launch_waves(const TilesParams& tp, const CUtensorMap (&tm)[4], int64_t groups, int tiles, cudaStream_t st) {
+  static const bool ready = cudaFuncSetAttribute(cached_attn_tiles_kernel<WIDE>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kTilesSmem) == cudaSuccess;
+  if (!ready) return set_error(QIA_ERR_CUDA, "qia_cached_attention: cudaFuncSetAttribute failed");
+  const int64_t whole = groups / sm_count() * sm_count();
+  const int rest = int(groups - whole);
+  int splits = 1;
+  const auto cost = [&](int s) { return (tiles + s - 1) / s + (s > 1 ? 4 : 2); };
+  for (int s = 2; s <= 8 && s <= tiles && rest > 0; ++s)
+    if (rest <= resident_clusters<WIDE>(s) && cost(s) < cost(splits)) splits = s;
+  if (splits == 1 || whole == 0) return launch_groups<WIDE>(tp, tm, 0, groups, splits, WIDE, st);
+  const int rc = launch_groups<WIDE>(tp, tm, 0, whole, 1, WIDE, st);
+  return rc ? rc : launch_groups<WIDE>(tp, tm, whole, rest, splits, false, st);
+}
+
+// Widened operands pay from three query tiles of a request on: every pair of
+// tiles converts the codes again otherwise.
+bool use_wide(int64_t q_tiles) { return q_tiles > 2; }
+
+struct WideSizes {
+  int64_t cached_cap, fresh_cap, kv_tiles, kv_bytes, scalar_bytes;
+};
+
+WideSizes wide_sizes(int64_t batch, int64_t kv_heads, int64_t extent, int64_t seq_k, bool masked) {
+  WideSizes w;
+  w.cached_cap = (extent + 127) / 128;
+  w.fresh_cap = (seq_k + 127) / 128;
+  w.kv_tiles = w.cached_cap + (masked ? w.fresh_cap : 0);
+  w.kv_bytes = batch * kv_heads * w.kv_tiles * kTileBytes;
+  w.scalar_bytes = batch * kv_heads * (w.cached_cap + w.fresh_cap) * kScalarBytes;
+  return w;
+}
+
 }  // namespace
 
-int launch_cached_tiles(const CachedAttn& p, int batch, cudaStream_t st) {
-  static const bool ready = cudaFuncSetAttribute(cached_attn_tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 kTilesSmem) == cudaSuccess;
-  if (!ready) return set_error(QIA_ERR_CUDA, "qia_cached_attention: cudaFuncSetAttribute failed");
-  TilesParams tp;
+int64_t cached_tiles_workspace(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t share, int64_t kv_heads,
+                               int64_t extent, bool masked) {
+  const int64_t per = kTileRows / share;
+  if (!use_wide((seq_q + per - 1) / per)) return 0;
+  const WideSizes w = wide_sizes(batch, kv_heads, extent, seq_k, masked);
+  return 2 * w.kv_bytes + w.scalar_bytes;
+}
+
+int launch_cached_tiles(const CachedAttn& p, int batch, void* workspace, cudaStream_t st) {
+  const char* who = "qia_cached_attention";
+  TilesParams tp = {};
   tp.a = p;
   tp.tokens_per_tile = kTileRows / p.share;
   tp.q_tiles = (p.sq + tp.tokens_per_tile - 1) / tp.tokens_per_tile;
-  const int64_t pairs = (tp.q_tiles + 1) / 2;
-  const int64_t groups = pairs * p.kv_heads * batch;
+  tp.pairs = (tp.q_tiles + 1) / 2;
+  const int64_t groups = int64_t(tp.pairs) * p.kv_heads * batch;
+  if (groups > 0x0fffffff) return set_error(QIA_ERR_UNSUPPORTED, "%s: too many query rows", who);
   const int tiles = (p.extent + 127) / 128 + (p.sk + 127) / 128;
-  // splits of the keys: the count with the shortest schedule, in key tiles --
-  // waves of one CTA per SM, each its share of the keys plus the fixed part of
-  // a CTA (prologue, epilogue; twice that when it also joins)
-  int splits = 1;
-  double best = 1e30;
-  for (int s = 1; s <= 8 && s <= (tiles > 0 ? tiles : 1); s *= 2) {
-    const double waves = double((groups * s + sm_count() - 1) / sm_count());
-    const double cost = waves * ((tiles + s - 1) / s + (s == 1 ? 2.0 : 4.0));
-    if (cost < best) {
-      best = cost;
-      splits = s;
-    }
+  CUtensorMap tm[4] = {};
+  if (!use_wide(tp.q_tiles)) return launch_waves<false>(tp, tm, groups, tiles, st);
+
+  if (!workspace || !aligned(workspace, 128))
+    return set_error(QIA_ERR_INVALID, "%s: the workspace is null or misaligned", who);
+  const WideSizes ws = wide_sizes(batch, p.kv_heads, p.extent, p.sk, p.key_valid != nullptr);
+  if (int64_t(batch) * p.kv_heads * ws.kv_tiles * 128 > 0x7fffffff || p.kv_heads > 65535)
+    return set_error(QIA_ERR_UNSUPPORTED, "%s: too many cached tokens for one call", who);
+  uint8_t* base = (uint8_t*)workspace;
+  tp.wide.k = (__nv_bfloat16*)base;
+  tp.wide.v = (__nv_bfloat16*)(base + ws.kv_bytes);
+  tp.wide.scalars = (float*)(base + 2 * ws.kv_bytes);
+  tp.wide.cached_cap = int(ws.cached_cap);
+  tp.wide.fresh_cap = int(ws.fresh_cap);
+  tp.wide.kv_tiles = int(ws.kv_tiles);
+  int rc = QIA_OK;
+  if (ws.kv_tiles) {
+    const int64_t rows = int64_t(batch) * p.kv_heads * ws.kv_tiles * 128;
+    rc = make_map(&tm[0], tp.wide.k, rows, kCaD);
+    if (!rc) rc = make_map(&tm[1], tp.wide.v, rows, kCaD);
   }
-  if (pairs * splits > 0x7fffffff) return set_error(QIA_ERR_UNSUPPORTED, "qia_cached_attention: too many query rows");
-  return launch_cluster("qia_cached_attention", cached_attn_tiles_kernel,
-                        dim3(unsigned(pairs * splits), unsigned(p.kv_heads), unsigned(batch)), kTilesThreads,
-                        size_t(kTilesSmem), splits, st, tp, device_error_word());
+  if (!rc && p.sk && !p.key_valid) {
+    rc = make_map(&tm[2], p.k, p.sk, p.k_ss, p.kv_heads, p.k_sh, batch, p.k_sb);
+    if (!rc) rc = make_map(&tm[3], p.v, p.sk, p.v_ss, p.kv_heads, p.v_sh, batch, p.v_sb);
+  }
+  if (rc) return rc;
+  if (tiles) {
+    cached_widen_kernel<<<dim3(unsigned(tiles), unsigned(p.kv_heads), unsigned(batch)), 256, 0, st>>>(p, tp.wide);
+    rc = check_launch("cached_widen_kernel");
+    if (rc) return rc;
+  }
+  return launch_waves<true>(tp, tm, groups, tiles, st);
 }
 
 }  // namespace qia

@@ -86,7 +86,7 @@ SIGNATURES.update({
 SIGNATURES.update({
     "qia_kv_cache_write": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P],
     "qia_kv_cache_read": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P],
-    "qia_cached_attention": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P],
+    "qia_cached_attention": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P, _P],
     "qia_lora_add": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P],
 })
 
@@ -94,6 +94,7 @@ SIGNATURES.update({
 RAW_SIGNATURES: dict[str, tuple] = {
     "qia_sage_workspace_bytes": (ctypes.c_int64, [_I, _I, _I, _I]),
     "qia_ipc_handle_bytes": (ctypes.c_int64, []),
+    "qia_cached_attention_workspace_bytes": (ctypes.c_int64, [_I, _I, _I, _I, _I, _I, ctypes.c_int]),
     "qia_lora_workspace_bytes": (ctypes.c_int64, [_I, _I, _I]),
     "qia_sage_attn_ctas": (ctypes.c_int64, [_I, _I, _I]),
 }

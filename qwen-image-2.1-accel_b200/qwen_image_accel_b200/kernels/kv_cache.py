@@ -195,11 +195,14 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
         raise ValueError(f"{who}: out must be like q")
     if not out.numel():
         return out
+    size = _lib.load().qia_cached_attention_workspace_bytes(cache.batch, q.shape[1], fresh, q.shape[2], cache.kv_heads,
+                                                            cache.extent, key_valid is not None)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     kc, vc, ks, vs, lengths = cache._buffers
     rows = (*k.stride()[:3], *v.stride()[:3]) if fresh else (0,) * 6
     _lib.call("qia_cached_attention", q.data_ptr(), k.data_ptr() if fresh else None, v.data_ptr() if fresh else None,
               kc, vc, ks, vs, lengths, None if key_valid is None else key_valid.data_ptr(), out.data_ptr(),
               cache.batch, q.shape[1], fresh, q.shape[2], cache.kv_heads, HEAD_DIM, cache.capacity, cache.extent,
               _Strides12(*q.stride()[:3], *rows, *out.stride()[:3]), mask_stride,
-              0.0 if scale is None else float(scale), _lib.stream(q.device))
+              0.0 if scale is None else float(scale), _lib.ptr(ws), _lib.stream(q.device))
     return out
