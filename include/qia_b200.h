@@ -610,8 +610,8 @@ int qia_kv_cache_read(const void* k_codes, const void* v_codes,
  * 1/sqrt(128). Products of exact INT8 codes (cached) or bf16 rows (fresh),
  * fp32 scores, sums and accumulators; softmax weights are rounded once for the
  * second product. head_dim = 128, heads / kv_heads <= 128. workspace:
- * qia_cached_attention_workspace_bytes bytes of device memory (masked: whether
- * key_valid is given), 128-byte aligned (NULL when that is 0). */
+ * qia_cached_attention_workspace_bytes bytes of device memory, 128-byte
+ * aligned (NULL when that is 0). */
 int qia_cached_attention(const void* q, const void* k, const void* v,
                          const void* k_codes, const void* v_codes,
                          const void* k_scales, const void* v_scales,
@@ -623,8 +623,7 @@ int qia_cached_attention(const void* q, const void* k, const void* v,
                          void* stream);
 int64_t qia_cached_attention_workspace_bytes(int64_t batch, int64_t seq_q,
                                              int64_t seq_k, int64_t heads,
-                                             int64_t kv_heads, int64_t extent,
-                                             int masked);
+                                             int64_t kv_heads, int64_t extent);
 
 /* ---------------------------------------------------------------------------
  * Low-rank adapters, one per request, beside a shared projection (no

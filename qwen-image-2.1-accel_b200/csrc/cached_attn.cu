@@ -474,11 +474,11 @@ using namespace qia;
 static bool use_rows(int64_t seq_q, int64_t share) { return seq_q * share <= 16; }
 
 extern "C" int64_t qia_cached_attention_workspace_bytes(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t heads,
-                                                        int64_t kv_heads, int64_t extent, int masked) {
+                                                        int64_t kv_heads, int64_t extent) {
   if (batch <= 0 || seq_q <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || heads / kv_heads > 128 ||
-      use_rows(seq_q, heads / kv_heads))
+      use_rows(seq_q, heads / kv_heads) || !cached_use_wide(seq_q, heads / kv_heads))
     return 0;
-  return cached_tiles_workspace(batch, seq_q, seq_k, heads / kv_heads, kv_heads, extent, masked != 0);
+  return cached_wide_workspace(batch, seq_k, kv_heads, extent);
 }
 
 extern "C" int qia_cached_attention(const void* q, const void* k, const void* v, const void* k_codes,
@@ -537,12 +537,6 @@ extern "C" int qia_cached_attention(const void* q, const void* k, const void* v,
   p.scale_log2 = (sm_scale > 0.0f ? sm_scale : 0.08838834764831845f) * 1.4426950408889634f;
   // rows that share a K/V head fill one 16-row tile, or the tensor-core tiles
   if (use_rows(seq_q, p.share)) return launch_cached_rows(p, int(batch), as_stream(stream));
-  // a zero stride (broadcast k or v) is not a tensor map's: such rows are given another stride where
-  // it does not matter, and refused where it does
-  if (batch == 1) p.k_sb = p.v_sb = kCaD;
-  if (kv_heads == 1) p.k_sh = p.v_sh = kCaD;
-  if (seq_k == 1) p.k_ss = p.v_ss = kCaD;
-  if (seq_k > 0 && (p.k_sb <= 0 || p.v_sb <= 0 || p.k_sh <= 0 || p.v_sh <= 0 || p.k_ss <= 0 || p.v_ss <= 0))
-    return set_error(QIA_ERR_UNSUPPORTED, "%s: k and v may not be broadcast views", who);
-  return launch_cached_tiles(p, int(batch), workspace, as_stream(stream));
+  if (!cached_use_wide(seq_q, p.share)) return launch_cached_tiles(p, int(batch), as_stream(stream));
+  return launch_cached_wide(p, int(batch), workspace, as_stream(stream));
 }

@@ -62,10 +62,14 @@ __device__ __forceinline__ KeyScalars key_scalars(const CachedAttn& p, float ks,
   return r;
 }
 
-int launch_cached_rows(const CachedAttn& p, int batch, cudaStream_t st);    // few query rows (cached_attn.cu)
-int launch_cached_tiles(const CachedAttn& p, int batch, void* workspace, cudaStream_t st);   // many (cached_attn_tiles.cu)
-int64_t cached_tiles_workspace(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t share, int64_t kv_heads,
-                               int64_t extent, bool masked);
+// The forms by query rows per K/V head (seq_q * share): one 16-row tile
+// (cached_attn.cu), up to two 128-row tiles (cached_attn_tiles.cu), more
+// (cached_attn_wide.cu, which needs a workspace).
+int launch_cached_rows(const CachedAttn& p, int batch, cudaStream_t st);
+int launch_cached_tiles(const CachedAttn& p, int batch, cudaStream_t st);
+int launch_cached_wide(const CachedAttn& p, int batch, void* workspace, cudaStream_t st);
+bool cached_use_wide(int64_t seq_q, int64_t share);
+int64_t cached_wide_workspace(int64_t batch, int64_t seq_k, int64_t kv_heads, int64_t extent);
 
 __device__ __forceinline__ float ex2_ftz(float x) {
   float y;

@@ -1,11 +1,11 @@
-// Attention of many query rows over the INT8 prefix cache: 256 query rows per
-// CTA on tcgen05.
+// Attention of some tens to some hundreds of query rows over the INT8 prefix
+// cache (at most two tiles of 128 rows per request and K/V head), on tcgen05.
 //
-// Roles (384 threads, one CTA per SM):
+// Roles (512 threads, one CTA per SM):
 //   warps 0-3, 4-7  softmax groups 0 and 1 (a query row per thread): scores from
 //                   TMEM, weights back into TMEM;
 //   warp 8          issues the MMAs;
-//   warps 9-11      operand writers: INT8 codes -> bf16 (exact), fresh bf16 rows
+//   warps 9-15      operand writers: INT8 codes -> bf16 (exact), fresh bf16 rows
 //                   copied, into the swizzled shared-memory tiles, and the
 //                   per-key numbers of the softmax.
 // A key tile is 128 keys. K and V tiles (32 KB each) have two stages. TMEM:
@@ -32,36 +32,19 @@
 // Keys may be split over a cluster, which joins through distributed shared
 // memory in rank order (no workspace, fixed order). Every wait is bounded (1 s)
 // and reports QIA_ERR_TIMEOUT through the device error word.
-#include <cudaTypedefs.h>
-
-#include <mutex>
-
-#include "cached_attn.cuh"
-#include "cluster.cuh"
-#include "sm100.cuh"
+#include "cached_attn_tc.cuh"
 
 namespace qia {
 namespace {
 
-constexpr int kTileRows = 128;                 // query rows per tile, keys per tile
-constexpr int kTileBytes = kTileRows * kCaD * 2;   // 32 KB: two 64-channel panels of 16 KB
-constexpr int kPanel = kTileBytes / 2;
-constexpr int kSmemQ = 0;
-constexpr int kSmemKV = 2 * kTileBytes;        // stage s: K at 2 s, V at 2 s + 1
-constexpr int kScalarRing = 4;
-constexpr int kScalarBytes = 3 * 128 * 4;      // [sk | vs | bias][128] f32
-constexpr int kSmemScal = kSmemKV + 4 * kTileBytes;
-constexpr int kSmemML = kSmemScal + kScalarRing * kScalarBytes;       // m, l of 256 rows (joining)
+constexpr int kThreads = 512;
+constexpr int kWriters = 7;                     // operand-writer warps: arrivals of a written tile
+constexpr int kScalarBytes = 3 * 128 * 4;       // [sk | vs | bias][128] f32
+constexpr int kSmemML = kSmemTail + kScalarRing * kScalarBytes;   // m, l of 256 rows (joining)
 constexpr int kSmemBars = kSmemML + 2 * 256 * 4;
-constexpr int kTilesSmem = kSmemBars + 256 + 1024;
-// Warps, and the registers of a softmax and of any other thread: the shares add
-// up to what the block starts with (384 x 168, 512 x 128).
-template <bool WIDE>
-struct Roles {
-  static constexpr int threads = WIDE ? 384 : 512;
-  static constexpr int writers = WIDE ? 1 : 7;         // arrivals of a written operand tile
-  static constexpr int softmax_regs = WIDE ? 208 : 160, other_regs = WIDE ? 88 : 96;
-};
+constexpr int kSmemBytes = kSmemBars + 256 + 1024;
+// registers of a softmax thread and of any other: 256 x 160 + 256 x 96 = 512 x 128, what the block starts with
+constexpr int kSoftmaxRegs = 160, kOtherRegs = 96;
 constexpr float kTilesLag = 8.0f;
 constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 constexpr uint32_t kIdescO = kIdescS | (1u << 16);   // B (V) is MN-major
@@ -73,123 +56,12 @@ __device__ __forceinline__ void cp_async16_zfill(uint32_t smem, const void* gmem
 }
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
 // bf16 pair of two codes of `w` (bytes picked by `sel`)
 __device__ __forceinline__ uint32_t codes_bf16x2(uint32_t w, uint32_t sel) {
   const uint32_t t = __byte_perm(w, 0x43434343u, sel);
   uint32_t r;
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t & 0xff7fff7fu), "r"(t & 0xff80ff80u));
   return r;
-}
-
-// Shared-memory offset of 16-byte piece `piece` (0..15) of row `row` in a tile.
-__device__ __forceinline__ uint32_t tile_offset(int row, int piece) {
-  return uint32_t((piece >> 3) * kPanel + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
-}
-
-__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
-  uint32_t out;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
-  return out;
-}
-
-// Operands widened ahead of the products, per (request, K/V head): the cached
-// tiles (cached_cap of them) and, when keys are masked, the fresh tiles behind
-// them as bf16 rows (masked and missing ones zeros), and the per-key numbers of
-// all tiles.
-struct Widened {
-  __nv_bfloat16* k;      // [B Hkv, kv_tiles * 128, 128]
-  __nv_bfloat16* v;
-  float* scalars;        // [B Hkv, cached_cap + fresh_cap, 3, 128]
-  int cached_cap, fresh_cap, kv_tiles;
-};
-
-struct TilesParams {
-  CachedAttn a;
-  Widened wide;
-  int tokens_per_tile;   // query tokens in a tile of 128 rows: 128 / share
-  int q_tiles, pairs;    // tiles of a request, and pairs of them
-  int first_group;       // group = (request, K/V head, pair), pairs fastest
-};
-
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
-          "r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
-
-// One CTA per (key tile, K/V head, request): fills Widened. Bytes only: one in
-// and two out per code.
-__global__ void __launch_bounds__(256) cached_widen_kernel(const __grid_constant__ CachedAttn p,
-                                                           const __grid_constant__ Widened w) {
-  const int tile = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-  grid_launch_dependents();
-  const bool cached = tile < w.cached_cap;
-  const int len = cached_len(p, b), end = cached ? len : p.sk, k0 = (cached ? tile : tile - w.cached_cap) * 128;
-  if (k0 >= end) return;
-  const int group = b * p.kv_heads + kvh;
-  const int64_t head_row = int64_t(group) * p.capacity;
-  const uint8_t* mask = p.key_valid ? p.key_valid + b * p.mask_sb + (cached ? 0 : p.extent) : nullptr;
-  if (threadIdx.x < 128) {
-    const int key = k0 + threadIdx.x;
-    const bool held = key < end, valid = held && (!mask || __ldg(mask + key) != 0);
-    float* dst = w.scalars + (int64_t(group) * (w.cached_cap + w.fresh_cap) + tile) * 384 + threadIdx.x;
-    const float ks = valid && cached ? __ldg(p.ks + head_row + key) : 1.0f;
-    dst[0] = valid ? p.scale_log2 * ks : 0.0f;
-    dst[128] = !valid ? 0.0f : cached ? __ldg(p.vs + head_row + key) : 1.0f;
-    dst[256] = valid ? 0.0f : -INFINITY;
-  }
-  if (tile >= w.kv_tiles) return;
-  const int64_t row0 = (int64_t(group) * w.kv_tiles + tile) * 128;
-  if (cached) {
-#pragma unroll
-    for (int z = 0; z < 2; ++z) {
-      const int8_t* src = (z ? p.vc : p.kc) + head_row * kCaD;
-      __nv_bfloat16* dst = (z ? w.v : w.k) + row0 * kCaD;
-      uint4 c[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = i * 32 + (threadIdx.x >> 3), key = k0 + row;
-        c[i] = key < end ? __ldg(reinterpret_cast<const uint4*>(src + int64_t(key) * kCaD) + (threadIdx.x & 7))
-                         : make_uint4(0u, 0u, 0u, 0u);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = i * 32 + (threadIdx.x >> 3);
-        uint4* out = reinterpret_cast<uint4*>(dst + int64_t(row) * kCaD) + 2 * (threadIdx.x & 7);
-        st_global_v8(out,
-                     make_uint4(codes_bf16x2(c[i].x, 0x4140), codes_bf16x2(c[i].x, 0x4342),
-                                codes_bf16x2(c[i].y, 0x4140), codes_bf16x2(c[i].y, 0x4342)),
-                     make_uint4(codes_bf16x2(c[i].z, 0x4140), codes_bf16x2(c[i].z, 0x4342),
-                                codes_bf16x2(c[i].w, 0x4140), codes_bf16x2(c[i].w, 0x4342)));
-      }
-    }
-  } else {
-#pragma unroll
-    for (int z = 0; z < 2; ++z) {
-      const __nv_bfloat16* src = z ? p.v + b * p.v_sb + kvh * p.v_sh : p.k + b * p.k_sb + kvh * p.k_sh;
-      const int64_t ss = z ? p.v_ss : p.k_ss;
-      __nv_bfloat16* dst = (z ? w.v : w.k) + row0 * kCaD;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = i * 16 + (threadIdx.x >> 4), key = k0 + row;
-        const bool valid = key < end && (!mask || __ldg(mask + key) != 0);
-        reinterpret_cast<uint4*>(dst + int64_t(row) * kCaD)[threadIdx.x & 15] =
-            valid ? __ldg(reinterpret_cast<const uint4*>(src + int64_t(key) * ss) + (threadIdx.x & 15))
-                  : make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
-  }
 }
 
 // The 128 scores of a row in registers -> their maximum, and for tiles with
@@ -251,17 +123,10 @@ __device__ __forceinline__ void row_weights(const uint32_t (&s)[128], int h, con
   }
 }
 
-// WIDE: operands come by TMA, cached ones (and masked fresh ones) from Widened,
-// fresh ones straight from k and v; else seven warps write them from the codes.
-template <bool WIDE>
-__global__ void __launch_bounds__(Roles<WIDE>::threads, 1)
-cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, const __grid_constant__ CUtensorMap tm_wk,
-                         const __grid_constant__ CUtensorMap tm_wv, const __grid_constant__ CUtensorMap tm_k,
-                         const __grid_constant__ CUtensorMap tm_v, int* err) {
-  constexpr int kTilesThreads = Roles<WIDE>::threads, kWriters = Roles<WIDE>::writers;
+__global__ void __launch_bounds__(kThreads, 1)
+cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_constant__ TileGrid tp, int* err) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const CachedAttn& p = tp.a;
   const uint32_t sbase = smem_u32(smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemBars);
   uint64_t* k_full = bars;            // [2] operand writers -> issuer
@@ -304,7 +169,7 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, const __grid_co
   if (warp == 8) tmem_alloc(smem_u32(tmem_slot), 512);
   // ---- query tiles (rows past the end are zeros)
   const int tile_rows = tp.tokens_per_tile * p.share;
-  for (int i = threadIdx.x; i < n_tiles * kTileRows * 16; i += kTilesThreads) {
+  for (int i = threadIdx.x; i < n_tiles * kTileRows * 16; i += kThreads) {
     const int tile = i >> 11, row = (i >> 4) & 127, piece = i & 15;
     const int token = (2 * pair + tile) * tp.tokens_per_tile + row / p.share;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -322,7 +187,7 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, const __grid_co
   const auto tiles_of = [&](int w) { return duo ? (n - w + 1) / 2 : n; };
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Roles<WIDE>::other_regs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
       // ------------------------------------------------------------ MMA issuer
       if (lane == 0 && n > 0) {
@@ -401,48 +266,6 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, const __grid_co
         mbar_wait(smem_u32(drain), 0, ok ? err : nullptr, 100000000ull);
       }
       __syncwarp();
-    } else if constexpr (WIDE) {
-      // ---------------------------------------------------------- TMA producer
-      if (warp == 9 && lane == 0 && n > 0) {
-        const int bh = b * p.kv_heads + kvh;
-        bool ok = true;
-        grid_wait();                           // the operands are widened
-        int issued = 0;
-        for (int u = 0; u < 2 * n && ok; ++u) {
-          const int j = u >> 1, tile = first + j, st = j & 1;
-          if (!(u & 1)) {                      // (ring slot j % 4: tile j - 4 was done before V of j - 3 left)
-            const uint32_t bar = smem_u32(&scal_full[j % kScalarRing]);
-            const int at = tile < cached_tiles ? tile : tp.wide.cached_cap + tile - cached_tiles;
-            mbar_arrive_expect_tx(bar, kScalarBytes);
-            bulk_load(sbase + kSmemScal + uint32_t(j % kScalarRing) * kScalarBytes,
-                      tp.wide.scalars + (int64_t(bh) * (tp.wide.cached_cap + tp.wide.fresh_cap) + at) * 384,
-                      kScalarBytes, bar);
-          }
-          ok = mbar_wait(smem_u32((u & 1) ? &v_empty[st] : &k_empty[st]), ((j >> 1) & 1) ^ 1, err);
-          if (!ok) break;
-          const uint32_t bar = smem_u32((u & 1) ? &v_full[st] : &k_full[st]);
-          const uint32_t slot = sbase + kSmemKV + uint32_t(st * 2 + (u & 1)) * kTileBytes;
-          mbar_arrive_expect_tx(bar, kTileBytes);
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t dst = slot + uint32_t(h * kPanel);
-            if (tile < cached_tiles || p.key_valid) {
-              const int at = tile < cached_tiles ? tile : tp.wide.cached_cap + tile - cached_tiles;
-              tma_load_2d(dst, (u & 1) ? &tm_wv : &tm_wk, bar, h * 64, (bh * tp.wide.kv_tiles + at) * 128);
-            } else {
-              tma_load_4d(dst, (u & 1) ? &tm_v : &tm_k, bar, h * 64, (tile - cached_tiles) * 128, kvh, b);
-            }
-          }
-          issued = u + 1;
-        }
-        if (!ok) {   // let queued copies land before the shared memory is released
-          for (int u = max(0, issued - 4); u < issued; ++u)
-            mbar_wait(smem_u32((u & 1) ? &v_full[(u >> 1) & 1] : &k_full[(u >> 1) & 1]), (u >> 2) & 1, nullptr,
-                      100000000ull);
-          for (int j = max(0, (issued + 1) / 2 - kScalarRing); j <= issued / 2; ++j)
-            mbar_wait(smem_u32(&scal_full[j % kScalarRing]), (j / kScalarRing) & 1, nullptr, 100000000ull);
-        }
-      }
-      __syncwarp();
     } else {
       // ------------------------------------------------------- operand writers
       const int t = threadIdx.x - 32 * 9;
@@ -500,7 +323,7 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, const __grid_co
       };
       const auto store_scalars = [&](int j) {
         if (t < 128) {
-          float* dst = reinterpret_cast<float*>(smem + kSmemScal + (j % kScalarRing) * kScalarBytes) + t;
+          float* dst = reinterpret_cast<float*>(smem + kSmemTail + (j % kScalarRing) * kScalarBytes) + t;
           dst[0] = valid ? p.scale_log2 * ks : 0.0f;
           dst[128] = valid ? vs : 0.0f;
           dst[256] = valid ? 0.0f : -INFINITY;
@@ -569,7 +392,7 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, const __grid_co
     }
   } else {
     // ----------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Roles<WIDE>::softmax_regs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int w = warp >> 2;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + t_lane + uint32_t(128 * w), t_o = tmem + t_lane + uint32_t(256 + 128 * w);
@@ -588,7 +411,7 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, const __grid_co
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         tc_ld_32x32b_x32(t_s + uint32_t(q * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[q * 32]));
-      const float* scal = reinterpret_cast<const float*>(smem + kSmemScal + (j % kScalarRing) * kScalarBytes);
+      const float* scal = reinterpret_cast<const float*>(smem + kSmemTail + (j % kScalarRing) * kScalarBytes);
       const int tile = first + j, tail = tile < cached_tiles ? len - tile * 128 : p.sk - (tile - cached_tiles) * 128;
       const int kind = p.key_valid || tail < 128 ? kMasked : tile < cached_tiles ? kCachedFull : kFreshFull;
       tc_wait_ld();
@@ -634,55 +457,12 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, const __grid_co
     tc_fence_after();
     // ------------------------------------------------------------------ output
     const int row = (warp & 3) * 32 + lane;
-    if (splits == 1 && !duo) {
-      const int token = (2 * pair + w) * tp.tokens_per_tile + row / p.share;
-      const bool live = row < tile_rows && token < p.sq;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      uint4* dst = reinterpret_cast<uint4*>(p.out + b * p.o_sb + int64_t(token) * p.o_ss +
-                                            int64_t(kvh * p.share + row % p.share) * p.o_sh);
-#pragma unroll 1
-      for (int q = 0; q < 4; ++q) {
-        uint32_t o[32];
-        if (have) {
-          tc_ld_32x32b_x32(t_o + uint32_t(q * 32), o);
-          tc_wait_ld();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
-        }
-        if (live) {
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            float f[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[h * 8 + e]) * inv;
-            dst[q * 4 + h] = pack8(f);
-          }
-        }
-      }
-    } else {
-      // this group's rows into the K/V stages (every MMA that read them is done),
-      // 16-byte pieces swizzled by the row so that a warp's stores spread
-      const int r = w * kTileRows + row;
-      float* ml = reinterpret_cast<float*>(smem + kSmemML);
-      ml[r] = have ? m : -INFINITY;
-      ml[256 + r] = have ? l : 0.0f;
-#pragma unroll 1
-      for (int q = 0; q < 4; ++q) {
-        uint32_t o[32];
-        if (have) {
-          tc_ld_32x32b_x32(t_o + uint32_t(q * 32), o);
-          tc_wait_ld();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
-        }
-#pragma unroll
-        for (int h = 0; h < 8; ++h)
-          st_shared_v4(sbase + kSmemKV + r * 512 + (((q * 8 + h) ^ (r & 31)) << 4), o[4 * h], o[4 * h + 1],
-                       o[4 * h + 2], o[4 * h + 3]);
-      }
-    }
+    const int token = (2 * pair + w) * tp.tokens_per_tile + row / p.share;
+    if (splits == 1 && !duo)
+      store_row(t_o, have, l, row < tile_rows && token < p.sq,
+                p.out + b * p.o_sb + int64_t(token) * p.o_ss + int64_t(kvh * p.share + row % p.share) * p.o_sh);
+    else
+      stage_row(t_o, have, m, l, sbase, reinterpret_cast<float*>(smem + kSmemML), w * kTileRows + row);
   }
   tc_fence_before();
   __syncthreads();
@@ -690,217 +470,28 @@ cached_attn_tiles_kernel(const __grid_constant__ TilesParams tp, const __grid_co
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (splits == 1 && !duo) return;      // (the same in every CTA of a cluster)
-  cluster_sync();
-  // ---- join the splits and, of a shared query tile, the groups: (row, four
-  // channels) pieces shared out over the CTAs
-  const int sets = duo ? 2 : 1, pieces = n_tiles * kTileRows * 32;
-  for (int i = split * kTilesThreads + int(threadIdx.x); i < pieces; i += splits * kTilesThreads) {
-    const int r = i >> 5, q = i & 31, tile = r >> 7, row = r & 127;
-    const int token = (2 * pair + tile) * tp.tokens_per_tile + row / p.share;
-    if (row >= tile_rows || token >= p.sq) continue;
-    float mx = -INFINITY;
-    for (int k = 0; k < splits * sets; ++k)
-      mx = fmaxf(mx, ld_cluster_f32(cluster_addr(sbase + kSmemML + uint32_t((r + k % sets * kTileRows) * 4), k / sets)));
-    float sum = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = 0; k < splits * sets; ++k) {
-      const int rk = r + k % sets * kTileRows;
-      const uint32_t ml = cluster_addr(sbase + kSmemML + uint32_t(rk * 4), k / sets);
-      const float mk = ld_cluster_f32(ml);
-      const float f = mk == -INFINITY ? 0.0f : ex2_ftz(mk - mx);
-      sum = fmaf(ld_cluster_f32(ml + 1024), f, sum);
-      const float4 x = ld_cluster_f32x4(
-          cluster_addr(sbase + kSmemKV + uint32_t(rk * 512 + ((q ^ (rk & 31)) << 4)), k / sets));
-      acc.x = fmaf(x.x, f, acc.x);
-      acc.y = fmaf(x.y, f, acc.y);
-      acc.z = fmaf(x.z, f, acc.z);
-      acc.w = fmaf(x.w, f, acc.w);
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const float f[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-    *reinterpret_cast<uint2*>(p.out + b * p.o_sb + int64_t(token) * p.o_ss +
-                              int64_t(kvh * p.share + row % p.share) * p.o_sh + 4 * q) = pack4(f);
-  }
-  cluster_sync();
-}
-
-// Clusters of `size` CTAs that the device holds at once (one CTA per SM; a
-// cluster stays within a GPU processing cluster, so this is less than SMs / size).
-template <bool WIDE>
-int resident_clusters(int size) {
-  static int cached[9] = {0};
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lock(mu);
-  if (cached[size] == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(size));
-    cfg.blockDim = dim3(Roles<WIDE>::threads);
-    cfg.dynamicSmemBytes = kTilesSmem;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = unsigned(size);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, cached_attn_tiles_kernel<WIDE>, &cfg) != cudaSuccess || n <= 0) {
-      cudaGetLastError();
-      n = sm_count() / size > 0 ? sm_count() / size : 1;
-    }
-    cached[size] = n;
-  }
-  return cached[size];
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 tiles_encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* q = nullptr;
-    cudaDriverEntryPointQueryResult r;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) == cudaSuccess &&
-        r == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(q);
-  });
-  return fn;
-}
-
-// bf16 rows of 128 channels, boxes of 128 rows x 64 channels: [rows, 128] (d2 =
-// d3 = 0), or rows of (d3 requests, d2 heads) with element strides s1, s2, s3.
-int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t s1, int64_t d2 = 0, int64_t s2 = 0,
-             int64_t d3 = 0, int64_t s3 = 0) {
-  auto fn = tiles_encode_fn();
-  if (!fn) return set_error(QIA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  cuuint64_t dims[4] = {cuuint64_t(kCaD), cuuint64_t(rows), cuuint64_t(d2), cuuint64_t(d3)};
-  cuuint64_t strides[3] = {cuuint64_t(s1 * 2), cuuint64_t(s2 * 2), cuuint64_t(s3 * 2)};
-  cuuint32_t box[4] = {64u, 128u, 1u, 1u};
-  cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d2 ? 4 : 2, const_cast<void*>(base), dims, strides, box,
-                        estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(QIA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
-  return QIA_OK;
-}
-
-// The kernel over groups [first, first + count), keys split over `splits`.
-template <bool WIDE>
-int launch_groups(TilesParams tp, const CUtensorMap (&tm)[4], int64_t first, int64_t count, int splits, bool after_widen,
-                  cudaStream_t st) {
-  tp.first_group = int(first);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(count * splits));
-  cfg.blockDim = dim3(Roles<WIDE>::threads);
-  cfg.dynamicSmemBytes = kTilesSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = unsigned(splits);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = after_widen ? 2 : 1;
-  const cudaError_t e =
-      cudaLaunchKernelEx(&cfg, cached_attn_tiles_kernel<WIDE>, tp, tm[0], tm[1], tm[2], tm[3], device_error_word());
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return set_error(QIA_ERR_CUDA, "cached_attn_tiles_kernel: %s", cudaGetErrorString(e));
-  }
-  return QIA_OK;
-}
-
-// Whole waves of one CTA per SM run unsplit; what is left over splits its keys
-// so that it fills the device, when that is shorter (in key tiles, with the
-// fixed part of a CTA -- prologue and output -- as two, joining as two more).
-template <bool WIDE>
-int launch_waves(const TilesParams& tp, const CUtensorMap (&tm)[4], int64_t groups, int tiles, cudaStream_t st) {
-  static const bool ready = cudaFuncSetAttribute(cached_attn_tiles_kernel<WIDE>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kTilesSmem) == cudaSuccess;
-  if (!ready) return set_error(QIA_ERR_CUDA, "qia_cached_attention: cudaFuncSetAttribute failed");
-  const int64_t whole = groups / sm_count() * sm_count();
-  const int rest = int(groups - whole);
-  int splits = 1;
-  const auto cost = [&](int s) { return (tiles + s - 1) / s + (s > 1 ? 4 : 2); };
-  for (int s = 2; s <= 8 && s <= tiles && rest > 0; ++s)
-    if (rest <= resident_clusters<WIDE>(s) && cost(s) < cost(splits)) splits = s;
-  if (splits == 1 || whole == 0) return launch_groups<WIDE>(tp, tm, 0, groups, splits, WIDE, st);
-  const int rc = launch_groups<WIDE>(tp, tm, 0, whole, 1, WIDE, st);
-  return rc ? rc : launch_groups<WIDE>(tp, tm, whole, rest, splits, false, st);
-}
-
-// Widened operands pay from three query tiles of a request on: every pair of
-// tiles converts the codes again otherwise.
-bool use_wide(int64_t q_tiles) { return q_tiles > 2; }
-
-struct WideSizes {
-  int64_t cached_cap, fresh_cap, kv_tiles, kv_bytes, scalar_bytes;
-};
-
-WideSizes wide_sizes(int64_t batch, int64_t kv_heads, int64_t extent, int64_t seq_k, bool masked) {
-  WideSizes w;
-  w.cached_cap = (extent + 127) / 128;
-  w.fresh_cap = (seq_k + 127) / 128;
-  w.kv_tiles = w.cached_cap + (masked ? w.fresh_cap : 0);
-  w.kv_bytes = batch * kv_heads * w.kv_tiles * kTileBytes;
-  w.scalar_bytes = batch * kv_heads * (w.cached_cap + w.fresh_cap) * kScalarBytes;
-  return w;
+  if (splits > 1 || duo)     // (the same in every CTA of a cluster)
+    join_rows(p, tp, sbase, sbase + kSmemML, splits, split, duo ? 2 : 1, n_tiles, pair, kvh, b);
 }
 
 }  // namespace
 
-int64_t cached_tiles_workspace(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t share, int64_t kv_heads,
-                               int64_t extent, bool masked) {
-  const int64_t per = kTileRows / share;
-  if (!use_wide((seq_q + per - 1) / per)) return 0;
-  const WideSizes w = wide_sizes(batch, kv_heads, extent, seq_k, masked);
-  return 2 * w.kv_bytes + w.scalar_bytes;
-}
-
-int launch_cached_tiles(const CachedAttn& p, int batch, void* workspace, cudaStream_t st) {
-  const char* who = "qia_cached_attention";
-  TilesParams tp = {};
-  tp.a = p;
-  tp.tokens_per_tile = kTileRows / p.share;
-  tp.q_tiles = (p.sq + tp.tokens_per_tile - 1) / tp.tokens_per_tile;
-  tp.pairs = (tp.q_tiles + 1) / 2;
-  const int64_t groups = int64_t(tp.pairs) * p.kv_heads * batch;
-  if (groups > 0x0fffffff) return set_error(QIA_ERR_UNSUPPORTED, "%s: too many query rows", who);
-  const int tiles = (p.extent + 127) / 128 + (p.sk + 127) / 128;
-  CUtensorMap tm[4] = {};
-  if (!use_wide(tp.q_tiles)) return launch_waves<false>(tp, tm, groups, tiles, st);
-
-  if (!workspace || !aligned(workspace, 128))
-    return set_error(QIA_ERR_INVALID, "%s: the workspace is null or misaligned", who);
-  const WideSizes ws = wide_sizes(batch, p.kv_heads, p.extent, p.sk, p.key_valid != nullptr);
-  if (int64_t(batch) * p.kv_heads * ws.kv_tiles * 128 > 0x7fffffff || p.kv_heads > 65535)
-    return set_error(QIA_ERR_UNSUPPORTED, "%s: too many cached tokens for one call", who);
-  uint8_t* base = (uint8_t*)workspace;
-  tp.wide.k = (__nv_bfloat16*)base;
-  tp.wide.v = (__nv_bfloat16*)(base + ws.kv_bytes);
-  tp.wide.scalars = (float*)(base + 2 * ws.kv_bytes);
-  tp.wide.cached_cap = int(ws.cached_cap);
-  tp.wide.fresh_cap = int(ws.fresh_cap);
-  tp.wide.kv_tiles = int(ws.kv_tiles);
-  int rc = QIA_OK;
-  if (ws.kv_tiles) {
-    const int64_t rows = int64_t(batch) * p.kv_heads * ws.kv_tiles * 128;
-    rc = make_map(&tm[0], tp.wide.k, rows, kCaD);
-    if (!rc) rc = make_map(&tm[1], tp.wide.v, rows, kCaD);
-  }
-  if (!rc && p.sk && !p.key_valid) {
-    rc = make_map(&tm[2], p.k, p.sk, p.k_ss, p.kv_heads, p.k_sh, batch, p.k_sb);
-    if (!rc) rc = make_map(&tm[3], p.v, p.sk, p.v_ss, p.kv_heads, p.v_sh, batch, p.v_sb);
-  }
-  if (rc) return rc;
-  if (tiles) {
-    cached_widen_kernel<<<dim3(unsigned(tiles), unsigned(p.kv_heads), unsigned(batch)), 256, 0, st>>>(p, tp.wide);
-    rc = check_launch("cached_widen_kernel");
-    if (rc) return rc;
-  }
-  return launch_waves<true>(tp, tm, groups, tiles, st);
+int launch_cached_tiles(const CachedAttn& p, int batch, cudaStream_t st) {
+  static const bool ready = cudaFuncSetAttribute(cached_attn_tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 kSmemBytes) == cudaSuccess;
+  if (!ready) return set_error(QIA_ERR_CUDA, "qia_cached_attention: cudaFuncSetAttribute failed");
+  TileGrid g = tile_grid(p);
+  const int64_t groups = int64_t(g.pairs) * p.kv_heads * batch;
+  if (groups > 0x0fffffff) return set_error(QIA_ERR_UNSUPPORTED, "qia_cached_attention: too many query rows");
+  static int resident[9] = {0};
+  return launch_waves(
+      groups, (p.extent + 127) / 128 + (p.sk + 127) / 128,
+      [&](int s) { return resident_clusters(cached_attn_tiles_kernel, kThreads, kSmemBytes, s, resident); },
+      [&](int64_t first, int64_t count, int splits, bool) {
+        g.first_group = int(first);
+        return launch_cluster("cached_attn_tiles_kernel", cached_attn_tiles_kernel, dim3(unsigned(count * splits)),
+                              kThreads, size_t(kSmemBytes), splits, st, p, g, device_error_word());
+      });
 }
 
 }  // namespace qia

@@ -1,0 +1,572 @@
+// Attention of many query rows over the INT8 prefix cache (more than two query
+// tiles per request and K/V head): the keys are widened once, then every group
+// of 256 query rows streams them by TMA.
+//
+// cached_widen_kernel writes, per (request, K/V head), the cached and the fresh
+// keys as f16 rows, each tile of 128 keys scaled by powers of two of its own:
+//   kw_j = ks_j kc_j 2^-e,  vw_j = vs_j vc_j 2^-f     (masked keys: zeros)
+// with the tile's largest |ks|, |vs| just inside 2^14. f16 keeps eleven bits down
+// to 2^-28 of that, an eighth of bf16's rounding, and no factor is left per key:
+// with x = q_i . kw_j (q_i scaled by a power of two per row),
+//   t_ij = x c_i + f,  c_i = c log2e 2^(e + e_i)        log2 of the weight of vw_j
+//   w_ij = 2^(t_ij - M_i + 8)
+//   o_i  = sum_j w_ij vw_j / sum_tiles 2^-f sum_j w_ij
+// so a score costs half a maximum, half a multiply-add, one exponential, half an
+// addition and half a conversion, and the softmax reads 32 bytes per tile. (With
+// the scales as per-key numbers in shared memory it took 5700 cycles a step of
+// 256 x 128 scores instead of 4200: the broadcast reads compete with the MMA
+// operands.) The widening moves 3 bytes per code, once, instead of converting
+// them again in every CTA.
+//
+// Roles (384 threads, one CTA per SM): warps 0-3 and 4-7 softmax of the two query
+// tiles (a row per thread), warp 8 issues the MMAs, warp 9 the TMA loads. TMEM:
+// scores of tile i at columns [128 i, +128), its f16 weights over the first 64 of
+// them (the A operand of P.V), accumulators at 256 + 128 i. The issuer runs, per
+// query tile: P(j).V(j), as each half of P(j) is stored, then Q.K(j+1), so while
+// one tile's products run, the other tile's softmax works. MMAs of one thread
+// complete in order: Q.K(j+1) may overwrite the scores that hold P(j), and once
+// its scores are there, the accumulators hold all of P.V up to j and the softmax
+// may rescale them (only when a row's maximum grew by more than 2^7; f16 weights
+// are at most 2^15).
+//
+// What bounds it: per key tile 4 x 512 tensor cycles and 2 x 1024 cycles of
+// exponentials per SM.
+#include <cuda_fp16.h>
+
+#include "cached_attn_tc.cuh"
+
+namespace qia {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kInfoBytes = 32;
+constexpr int kSmemQScale = kSmemTail + kScalarRing * kInfoBytes;   // 2^e_i of 256 rows
+constexpr int kSmemML = kSmemQScale + 256 * 4;                      // m, l of 256 rows (joining)
+constexpr int kSmemBars = kSmemML + 2 * 256 * 4;
+constexpr int kSmemBytes = kSmemBars + 256 + 1024;
+// registers of a softmax thread and of any other: 256 x 208 + 128 x 88 = 384 x 168, what the block starts with
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+constexpr float kBias = 8.0f, kLag = 7.0f;
+constexpr uint32_t kIdescS = (1u << 4) | (uint32_t(128 >> 3) << 17) | (uint32_t(128 >> 4) << 24);   // f16 x f16 -> f32
+constexpr uint32_t kIdescO = kIdescS | (1u << 16);   // B (V) is MN-major
+
+// A tile of 128 keys: the softmax's numbers and which keys take part.
+struct __align__(16) TileInfo {
+  float c, f, inv_f;     // c log2e 2^e, f, 2^-f
+  uint32_t all;          // every key takes part
+  uint32_t valid[4];
+};
+static_assert(sizeof(TileInfo) == kInfoBytes, "bulk copy size");
+
+struct Widened {
+  __half* k;             // [B Hkv, tiles * 128, 128]: cached_cap cached tiles, then the fresh ones
+  __half* v;
+  TileInfo* info;        // [B Hkv, tiles]
+  int cached_cap, tiles;
+};
+
+__device__ __forceinline__ uint32_t cvt_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Four codes (a word of INT8) times a -> four f16: byte u = code + 128 under
+// 0x4B0000 is the float 2^23 + u.
+__device__ __forceinline__ uint2 widen4(uint32_t w, float a) {
+  const uint32_t u = w ^ 0x80808080u;
+  const uint64_t off = f2_pack(-8388736.0f, -8388736.0f), a2 = f2_pack(a, a);
+  float x[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t t = f2_pack(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + 2 * i)),
+                               __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7541 + 2 * i)));
+    f2_unpack(f2_mul(f2_add(t, off), a2), x[2 * i], x[2 * i + 1]);
+  }
+  return make_uint2(cvt_f16x2(x[0], x[1]), cvt_f16x2(x[2], x[3]));
+}
+
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
+
+// Maximum of |x| over the block as bits (NaN and infinity above every number); 256 threads.
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* slots) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+  __syncthreads();
+  uint32_t m = slots[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = max(m, slots[i]);
+  return m;
+}
+
+// Exponent e with max 2^-e in [2^13, 2^14) for a maximum given as bits; kept in
+// a range where c 2^(e + e_i) and 2^+-f stay normal (rows beyond it only lose
+// bits: below 2^-44 they no longer matter to a score, above they saturate f16
+// to infinity at 2^106).
+__device__ __forceinline__ int tile_exponent(uint32_t bits, int lo) {
+  return min(max(int(bits >> 23) - 127 - 13, lo), 90);
+}
+
+// One CTA per (tile, K/V head, request).
+__global__ void __launch_bounds__(256) cached_widen_kernel(const __grid_constant__ CachedAttn p,
+                                                           const __grid_constant__ Widened w) {
+  __shared__ float factor[2][128];
+  __shared__ uint32_t slots[2][8], valid_bits[4];
+  const int tile = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
+  grid_launch_dependents();
+  const bool cached = tile < w.cached_cap;
+  const int end = cached ? cached_len(p, b) : p.sk, k0 = (cached ? tile : tile - w.cached_cap) * 128;
+  if (k0 >= end) return;
+  const int group = b * p.kv_heads + kvh;
+  const int64_t head_row = int64_t(group) * p.capacity, out_row = (int64_t(group) * w.tiles + tile) * 128;
+  const uint8_t* mask = p.key_valid ? p.key_valid + b * p.mask_sb + (cached ? 0 : p.extent) : nullptr;
+  if (t < 128) {
+    const bool valid = k0 + t < end && (!mask || __ldg(mask + k0 + t) != 0);
+    const uint32_t bits = __ballot_sync(0xffffffffu, valid);
+    if ((t & 31) == 0) valid_bits[t >> 5] = bits;
+  }
+  int e[2];
+  if (cached) {
+    uint4 c[2][4];
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const int8_t* src = (z ? p.vc : p.kc) + head_row * kCaD;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = k0 + i * 32 + (t >> 3);
+        c[z][i] = key < end ? __ldg(reinterpret_cast<const uint4*>(src + int64_t(key) * kCaD) + (t & 7))
+                            : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+    // thread t: K's scale of key t, or V's of key t - 128
+    const int key = k0 + (t & 127);
+    const float s = key < end ? __ldg((t < 128 ? p.ks : p.vs) + head_row + key) : 0.0f;
+    __syncthreads();
+    const float mine = (valid_bits[(t & 127) >> 5] >> (t & 31)) & 1 ? s : 0.0f;
+    // (a NaN scale takes no part in the maximum)
+    const uint32_t mag = mine == mine ? __float_as_uint(fabsf(mine)) : 0u;
+    const uint32_t mk = block_max(t < 128 ? mag : 0u, slots[0]), mv = block_max(t < 128 ? 0u : mag, slots[1]);
+    e[0] = tile_exponent(mk + (7u << 23), -30);     // (|code| < 2^7)
+    e[1] = tile_exponent(mv + (7u << 23), -90);
+    factor[t >> 7][t & 127] = mine * pow2f(-e[t >> 7]);
+    __syncthreads();
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = i * 32 + (t >> 3);
+        const float a = factor[z][row];
+        const uint2 x = widen4(c[z][i].x, a), y = widen4(c[z][i].y, a), u = widen4(c[z][i].z, a), v = widen4(c[z][i].w, a);
+        st_global_v8((z ? w.v : w.k) + (out_row + row) * kCaD + 16 * (t & 7), make_uint4(x.x, x.y, y.x, y.y),
+                     make_uint4(u.x, u.y, v.x, v.y));
+      }
+    }
+  } else {
+    __syncthreads();
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const __nv_bfloat16* src = z ? p.v + b * p.v_sb + kvh * p.v_sh : p.k + b * p.k_sb + kvh * p.k_sh;
+      const int64_t ss = z ? p.v_ss : p.k_ss;
+      uint4 c[8];
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = i * 16 + (t >> 4);
+        c[i] = (valid_bits[row >> 5] >> (row & 31)) & 1
+                   ? __ldg(reinterpret_cast<const uint4*>(src + int64_t(k0 + row) * ss) + (t & 15))
+                   : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t x[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t lo = (x[q] << 16) & 0x7fffffffu, hi = x[q] & 0x7fff0000u;
+          m = max(m, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));   // finite values
+        }
+      }
+      e[z] = tile_exponent(block_max(m, slots[z]), z ? -90 : -30);
+      const float a = pow2f(-e[z]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = i * 16 + (t >> 4);
+        float f[8];
+        unpack8(c[i], f);
+        reinterpret_cast<uint4*>((z ? w.v : w.k) + (out_row + row) * kCaD)[t & 15] =
+            make_uint4(cvt_f16x2(f[0] * a, f[1] * a), cvt_f16x2(f[2] * a, f[3] * a), cvt_f16x2(f[4] * a, f[5] * a),
+                       cvt_f16x2(f[6] * a, f[7] * a));
+      }
+    }
+  }
+  if (t == 0) {
+    TileInfo info;
+    info.c = p.scale_log2 * pow2f(e[0]);
+    info.f = float(e[1]);
+    info.inv_f = pow2f(-e[1]);
+    info.all = (valid_bits[0] & valid_bits[1] & valid_bits[2] & valid_bits[3]) == 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) info.valid[i] = valid_bits[i];
+    w.info[int64_t(group) * w.tiles + tile] = info;
+  }
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_constant__ TileGrid tp,
+                        const __grid_constant__ Widened wd, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v, int* err) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSmemBars);
+  uint64_t* k_full = bars;            // [2] TMA -> issuer
+  uint64_t* v_full = bars + 2;        // [2]
+  uint64_t* k_empty = bars + 4;       // [2] issuer -> TMA
+  uint64_t* v_empty = bars + 6;       // [2]
+  uint64_t* info_full = bars + 8;     // [4] TMA -> softmax
+  uint64_t* s_full = bars + 12;       // [2] scores of query tile i
+  uint64_t* p_full = bars + 14;       // [2][2] weights of query tile i, half h, stored
+  uint64_t* o_full = bars + 18;
+  uint64_t* drain = bars + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int splits = int(cluster_size()), split = int(cluster_rank());
+  const int group = tp.first_group + int(blockIdx.x) / splits;
+  const int pair = group % tp.pairs, kvh = group / tp.pairs % p.kv_heads, b = group / tp.pairs / p.kv_heads;
+  const int n_tiles = min(2, tp.q_tiles - 2 * pair);   // query tiles of this CTA
+  const int len = cached_len(p, b);
+  const int cached_tiles = (len + 127) / 128;
+  const int all_tiles = cached_tiles + (p.sk + 127) / 128;
+  const int per = (all_tiles + splits - 1) / splits;
+  const int first = min(all_tiles, split * per), n = min(all_tiles, first + per) - first;   // this CTA's key tiles
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 12; ++i) mbar_init(smem_u32(&bars[i]), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1);
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&p_full[i]), 4);
+    mbar_init(smem_u32(o_full), 1);
+    mbar_init(smem_u32(drain), 1);
+    fence_barrier_init();
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
+  if (warp == 8) tmem_alloc(smem_u32(tmem_slot), 512);
+  // ---- query rows as f16, scaled by a power of two each (sixteen threads per
+  // row; rows past the end are zeros)
+  const int tile_rows = tp.tokens_per_tile * p.share;
+  for (int i = threadIdx.x; i < n_tiles * kTileRows * 16; i += kThreads) {
+    const int tile = i >> 11, row = (i >> 4) & 127, piece = i & 15;
+    const int token = (2 * pair + tile) * tp.tokens_per_tile + row / p.share;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (row < tile_rows && token < p.sq)
+      v = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_sb + int64_t(token) * p.q_ss +
+                                               int64_t(kvh * p.share + row % p.share) * p.q_sh) + piece);
+    float f[8];
+    unpack8(v, f);
+    uint32_t mx = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(f[e]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const int e = min(max(int(mx >> 23) - 127, -80), 120);
+    const float inv = pow2f(-e);
+    if (piece == 0) reinterpret_cast<float*>(smem + kSmemQScale)[tile * kTileRows + row] = pow2f(e);
+    st_shared_v4(sbase + kSmemQ + tile * kTileBytes + tile_offset(row, piece), cvt_f16x2(f[0] * inv, f[1] * inv),
+                 cvt_f16x2(f[2] * inv, f[3] * inv), cvt_f16x2(f[4] * inv, f[5] * inv), cvt_f16x2(f[6] * inv, f[7] * inv));
+  }
+  fence_proxy_async_shared();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 8) {
+      // ------------------------------------------------------------ MMA issuer
+      if (lane == 0 && n > 0) {
+        const auto qk = [&](int i, int j) {
+          const uint64_t qd = smem_desc_k_sw128(sbase + kSmemQ + i * kTileBytes);
+          const uint64_t kd = smem_desc_k_sw128(sbase + kSmemKV + (j & 1) * 2 * kTileBytes);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint64_t off = uint64_t(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
+            tc_mma_f16_ss(tmem + uint32_t(128 * i), qd + off, kd + off, kIdescS, kk > 0);
+          }
+          tc_commit(smem_u32(&s_full[i]));
+        };
+        const auto wait_k = [&](int j) { return mbar_wait(smem_u32(&k_full[j & 1]), (j >> 1) & 1, err); };
+        // P.V of query tile i and key tile j, in halves of 64 keys as they are stored
+        const auto pv = [&](int i, int j) {
+          const uint64_t vd = smem_desc_mn_sw128(sbase + kSmemKV + ((j & 1) * 2 + 1) * kTileBytes, kPanel);
+          for (int h = 0; h < 2; ++h) {
+            if (!mbar_wait(smem_u32(&p_full[2 * i + h]), j & 1, err)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {   // 16 keys: two 8-key groups of 1 KB
+              const int kk = 4 * h + k;
+              tc_mma_f16_ts(tmem + uint32_t(256 + 128 * i), tmem + uint32_t(128 * i + 8 * kk), vd + uint64_t(128 * kk),
+                            kIdescO, (j | kk) != 0);
+            }
+          }
+          return true;
+        };
+        bool ok = wait_k(0);
+        tc_fence_after();
+        if (ok) {
+          for (int i = 0; i < n_tiles; ++i) qk(i, 0);
+          tc_commit(smem_u32(&k_empty[0]));
+        }
+        for (int j = 0; j < n && ok; ++j) {
+          ok = mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, err);
+          for (int i = 0; i < n_tiles && ok; ++i) {
+            ok = pv(i, j);
+            if (ok && j + 1 < n) {
+              ok = i > 0 || wait_k(j + 1);
+              if (!ok) break;
+              tc_fence_after();
+              qk(i, j + 1);
+            }
+          }
+          if (!ok) break;
+          tc_commit(smem_u32(&v_empty[j & 1]));
+          if (j + 1 < n) tc_commit(smem_u32(&k_empty[(j + 1) & 1]));
+        }
+        if (ok) tc_commit(smem_u32(o_full));
+        tc_commit(smem_u32(drain));
+        mbar_wait(smem_u32(drain), 0, ok ? err : nullptr, 100000000ull);
+      }
+    } else if (warp == 9 && lane == 0 && n > 0) {
+      // ---------------------------------------------------------- TMA producer
+      const int64_t bh = int64_t(b) * p.kv_heads + kvh;
+      bool ok = true;
+      grid_wait();                           // the keys are widened
+      int issued = 0;
+      for (int u = 0; u < 2 * n && ok; ++u) {
+        const int j = u >> 1, st = j & 1;
+        const int tile = first + j < cached_tiles ? first + j : wd.cached_cap + first + j - cached_tiles;
+        if (!(u & 1)) {                      // (ring slot j % 4: tile j - 4 was done before V of j - 3 left)
+          const uint32_t bar = smem_u32(&info_full[j % kScalarRing]);
+          mbar_arrive_expect_tx(bar, kInfoBytes);
+          bulk_load(sbase + kSmemTail + uint32_t(j % kScalarRing) * kInfoBytes, wd.info + bh * wd.tiles + tile,
+                    kInfoBytes, bar);
+        }
+        ok = mbar_wait(smem_u32((u & 1) ? &v_empty[st] : &k_empty[st]), ((j >> 1) & 1) ^ 1, err);
+        if (!ok) break;
+        const uint32_t bar = smem_u32((u & 1) ? &v_full[st] : &k_full[st]);
+        const uint32_t slot = sbase + kSmemKV + uint32_t(st * 2 + (u & 1)) * kTileBytes;
+        mbar_arrive_expect_tx(bar, kTileBytes);
+        for (int h = 0; h < 2; ++h)
+          tma_load_2d(slot + uint32_t(h * kPanel), (u & 1) ? &tm_v : &tm_k, bar, h * 64, int((bh * wd.tiles + tile) * 128));
+        issued = u + 1;
+      }
+      if (!ok) {   // let queued copies land before the shared memory is released
+        for (int u = max(0, issued - 4); u < issued; ++u)
+          mbar_wait(smem_u32((u & 1) ? &v_full[(u >> 1) & 1] : &k_full[(u >> 1) & 1]), (u >> 2) & 1, nullptr,
+                    100000000ull);
+        for (int j = max(0, (issued + 1) / 2 - kScalarRing); j <= issued / 2; ++j)
+          mbar_wait(smem_u32(&info_full[j % kScalarRing]), (j / kScalarRing) & 1, nullptr, 100000000ull);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ----------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int w = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + t_lane + uint32_t(128 * w), t_o = tmem + t_lane + uint32_t(256 + 128 * w);
+    const float q_up = reinterpret_cast<const float*>(smem + kSmemQScale)[w < n_tiles ? w * kTileRows + row : 0];
+    bool ok = w < n_tiles;
+    float m = -INFINITY, l = 0.0f;
+    for (int j = 0; j < n && ok; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[w]), j & 1, err) &&
+                                       mbar_wait(smem_u32(&info_full[j % kScalarRing]), (j / kScalarRing) & 1, err));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[128];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        tc_ld_32x32b_x32(t_s + uint32_t(q * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[q * 32]));
+      const TileInfo* info = reinterpret_cast<const TileInfo*>(smem + kSmemTail + (j % kScalarRing) * kInfoBytes);
+      const float4 num = *reinterpret_cast<const float4*>(info);
+      const float c = num.x * q_up, f = num.y;
+      tc_wait_ld();
+      if (!__float_as_uint(num.w)) {         // some keys take no part
+        const uint4 bits = *reinterpret_cast<const uint4*>(info->valid);
+        const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+        for (int i = 0; i < 128; ++i)
+          if (!((word[i >> 5] >> (i & 31)) & 1)) s[i] = 0xff800000u;
+      }
+      float mx[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s[i]);
+#pragma unroll
+      for (int i = 4; i < 124; i += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) mx[k] = max3(mx[k], __uint_as_float(s[124 + 2 * k]), __uint_as_float(s[125 + 2 * k]));
+      const float top = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), c, f);
+      const bool grow = top > m + kLag;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float r = grow ? ex2_ftz(m - top) : 1.0f;   // (m = -inf: 0)
+        if (grow) m = top;
+        l *= r;
+        if (j > 0) {
+#pragma unroll 1
+          for (int q = 0; q < 8; ++q) {
+            uint32_t o[16];
+            tc_ld_32x32b_x16(t_o + uint32_t(q * 16), o);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * r);
+            tc_st_32x32b_x16(t_o + uint32_t(q * 16), o);
+          }
+        }
+      }
+      const float n1 = f + kBias - (m == -INFINITY ? 0.0f : m);
+      const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(n1, n1);
+      uint64_t sum[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t x[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float a, b2;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[64 * h + 2 * i]), __uint_as_float(s[64 * h + 2 * i + 1])), c2, n2), a, b2);
+          a = ex2_ftz(a);
+          b2 = ex2_ftz(b2);
+          sum[i & 1] = f2_add(sum[i & 1], f2_pack(a, b2));
+          x[i] = cvt_f16x2(a, b2);
+        }
+        tc_st_32x32b_x32(t_s + uint32_t(32 * h), x);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&p_full[2 * w + h]));
+      }
+      float a, b2;
+      f2_unpack(f2_add(sum[0], sum[1]), a, b2);
+      l = fmaf(a + b2, num.z, l);
+    }
+    const bool have = ok && n > 0 && __all_sync(0xffffffffu, mbar_wait(smem_u32(o_full), 0, err));
+    tc_fence_after();
+    if (w < n_tiles) {
+      const int token = (2 * pair + w) * tp.tokens_per_tile + row / p.share;
+      if (splits == 1)
+        store_row(t_o, have, l, row < tile_rows && token < p.sq,
+                  p.out + b * p.o_sb + int64_t(token) * p.o_ss + int64_t(kvh * p.share + row % p.share) * p.o_sh);
+      else
+        stage_row(t_o, have, m, l, sbase, reinterpret_cast<float*>(smem + kSmemML), w * kTileRows + row);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (splits > 1) join_rows(p, tp, sbase, sbase + kSmemML, splits, split, 1, n_tiles, pair, kvh, b);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 wide_encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* q = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) == cudaSuccess &&
+        r == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(q);
+  });
+  return fn;
+}
+
+// f16 [rows, 128], boxes of 128 rows x 64 channels
+int make_rows_map(CUtensorMap* map, const void* base, int64_t rows) {
+  auto fn = wide_encode_fn();
+  if (!fn) return set_error(QIA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {cuuint64_t(kCaD), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(kCaD * 2)};
+  cuuint32_t box[2] = {64u, 128u};
+  cuuint32_t estr[2] = {1u, 1u};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(QIA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+  return QIA_OK;
+}
+
+}  // namespace
+
+// Two query tiles or fewer per request and K/V head convert the codes as they go
+// (cached_attn_tiles.cu); from three on, converting once is less work.
+bool cached_use_wide(int64_t seq_q, int64_t share) {
+  const int64_t per = kTileRows / share;
+  return (seq_q + per - 1) / per > 2;
+}
+
+int64_t cached_wide_workspace(int64_t batch, int64_t seq_k, int64_t kv_heads, int64_t extent) {
+  return batch * kv_heads * ((extent + 127) / 128 + (seq_k + 127) / 128) * (2 * kTileBytes + kInfoBytes);
+}
+
+int launch_cached_wide(const CachedAttn& p, int batch, void* workspace, cudaStream_t st) {
+  const char* who = "qia_cached_attention";
+  static const bool ready = cudaFuncSetAttribute(cached_attn_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 kSmemBytes) == cudaSuccess;
+  if (!ready) return set_error(QIA_ERR_CUDA, "%s: cudaFuncSetAttribute failed", who);
+  TileGrid g = tile_grid(p);
+  const int64_t groups = int64_t(g.pairs) * p.kv_heads * batch, heads = int64_t(batch) * p.kv_heads;
+  Widened wd;
+  wd.cached_cap = (p.extent + 127) / 128;
+  wd.tiles = wd.cached_cap + (p.sk + 127) / 128;
+  const int64_t rows = heads * wd.tiles * 128;
+  if (groups > 0x0fffffff || rows > 0x7fffffff)
+    return set_error(QIA_ERR_UNSUPPORTED, "%s: too many rows for one call", who);
+  CUtensorMap tm_k = {}, tm_v = {};
+  if (wd.tiles) {
+    if (!workspace || !aligned(workspace, 128))
+      return set_error(QIA_ERR_INVALID, "%s: the workspace is null or misaligned", who);
+    wd.k = (__half*)workspace;
+    wd.v = wd.k + rows * kCaD;
+    wd.info = (TileInfo*)(wd.v + rows * kCaD);
+    int rc = make_rows_map(&tm_k, wd.k, rows);
+    if (!rc) rc = make_rows_map(&tm_v, wd.v, rows);
+    if (rc) return rc;
+    cached_widen_kernel<<<dim3(unsigned(wd.tiles), unsigned(p.kv_heads), unsigned(batch)), 256, 0, st>>>(p, wd);
+    rc = check_launch("cached_widen_kernel");
+    if (rc) return rc;
+  }
+  static int resident[9] = {0};
+  return launch_waves(
+      groups, wd.tiles,
+      [&](int s) { return resident_clusters(cached_attn_wide_kernel, kThreads, kSmemBytes, s, resident); },
+      [&](int64_t first, int64_t count, int splits, bool follows) {
+        g.first_group = int(first);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(count * splits));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = kSmemBytes;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = unsigned(splits);
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        // the first launch follows the widening: its prologue overlaps it
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = follows && wd.tiles ? 2 : 1;
+        const cudaError_t e =
+            cudaLaunchKernelEx(&cfg, cached_attn_wide_kernel, p, g, wd, tm_k, tm_v, device_error_word());
+        if (e != cudaSuccess) {
+          cudaGetLastError();
+          return set_error(QIA_ERR_CUDA, "cached_attn_wide_kernel: %s", cudaGetErrorString(e));
+        }
+        return int(QIA_OK);
+      });
+}
+
+}  // namespace qia

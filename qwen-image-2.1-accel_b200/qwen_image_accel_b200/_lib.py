@@ -94,7 +94,7 @@ SIGNATURES.update({
 RAW_SIGNATURES: dict[str, tuple] = {
     "qia_sage_workspace_bytes": (ctypes.c_int64, [_I, _I, _I, _I]),
     "qia_ipc_handle_bytes": (ctypes.c_int64, []),
-    "qia_cached_attention_workspace_bytes": (ctypes.c_int64, [_I, _I, _I, _I, _I, _I, ctypes.c_int]),
+    "qia_cached_attention_workspace_bytes": (ctypes.c_int64, [_I, _I, _I, _I, _I, _I]),
     "qia_lora_workspace_bytes": (ctypes.c_int64, [_I, _I, _I]),
     "qia_sage_attn_ctas": (ctypes.c_int64, [_I, _I, _I]),
 }

@@ -196,7 +196,7 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
     if not out.numel():
         return out
     size = _lib.load().qia_cached_attention_workspace_bytes(cache.batch, q.shape[1], fresh, q.shape[2], cache.kv_heads,
-                                                            cache.extent, key_valid is not None)
+                                                            cache.extent)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     kc, vc, ks, vs, lengths = cache._buffers
     rows = (*k.stride()[:3], *v.stride()[:3]) if fresh else (0,) * 6
