@@ -190,82 +190,91 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
       // ------------------------------------------------------------ MMA issuer
-      if (lane == 0 && n > 0) {
-        bool ok = true;
+      // (warp-uniform control, one elected lane: see cached_attn_wide.cu)
+      if (n > 0) {
+        const bool lead = elect_one();
+        const auto wait = [&](uint64_t* bar, int parity) {
+          const bool got = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), uint32_t(parity), err));
+          tc_fence_after();
+          return got;
+        };
+        const auto commit = [&](uint64_t* bar) {
+          if (lead) tc_commit(smem_u32(bar));
+        };
         const auto qk = [&](int w, int j) {
           const uint64_t qd = smem_desc_k_sw128(sbase + kSmemQ + (duo ? 0 : w) * kTileBytes);
           const uint64_t kd = smem_desc_k_sw128(sbase + kSmemKV + (j & 1) * 2 * kTileBytes);
+          if (lead) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const uint64_t off = uint64_t(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
-            tc_mma_f16_ss(tmem + uint32_t(128 * w), qd + off, kd + off, kIdescS, kk > 0);
+            for (int kk = 0; kk < 8; ++kk) {
+              const uint64_t off = uint64_t(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
+              tc_mma_f16_ss(tmem + uint32_t(128 * w), qd + off, kd + off, kIdescS, kk > 0);
+            }
+            tc_commit(smem_u32(&s_full[w]));
           }
-          tc_commit(smem_u32(&s_full[w]));
         };
-        const auto wait_k = [&](int j) { return mbar_wait(smem_u32(&k_full[j & 1]), (j >> 1) & 1, err); };
+        const auto wait_k = [&](int j) { return wait(&k_full[j & 1], (j >> 1) & 1); };
         // P.V of group w's it-th key tile j, in halves of 64 keys as they are stored
         const auto pv = [&](int w, int it, int j) {
           const uint64_t vd = smem_desc_mn_sw128(sbase + kSmemKV + ((j & 1) * 2 + 1) * kTileBytes, kPanel);
-          for (int h = 0; h < 2; ++h) {
-            if (!mbar_wait(smem_u32(&p_full[2 * w + h]), it & 1, err)) return false;
-            tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {   // 16 keys: two 8-key groups of 1 KB
-              const int kk = 4 * h + k;
-              tc_mma_f16_ts(tmem + uint32_t(256 + 128 * w), tmem + uint32_t(128 * w + 8 * kk), vd + uint64_t(128 * kk),
-                            kIdescO, (it | kk) != 0);
+          for (int h = 0; h < 2; ++h) {
+            if (!wait(&p_full[2 * w + h], it & 1)) return false;
+            if (lead) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {   // 16 keys: two 8-key groups of 1 KB
+                const int kk = 4 * h + k;
+                tc_mma_f16_ts(tmem + uint32_t(256 + 128 * w), tmem + uint32_t(128 * w + 8 * kk),
+                              vd + uint64_t(128 * kk), kIdescO, kk > 0 || it > 0);
+              }
             }
           }
           return true;
         };
+        bool ok = true;
         if (duo) {
           for (int j = 0; j < 2 && j < n && ok; ++j) {
             ok = wait_k(j);
-            tc_fence_after();
             if (ok) qk(j, j);
-            if (ok) tc_commit(smem_u32(&k_empty[j]));
+            if (ok) commit(&k_empty[j]);
           }
           for (int j = 0; j < n && ok; ++j) {
-            ok = mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, err) && pv(j & 1, j >> 1, j);
+            ok = wait(&v_full[j & 1], (j >> 1) & 1) && pv(j & 1, j >> 1, j);
             if (!ok) break;
-            tc_commit(smem_u32(&v_empty[j & 1]));
+            commit(&v_empty[j & 1]);
             if (j + 2 < n) {
               ok = wait_k(j + 2);
               if (!ok) break;
-              tc_fence_after();
               qk(j & 1, j + 2);
-              tc_commit(smem_u32(&k_empty[j & 1]));
+              commit(&k_empty[j & 1]);
             }
           }
         } else {
           ok = wait_k(0);
-          tc_fence_after();
           if (ok) {
             qk(0, 0);
             qk(1, 0);
-            tc_commit(smem_u32(&k_empty[0]));
+            commit(&k_empty[0]);
           }
           for (int j = 0; j < n && ok; ++j) {
-            ok = mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, err);
-            for (int w = 0; w < 2 && ok; ++w) {
-              ok = pv(w, j, j);
+            ok = wait(&v_full[j & 1], (j >> 1) & 1);
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              ok = ok && pv(w, j, j);
               if (ok && j + 1 < n) {
                 ok = w > 0 || wait_k(j + 1);
-                if (!ok) break;
-                tc_fence_after();
-                qk(w, j + 1);
+                if (ok) qk(w, j + 1);
               }
             }
             if (!ok) break;
-            tc_commit(smem_u32(&v_empty[j & 1]));
-            if (j + 1 < n) tc_commit(smem_u32(&k_empty[(j + 1) & 1]));
+            commit(&v_empty[j & 1]);
+            if (j + 1 < n) commit(&k_empty[(j + 1) & 1]);
           }
         }
-        if (ok) tc_commit(smem_u32(o_full));
-        tc_commit(smem_u32(drain));
+        if (ok) commit(o_full);
+        commit(drain);
         mbar_wait(smem_u32(drain), 0, ok ? err : nullptr, 100000000ull);
       }
-      __syncwarp();
     } else {
       // ------------------------------------------------------- operand writers
       const int t = threadIdx.x - 32 * 9;

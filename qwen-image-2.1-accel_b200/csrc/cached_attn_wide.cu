@@ -284,56 +284,69 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
       // ------------------------------------------------------------ MMA issuer
-      if (lane == 0 && n > 0) {
+      // The whole warp runs the schedule and one elected lane issues: with warp-
+      // uniform control the descriptors stay in uniform registers (issued from a
+      // one-lane branch, a product of 128 x 128 x 128 took 611 cycles, not 512).
+      if (n > 0) {
+        const bool lead = elect_one();
+        const auto wait = [&](uint64_t* bar, int parity) {
+          const bool got = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), uint32_t(parity), err));
+          tc_fence_after();
+          return got;
+        };
         const auto qk = [&](int i, int j) {
           const uint64_t qd = smem_desc_k_sw128(sbase + kSmemQ + i * kTileBytes);
           const uint64_t kd = smem_desc_k_sw128(sbase + kSmemKV + (j & 1) * 2 * kTileBytes);
+          if (lead) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const uint64_t off = uint64_t(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
-            tc_mma_f16_ss(tmem + uint32_t(128 * i), qd + off, kd + off, kIdescS, kk > 0);
+            for (int kk = 0; kk < 8; ++kk) {
+              const uint64_t off = uint64_t(((kk >> 2) * kPanel + (kk & 3) * 32) >> 4);
+              tc_mma_f16_ss(tmem + uint32_t(128 * i), qd + off, kd + off, kIdescS, kk > 0);
+            }
+            tc_commit(smem_u32(&s_full[i]));
           }
-          tc_commit(smem_u32(&s_full[i]));
         };
-        const auto wait_k = [&](int j) { return mbar_wait(smem_u32(&k_full[j & 1]), (j >> 1) & 1, err); };
-        // P.V of query tile i and key tile j, in halves of 64 keys as they are stored
-        const auto pv = [&](int i, int j) {
+        // half h (64 keys) of P.V of query tile i and key tile j
+        const auto pv = [&](int i, int j, int h) {
           const uint64_t vd = smem_desc_mn_sw128(sbase + kSmemKV + ((j & 1) * 2 + 1) * kTileBytes, kPanel);
-          for (int h = 0; h < 2; ++h) {
-            if (!mbar_wait(smem_u32(&p_full[2 * i + h]), j & 1, err)) return false;
-            tc_fence_after();
+          if (lead) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {   // 16 keys: two 8-key groups of 1 KB
               const int kk = 4 * h + k;
               tc_mma_f16_ts(tmem + uint32_t(256 + 128 * i), tmem + uint32_t(128 * i + 8 * kk), vd + uint64_t(128 * kk),
-                            kIdescO, (j | kk) != 0);
+                            kIdescO, kk > 0 || j > 0);
             }
           }
-          return true;
         };
-        bool ok = wait_k(0);
-        tc_fence_after();
+        const auto commit = [&](uint64_t* bar) {
+          if (lead) tc_commit(smem_u32(bar));
+        };
+        bool ok = wait(&k_full[0], 0);
         if (ok) {
           for (int i = 0; i < n_tiles; ++i) qk(i, 0);
-          tc_commit(smem_u32(&k_empty[0]));
+          commit(&k_empty[0]);
         }
         for (int j = 0; j < n && ok; ++j) {
-          ok = mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, err);
-          for (int i = 0; i < n_tiles && ok; ++i) {
-            ok = pv(i, j);
-            if (ok && j + 1 < n) {
-              ok = i > 0 || wait_k(j + 1);
-              if (!ok) break;
-              tc_fence_after();
-              qk(i, j + 1);
+          ok = wait(&v_full[j & 1], (j >> 1) & 1);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (i < n_tiles && ok) {
+              ok = wait(&p_full[2 * i], j & 1);
+              if (ok) pv(i, j, 0);
+              ok = ok && wait(&p_full[2 * i + 1], j & 1);
+              if (ok) pv(i, j, 1);
+              if (ok && j + 1 < n) {
+                ok = i > 0 || wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
+                if (ok) qk(i, j + 1);
+              }
             }
           }
           if (!ok) break;
-          tc_commit(smem_u32(&v_empty[j & 1]));
-          if (j + 1 < n) tc_commit(smem_u32(&k_empty[(j + 1) & 1]));
+          commit(&v_empty[j & 1]);
+          if (j + 1 < n) commit(&k_empty[(j + 1) & 1]);
         }
-        if (ok) tc_commit(smem_u32(o_full));
-        tc_commit(smem_u32(drain));
+        if (ok) commit(o_full);
+        commit(drain);
         mbar_wait(smem_u32(drain), 0, ok ? err : nullptr, 100000000ull);
       }
     } else if (warp == 9 && lane == 0 && n > 0) {
@@ -404,9 +417,11 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
 #pragma unroll
       for (int i = 4; i < 124; i += 8)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
+        for (int k = 0; k < 4; ++k)
+          mx[k] = max3(mx[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
 #pragma unroll
-      for (int k = 0; k < 2; ++k) mx[k] = max3(mx[k], __uint_as_float(s[124 + 2 * k]), __uint_as_float(s[125 + 2 * k]));
+      for (int k = 0; k < 2; ++k)
+        mx[k] = max3(mx[k], __uint_as_float(s[124 + 2 * k]), __uint_as_float(s[125 + 2 * k]));
       const float top = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), c, f);
       const bool grow = top > m + kLag;
       if (__any_sync(0xffffffffu, grow)) {
