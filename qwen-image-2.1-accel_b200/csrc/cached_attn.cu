@@ -1,23 +1,27 @@
 // Attention of few query rows over the INT8 prefix cache, and the entry point
 // of the cached attention.
 //
-// cached_attn_rows_kernel: a tile of 16 query rows (token-major over the heads
-// that share a K/V head) against a slice of the keys. What bounds it is the
-// cache's bytes (one per element), so everything is arranged around streaming
-// them once: every warp keeps a ring of kRowsRing 16-key steps (4 KB of codes
-// each) in flight with cp.async into shared memory of its own -- no barrier
-// between warps -- and reads 16-byte pieces back with no bank conflicts (piece
-// p of row r is stored at p ^ (r & 7)). Each thread takes contiguous bytes and
-// the contraction is permuted instead:
-//   * q.k: thread c = lane % 4 holds channels [32c, 32c + 32) of key lane / 4,
-//     and step j of the eight m16n8k16 products takes channels 32c + 4j .. + 3
-//     of every c (the query fragments are loaded in the same order);
-//   * p.v: thread g = lane / 4 holds channels [16g, 16g + 16) of four keys, and
-//     product t of sixteen takes channel 16g + t of every g.
-// INT8 -> f16 is two byte permutes and one subtraction per four codes: byte
-// u = code + 128 under exponent byte 0x64 is the f16 1024 + u.
+// cached_attn_rows_kernel: a tile of up to 8 or 16 query rows (token-major over
+// the heads that share a K/V head) against a slice of the keys. What bounds it is
+// the cache's bytes (one per element) and, next, the instructions that widen
+// them, so the keys are the rows of the matrix products (m16n8k16 with the
+// queries as its eight columns) and are streamed once: every warp keeps the next
+// K or V half of a 32-key step in flight with cp.async into shared memory of its
+// own -- no barrier between warps -- and the contraction is permuted so that each
+// thread reads contiguous bytes:
+//   * row (mt, g, half) of the two score tiles of a step, g = lane / 4, is key
+//     4 g + 2 mt + half, so a thread owns the scores of four adjacent keys;
+//   * k.q: thread (g, c = lane % 4) holds channels [32 c, +32) of its keys, and
+//     product j of eight takes channels 32 c + 4 j .. + 3 of every c (the query
+//     fragments are loaded in the same order);
+//   * v.p: the weights are transposed in registers (movmatrix), which leaves
+//     thread c the keys 8 c .. 8 c + 7; thread (g, c) holds channels [16 g, +16)
+//     of them, and product t of eight takes channels 16 g + 2 t, + 1 of every g.
+// Piece p (16 bytes) of row r is stored at p ^ swizzle(r): no bank conflicts in
+// either read. INT8 -> f16 is two byte permutes and one subtraction per four
+// codes: byte u = code + 128 under exponent byte 0x64 is the f16 1024 + u.
 //
-// Warps take 16-key steps of the CTA's slice in turn, each with a running
+// Warps take 32-key steps of the CTA's slice in turn, each with a running
 // maximum and sum of its own; the CTA joins its warps in shared memory and the
 // CTAs of a cluster (which split the keys) join through distributed shared
 // memory, in rank order: one launch, no workspace, results that do not depend
@@ -31,23 +35,24 @@ namespace qia {
 namespace {
 
 constexpr int kRowsWarps = 4;
-constexpr int kRowsTile = 16;          // query rows per CTA
-constexpr int kRowsStep = 16;          // keys per warp step
-constexpr int kRowsRing = 4;           // steps in flight per warp
-constexpr int kRowsCodes = 2 * kRowsStep * kCaD;            // K, then V codes of a step
-constexpr int kRowsStage = kRowsCodes + 2 * kRowsStep * 4;  // and their scales
+constexpr int kRowsStep = 32;          // keys per warp step
+constexpr int kRowsHalf = kRowsStep * (kCaD + 4);   // K (or V) codes of a step and their scales
 // f16 weights: w = 2^(t - M + 8) <= 2^15 while t <= M + 7, so the accumulators
 // are rescaled only when a score passes its maximum by more than 7.
 constexpr float kRowsBias = 8.0f, kRowsLag = 7.0f;
 
-// The rings are done when the joining begins.
+// The staged steps are done when the joining begins.
+template <int ROWS, int DEPTH>
 union RowsSmem {
-  uint8_t ring[kRowsWarps][kRowsRing][kRowsStage];
   struct {
-  float o[kRowsWarps][kRowsTile][kCaD + 4];
-  float m[kRowsWarps][kRowsTile], l[kRowsWarps][kRowsTile];
-  float om[kRowsTile][kCaD + 4];        // the CTA's joined rows, read by the cluster
-  float mm[kRowsTile], lm[kRowsTile];
+    uint8_t half[kRowsWarps][2][DEPTH][kRowsHalf];
+    float key[kRowsWarps][3][kRowsStep];   // the softmax's numbers of a step's keys
+  };
+  struct {
+    float o[kRowsWarps][ROWS][kCaD + 4];
+    float m[kRowsWarps][ROWS], l[kRowsWarps][ROWS];
+    float om[ROWS][kCaD + 4];              // the CTA's joined rows, read by the cluster
+    float mm[ROWS], lm[ROWS];
   };
 };
 
@@ -108,14 +113,28 @@ __device__ __forceinline__ uint32_t absmax8(const uint4& v, uint32_t m) {
   return m;
 }
 
-__global__ void __launch_bounds__(kRowsWarps * 32, 3) cached_attn_rows_kernel(const __grid_constant__ CachedAttn p) {
+__device__ __forceinline__ int rows_swizzle(int row) { return ((row >> 2) & 1) ^ (((row >> 3) & 3) << 1); }
+
+// Transposes an 8 x 8 matrix of f16 held one row per four lanes.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+// NT: column tiles of eight query rows; DEPTH: steps that a warp holds, the next
+// DEPTH - 1 whole and the halves of one more in flight.
+template <int NT, int DEPTH>
+__global__ void __launch_bounds__(kRowsWarps * 32, NT == 1 && DEPTH == 1 ? 4 : 3)
+cached_attn_rows_kernel(const __grid_constant__ CachedAttn p) {
+  constexpr int ROWS = 8 * NT;
   extern __shared__ __align__(16) uint8_t rows_smem[];
-  RowsSmem& sm = *reinterpret_cast<RowsSmem*>(rows_smem);
+  RowsSmem<ROWS, DEPTH>& sm = *reinterpret_cast<RowsSmem<ROWS, DEPTH>*>(rows_smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int splits = int(cluster_size()), split = int(cluster_rank());
-  const int tile = blockIdx.x / splits, kvh = blockIdx.y, b = blockIdx.z;
-  const int rows = p.sq * p.share;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int rows = p.sq * p.share;                     // (one tile: at most ROWS)
   const int len = cached_len(p, b);
   const int cached_steps = (len + kRowsStep - 1) / kRowsStep;
   const int steps = cached_steps + (p.sk + kRowsStep - 1) / kRowsStep;
@@ -123,46 +142,46 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 3) cached_attn_rows_kernel(co
   const int step_end = min(steps, (split + 1) * per);
 
   const int64_t head_row = (int64_t(b) * p.kv_heads + kvh) * p.capacity;
-  const int8_t* kc = p.kc + head_row * kCaD;
-  const int8_t* vc = p.vc + head_row * kCaD;
   const uint8_t* mask = p.key_valid ? p.key_valid + b * p.mask_sb : nullptr;
-  // key of this thread's V row i (of four), and of its score columns
-  const auto vkey = [&](int i) { return 2 * c + (i & 1) + (i >> 1) * 8; };
 
-  // ---- the warp's ring of cached steps: step0, step0 + kRowsWarps, ...
+  // ---- the warp's cached steps: step0, step0 + kRowsWarps, ...; z: 0 K, 1 V
   const int cached_end = min(step_end, cached_steps);
   const int step0 = split * per + warp;
   const int mine_n = step0 < cached_end ? (cached_end - step0 + kRowsWarps - 1) / kRowsWarps : 0;
-  const auto issue = [&](int i) {
+  const auto issue = [&](int i, int z) {
     if (i < mine_n) {
-      uint8_t* st = sm.ring[warp][i % kRowsRing];
+      uint8_t* st = sm.half[warp][z][i % DEPTH];
       const int k0 = (step0 + i * kRowsWarps) * kRowsStep;
+      const int8_t* codes = (z ? p.vc : p.kc) + head_row * kCaD;
       // (keys past the length: any held row, weight 0)
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const int row = r4 * 4 + (lane >> 3), piece = lane & 7, at = row * kCaD + ((piece ^ (row & 7)) << 4);
-        const int64_t src = int64_t(min(k0 + row, len - 1)) * kCaD + piece * 16;
-        cp_async16(st + at, kc + src);
-        cp_async16(st + kRowsCodes / 2 + at, vc + src);
+      for (int r8 = 0; r8 < 8; ++r8) {
+        const int row = r8 * 4 + (lane >> 3), piece = lane & 7;
+        cp_async16(st + row * kCaD + ((piece ^ rows_swizzle(row)) << 4),
+                   codes + int64_t(min(k0 + row, len - 1)) * kCaD + piece * 16);
       }
-      cp_async4(st + kRowsCodes + lane * 4, (lane < 16 ? p.ks : p.vs) + head_row + min(k0 + (lane & 15), len - 1));
+      cp_async4(st + kRowsStep * kCaD + lane * 4, (z ? p.vs : p.ks) + head_row + min(k0 + lane, len - 1));
     }
     cp_async_commit();      // (an empty group keeps the count)
   };
-  const auto mask_of = [&](int i) {   // of key lane % 16 of step i
-    const int key = (step0 + i * kRowsWarps) * kRowsStep + (lane & 15);
+  const auto mask_of = [&](int i) {   // of key `lane` of step i
+    const int key = (step0 + i * kRowsWarps) * kRowsStep + lane;
     return i < mine_n && key < len && (!mask || __ldg(mask + key) != 0);
   };
 #pragma unroll
-  for (int i = 0; i < kRowsRing - 1; ++i) issue(i);
+  for (int i = 0; i < DEPTH; ++i) {
+    issue(i, 0);
+    issue(i, 1);
+  }
   bool valid = mask_of(0);
 
-  // ---- query fragments, normalised per row by a power of two (f16 operands)
-  uint32_t qa[8][4];
-  float qup[2];
+  // ---- query fragments, normalised per row by a power of two (f16 operands):
+  // thread (g, c) holds channels [32 c, +32) of row 8 nt + g
+  uint32_t qb[NT][8][2];
+  float qup[NT][2];                    // of the rows whose scores it owns, 8 nt + 2 c + e
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = tile * kRowsTile + g + 8 * r;
+  for (int nt = 0; nt < NT; ++nt) {
+    const int row = 8 * nt + g;
     uint4 x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -177,122 +196,162 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 3) cached_attn_rows_kernel(co
     for (int i = 0; i < 4; ++i) m = absmax8(x[i], m);
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    float inv;
-    pow2_scale(m, qup[r], inv);
+    float up, inv;
+    pow2_scale(m, up, inv);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) qup[nt][e] = __shfl_sync(0xffffffffu, up, 4 * (2 * c + e));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float f[8];
       unpack8(x[i], f);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        qa[2 * i + j][r] = cvt_f16x2(f[4 * j] * inv, f[4 * j + 1] * inv);
-        qa[2 * i + j][r + 2] = cvt_f16x2(f[4 * j + 2] * inv, f[4 * j + 3] * inv);
+        qb[nt][2 * i + j][0] = cvt_f16x2(f[4 * j] * inv, f[4 * j + 1] * inv);
+        qb[nt][2 * i + j][1] = cvt_f16x2(f[4 * j + 2] * inv, f[4 * j + 3] * inv);
       }
     }
   }
 
-  float o[16][4];
+  float o[NT][8][4];      // [..][t]: channels 16 g + 2 t (+ 1), rows 8 nt + 2 c (+ 1)
+  float m[NT][2], l[NT][2];
 #pragma unroll
-  for (int t = 0; t < 16; ++t)
+  for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[t][e] = 0.0f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[nt][t][e] = 0.0f;
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.0f;
+  }
 
-  // softmax of one step's scores s[nt][..] and p.v over four V rows given as
-  // f16 pair producers
-  const auto absorb = [&](float (&s)[2][4], const KeyScalars& mine, auto&& vpair) {
-    float sk[4], lsv[4], rsv[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sk[i] = __shfl_sync(0xffffffffu, mine.sk, vkey(i));
-      lsv[i] = __shfl_sync(0xffffffffu, mine.lsv, vkey(i));
-      rsv[i] = __shfl_sync(0xffffffffu, mine.rsv, vkey(i));
-    }
-    float t[2][4];   // [row][key]
+  // The softmax of a step's scores s[nt][mt] -> transposed weights: column
+  // fragments of two products of 16 keys (mt); `mine`: key `lane`'s numbers.
+  const auto softmax = [&](float (&s)[NT][2][4], const KeyScalars& mine, uint32_t (&pb)[NT][2][2]) {
+    float* key = sm.key[warp][0];
+    __syncwarp();                  // (the previous step's reads are done)
+    key[lane] = mine.sk;
+    key[kRowsStep + lane] = mine.lsv;
+    key[2 * kRowsStep + lane] = mine.rsv;
+    __syncwarp();
+    const float4 sk4 = *reinterpret_cast<const float4*>(key + 4 * g);
+    const float4 lsv4 = *reinterpret_cast<const float4*>(key + kRowsStep + 4 * g);
+    const float4 rsv4 = *reinterpret_cast<const float4*>(key + 2 * kRowsStep + 4 * g);
+    const float sk[4] = {sk4.x, sk4.y, sk4.z, sk4.w}, lsv[4] = {lsv4.x, lsv4.y, lsv4.z, lsv4.w};
+    const float rsv[4] = {rsv4.x, rsv4.y, rsv4.z, rsv4.w};
+    float t[NT][2][4], top[NT][2];   // [..][row e][key 4 g + i], i = 2 mt + half
     bool grow = false;
-    float top[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) t[r][i] = fmaf(s[i >> 1][2 * r + (i & 1)] * qup[r], sk[i], lsv[i]);
-      float x = fmaxf(fmaxf(t[r][0], t[r][1]), fmaxf(t[r][2], t[r][3]));
-      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-      top[r] = x;
-      grow |= x > m[r] + kRowsLag;
-    }
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          t[nt][e][i] = fmaf(s[nt][i >> 1][2 * (i & 1) + e] * qup[nt][e], sk[i], lsv[i]);
+        float x = fmaxf(fmaxf(t[nt][e][0], t[nt][e][1]), fmaxf(t[nt][e][2], t[nt][e][3]));
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+        top[nt][e] = x;
+        grow |= x > m[nt][e] + kRowsLag;
+      }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float mn = top[r] > m[r] + kRowsLag ? top[r] : m[r];
-        const float f = m[r] == mn ? 1.0f : ex2_ftz(m[r] - mn);   // (m = -inf: 0)
-        m[r] = mn;
-        l[r] *= f;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int tt = 0; tt < 16; ++tt) {
-          o[tt][2 * r] *= f;
-          o[tt][2 * r + 1] *= f;
+        for (int e = 0; e < 2; ++e) {
+          const float mn = top[nt][e] > m[nt][e] + kRowsLag ? top[nt][e] : m[nt][e];
+          const float f = m[nt][e] == mn ? 1.0f : ex2_ftz(m[nt][e] - mn);   // (m = -inf: 0)
+          m[nt][e] = mn;
+          l[nt][e] *= f;
+#pragma unroll
+          for (int tt = 0; tt < 8; ++tt) {
+            o[nt][tt][e] *= f;
+            o[nt][tt][2 + e] *= f;
+          }
+        }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float w[2][4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float base = m[nt][e] == -INFINITY ? 0.0f : m[nt][e] - kRowsBias;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[e][i] = ex2_ftz(t[nt][e][i] - base);
+          l[nt][e] = fmaf(w[e][i], rsv[i], l[nt][e]);
         }
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pb[nt][i >> 1][i & 1] = transpose8x8(cvt_f16x2(w[0][i], w[1][i]));
     }
-    uint32_t pa[4];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float base = m[r] == -INFINITY ? 0.0f : m[r] - kRowsBias;
-      float w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = ex2_ftz(t[r][i] - base);
-        l[r] = fmaf(w[i], rsv[i], l[r]);
-      }
-      pa[r] = cvt_f16x2(w[0], w[1]);
-      pa[r + 2] = cvt_f16x2(w[2], w[3]);
-    }
-#pragma unroll
-    for (int tt = 0; tt < 16; ++tt) mma_f16(o[tt], pa, vpair(0, tt), vpair(1, tt));
   };
 
   // ---- cached keys
   for (int i = 0; i < mine_n; ++i) {
-    cp_async_wait<kRowsRing - 2>();
+    cp_async_wait<2 * DEPTH - 1>();        // K
     __syncwarp();
-    issue(i + kRowsRing - 1);              // into the slot of step i - 1, which every lane has read
-    const bool next_valid = mask_of(i + 1);
-    const uint8_t* st = sm.ring[warp][i % kRowsRing];
-    const float* scales = reinterpret_cast<const float*>(st + kRowsCodes);
-    const KeyScalars mine = key_scalars(p, scales[lane & 15], scales[16 + (lane & 15)], valid);
-    float s[2][4];
+    const uint8_t* kst = sm.half[warp][0][i % DEPTH];
+    const uint8_t* vst = sm.half[warp][1][i % DEPTH];
+    const float ks = reinterpret_cast<const float*>(kst + kRowsStep * kCaD)[lane];
+    float s[NT][2][4];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
+    for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][mt][e] = 0.0f;
+      const int row = 4 * g + 2 * mt;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint4 x = *reinterpret_cast<const uint4*>(st + (nt * 8 + g) * kCaD + (((2 * c + h) ^ g) << 4));
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        const uint4 x = *reinterpret_cast<const uint4*>(kst + row * kCaD + (((2 * c + h) ^ rows_swizzle(row)) << 4));
+        const uint4 y =
+            *reinterpret_cast<const uint4*>(kst + (row + 1) * kCaD + (((2 * c + h) ^ rows_swizzle(row + 1)) << 4));
+        const uint32_t xa[4] = {x.x, x.y, x.z, x.w}, ya[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t u = w[j] ^ 0x80808080u;
-          mma_f16(s[nt], qa[4 * h + j], code_pair(u, 0x4140), code_pair(u, 0x4342));
+          const uint32_t u = xa[j] ^ 0x80808080u, v = ya[j] ^ 0x80808080u;
+          const uint32_t a[4] = {code_pair(u, 0x4140), code_pair(v, 0x4140), code_pair(u, 0x4342), code_pair(v, 0x4342)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt][mt], a, qb[nt][4 * h + j][0], qb[nt][4 * h + j][1]);
         }
       }
     }
-    // channel t of two V rows: interleave the rows' bytes, then widen
-    uint32_t il[2][8];
+    __syncwarp();
+    issue(i + DEPTH, 0);                   // (every lane has read K)
+    const bool next_valid = mask_of(i + 1);
+    cp_async_wait<2 * DEPTH - 1>();        // V
+    __syncwarp();
+    const float vs = reinterpret_cast<const float*>(vst + kRowsStep * kCaD)[lane];
+    uint32_t pb[NT][2][2];
+    softmax(s, key_scalars(p, ks, vs, valid), pb);
+    valid = next_valid;
 #pragma unroll
-    for (int pr = 0; pr < 2; ++pr) {
-      const uint8_t* v0 = st + kRowsCodes / 2 + vkey(2 * pr) * kCaD + ((g ^ (2 * c)) << 4);
-      const uint8_t* v1 = st + kRowsCodes / 2 + vkey(2 * pr + 1) * kCaD + ((g ^ (2 * c + 1)) << 4);
-      const uint4 x = *reinterpret_cast<const uint4*>(v0), y = *reinterpret_cast<const uint4*>(v1);
-      const uint32_t xa[4] = {x.x, x.y, x.z, x.w}, ya[4] = {y.x, y.y, y.z, y.w};
+    for (int mt = 0; mt < 2; ++mt) {
+      // columns of the transposed weights: keys 8 c + 2 mt + half and + 4; the
+      // rows' bytes are interleaved, then widened
+      uint32_t il[2][8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        il[pr][2 * k] = prmt(xa[k], ya[k], 0x5140) ^ 0x80808080u;
-        il[pr][2 * k + 1] = prmt(xa[k], ya[k], 0x7362) ^ 0x80808080u;
+      for (int half = 0; half < 2; ++half) {
+        const int row = 8 * c + 2 * mt + half;
+        const uint4 x = *reinterpret_cast<const uint4*>(vst + row * kCaD + ((g ^ rows_swizzle(row)) << 4));
+        const uint4 y = *reinterpret_cast<const uint4*>(vst + (row + 4) * kCaD + ((g ^ rows_swizzle(row + 4)) << 4));
+        const uint32_t xa[4] = {x.x, x.y, x.z, x.w}, ya[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          il[half][2 * k] = prmt(xa[k], ya[k], 0x5140) ^ 0x80808080u;
+          il[half][2 * k + 1] = prmt(xa[k], ya[k], 0x7362) ^ 0x80808080u;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const uint32_t a[4] = {code_pair(il[0][t], 0x4140), code_pair(il[0][t], 0x4342), code_pair(il[1][t], 0x4140),
+                               code_pair(il[1][t], 0x4342)};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][t], a, pb[nt][mt][0], pb[nt][mt][1]);
       }
     }
-    absorb(s, mine, [&](int pr, int tt) { return code_pair(il[pr][tt >> 1], (tt & 1) ? 0x4342 : 0x4140); });
-    valid = next_valid;
+    __syncwarp();
+    issue(i + DEPTH, 1);                   // (every lane has read V)
   }
   cp_async_wait<0>();
   int step = step0 + mine_n * kRowsWarps;
@@ -301,94 +360,115 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 3) cached_attn_rows_kernel(co
   for (; step < step_end; step += kRowsWarps) {
     const int k0 = (step - cached_steps) * kRowsStep;
     const auto fresh_ok = [&](int key) { return key < p.sk && (!mask || mask[p.extent + key] != 0); };
-    float s[2][4], kup[2];
+    const auto row_of = [&](int z, int key) {
+      return z ? p.v + b * p.v_sb + int64_t(key) * p.v_ss + kvh * p.v_sh : p.k + b * p.k_sb + int64_t(key) * p.k_ss + kvh * p.k_sh;
+    };
+    // lane j holds key j's scales: they are found first, row by row
+    float up[2] = {1.0f, 1.0f}, inv[2] = {1.0f, 1.0f};
+    for (int j = 0; j < min(kRowsStep, p.sk - k0); ++j) {
+      if (!fresh_ok(k0 + j)) continue;
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      const int key = k0 + nt * 8 + g;
-      uint4 x[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (fresh_ok(key)) {
-        const uint4* src = reinterpret_cast<const uint4*>(p.k + b * p.k_sb + int64_t(key) * p.k_ss + kvh * p.k_sh + 32 * c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __ldg(src + i);
+      for (int z = 0; z < 2; ++z) {
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(row_of(z, k0 + j)) + lane);
+        const uint32_t mx = absmax8(make_uint4(x.x, x.y, 0u, 0u), 0u);
+        float u, v;
+        pow2_scale(__reduce_max_sync(0xffffffffu, mx), u, v);
+        if (lane == j) up[z] = u, inv[z] = v;
       }
-      uint32_t mx = 0;
+    }
+    float s[NT][2][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mx = absmax8(x[i], mx);
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      float inv;
-      pow2_scale(mx, kup[nt], inv);
+    for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][mt][e] = 0.0f;
+      float f_inv[2];
+      bool held[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = 4 * g + 2 * mt + half;
+        f_inv[half] = __shfl_sync(0xffffffffu, inv[0], row);
+        held[half] = fresh_ok(k0 + row);
+      }
+      if (!__any_sync(0xffffffffu, held[0] || held[1])) continue;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float f[8];
-        unpack8(x[i], f);
+        float f[2][8];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          mma_f16(s[nt], qa[2 * i + j], cvt_f16x2(f[4 * j] * inv, f[4 * j + 1] * inv),
-                  cvt_f16x2(f[4 * j + 2] * inv, f[4 * j + 3] * inv));
+        for (int half = 0; half < 2; ++half) {
+          const int row = 4 * g + 2 * mt + half;
+          unpack8(held[half] ? __ldg(reinterpret_cast<const uint4*>(row_of(0, k0 + row)) + 4 * c + i)
+                             : make_uint4(0u, 0u, 0u, 0u), f[half]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[half][e] *= f_inv[half];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t a[4] = {cvt_f16x2(f[0][4 * j], f[0][4 * j + 1]), cvt_f16x2(f[1][4 * j], f[1][4 * j + 1]),
+                                 cvt_f16x2(f[0][4 * j + 2], f[0][4 * j + 3]), cvt_f16x2(f[1][4 * j + 2], f[1][4 * j + 3])};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt][mt], a, qb[nt][2 * i + j][0], qb[nt][2 * i + j][1]);
+        }
       }
     }
-    float vf[4][16], vup[4];
+    uint32_t pb[NT][2][2];
+    softmax(s, key_scalars(p, up[0], up[1], fresh_ok(k0 + lane)), pb);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = k0 + vkey(i);
-      uint4 x[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-      if (fresh_ok(key)) {
-        const uint4* src = reinterpret_cast<const uint4*>(p.v + b * p.v_sb + int64_t(key) * p.v_ss + kvh * p.v_sh + 16 * g);
-        x[0] = __ldg(src);
-        x[1] = __ldg(src + 1);
+    for (int mt = 0; mt < 2; ++mt) {
+      float v_inv[4];                      // keys 8 c + 2 mt + {0, 4, 1, 5}
+      bool held[4], any = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = 8 * c + 2 * mt + (e >> 1) + 4 * (e & 1);
+        v_inv[e] = __shfl_sync(0xffffffffu, inv[1], row);
+        held[e] = fresh_ok(k0 + row);
+        any |= held[e];
       }
-      uint32_t mx = absmax8(x[1], absmax8(x[0], 0));
+      if (!__any_sync(0xffffffffu, any)) continue;
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      float inv;
-      pow2_scale(mx, vup[i], inv);
-      unpack8(x[0], vf[i]);
-      unpack8(x[1], vf[i] + 8);
+      for (int q = 0; q < 2; ++q) {        // channels 16 g + 8 q .. + 7
+        float f[4][8];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) vf[i][e] *= inv;
+        for (int e = 0; e < 4; ++e) {
+          const int row = 8 * c + 2 * mt + (e >> 1) + 4 * (e & 1);
+          unpack8(held[e] ? __ldg(reinterpret_cast<const uint4*>(row_of(1, k0 + row)) + 2 * g + q)
+                          : make_uint4(0u, 0u, 0u, 0u), f[e]);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) f[e][x] *= v_inv[e];
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t a[4] = {cvt_f16x2(f[0][2 * t], f[1][2 * t]), cvt_f16x2(f[0][2 * t + 1], f[1][2 * t + 1]),
+                                 cvt_f16x2(f[2][2 * t], f[3][2 * t]), cvt_f16x2(f[2][2 * t + 1], f[3][2 * t + 1])};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * q + t], a, pb[nt][mt][0], pb[nt][mt][1]);
+        }
+      }
     }
-    // lane j < 16 collects key j's scales from the threads that hold them
-    const int j = lane & 15;
-    float ks = 0.0f, vs = 0.0f;
-    {
-      const float k_lo = __shfl_sync(0xffffffffu, kup[0], (j & 7) * 4), k_hi = __shfl_sync(0xffffffffu, kup[1], (j & 7) * 4);
-      ks = j < 8 ? k_lo : k_hi;
-      float part[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) part[i] = __shfl_sync(0xffffffffu, vup[i], (j & 7) >> 1);
-      vs = j < 8 ? ((j & 1) ? part[1] : part[0]) : ((j & 1) ? part[3] : part[2]);
-    }
-    const KeyScalars mine = key_scalars(p, ks, vs, fresh_ok(k0 + j));
-    absorb(s, mine, [&](int pr, int tt) { return cvt_f16x2(vf[2 * pr][tt], vf[2 * pr + 1][tt]); });
   }
 
   // ---- join the warps
-  __syncthreads();          // (every ring is done)
+  __syncthreads();          // (the staged steps are done)
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    const int row = g + 8 * r;
-    if (c == 0) {
-      sm.m[warp][row] = m[r];
-      sm.l[warp][row] = l[r];
-    }
-    // product t, columns 2c and 2c + 1: channels 32c + t and 32c + 16 + t
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int t4 = 0; t4 < 4; ++t4) {
-      float4* dst = reinterpret_cast<float4*>(&sm.o[warp][row][32 * c + 4 * t4]);
-      dst[0] = make_float4(o[4 * t4][2 * r], o[4 * t4 + 1][2 * r], o[4 * t4 + 2][2 * r], o[4 * t4 + 3][2 * r]);
-      dst[4] = make_float4(o[4 * t4][2 * r + 1], o[4 * t4 + 1][2 * r + 1], o[4 * t4 + 2][2 * r + 1],
-                           o[4 * t4 + 3][2 * r + 1]);
+    for (int e = 0; e < 2; ++e) {
+      const int row = 8 * nt + 2 * c + e;
+      float sum = l[nt][e];
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if (g == 0) {
+        sm.m[warp][row] = m[nt][e];
+        sm.l[warp][row] = sum;
+      }
+#pragma unroll
+      for (int t = 0; t < 8; t += 2)
+        *reinterpret_cast<float4*>(&sm.o[warp][row][16 * g + 2 * t]) =
+            make_float4(o[nt][t][e], o[nt][t][2 + e], o[nt][t + 1][e], o[nt][t + 1][2 + e]);
     }
-  }
   __syncthreads();
-  const int live = min(kRowsTile, rows - tile * kRowsTile);
+  const int live = min(ROWS, rows);
   for (int row = warp; row < live; row += kRowsWarps) {
     float mx = -INFINITY;
 #pragma unroll
@@ -430,40 +510,64 @@ __global__ void __launch_bounds__(kRowsWarps * 32, 3) cached_attn_rows_kernel(co
     }
     // no key at all: zeros (a NaN sum still divides, and stays NaN)
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int grow = tile * kRowsTile + row;
-    __nv_bfloat16* dst = p.out + b * p.o_sb + int64_t(grow / p.share) * p.o_ss +
-                         int64_t(kvh * p.share + grow % p.share) * p.o_sh + ch;
+    __nv_bfloat16* dst = p.out + b * p.o_sb + int64_t(row / p.share) * p.o_ss +
+                         int64_t(kvh * p.share + row % p.share) * p.o_sh + ch;
     const float f[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
     *reinterpret_cast<uint2*>(dst) = pack4(f);
   }
   cluster_sync();   // no CTA leaves while another reads its shared memory
 }
 
+// The shortest schedule of the keys over clusters of up to eight CTAs, in warp
+// steps: the waves of resident clusters, each a warp's share of the steps plus the
+// fixed part of a CTA (launch, query, joining), which costs as much as about six
+// of them.
+struct RowsPlan {
+  int64_t cost;
+  int splits;
+};
+
+template <int NT, int DEPTH>
+int plan_rows(int64_t groups, int steps, RowsPlan* plan) {
+  constexpr int smem = int(sizeof(RowsSmem<8 * NT, DEPTH>));
+  static const bool ready = cudaFuncSetAttribute(cached_attn_rows_kernel<NT, DEPTH>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess;
+  if (!ready) return set_error(QIA_ERR_CUDA, "qia_cached_attention: cudaFuncSetAttribute failed");
+  static int resident[17] = {0};
+  *plan = {INT64_MAX, 1};
+  for (int s = 1; s <= 8 && (s == 1 || s <= steps); ++s) {
+    const int64_t slots = resident_clusters(cached_attn_rows_kernel<NT, DEPTH>, kRowsWarps * 32, smem, s, resident);
+    if (slots == 0) continue;
+    const int64_t cost = (groups + slots - 1) / slots * ((steps + s * kRowsWarps - 1) / (s * kRowsWarps) + 6);
+    if (cost < plan->cost) *plan = {cost, s};
+  }
+  return QIA_OK;
+}
+
+template <int NT, int DEPTH>
+int run_rows(const CachedAttn& p, int batch, int splits, cudaStream_t st) {
+  return launch_cluster("cached_attn_rows_kernel", cached_attn_rows_kernel<NT, DEPTH>,
+                        dim3(unsigned(splits), unsigned(p.kv_heads), unsigned(batch)), kRowsWarps * 32,
+                        sizeof(RowsSmem<8 * NT, DEPTH>), splits, st, p);
+}
+
+// With few groups the device is not full, and a warp's own depth hides the
+// latency (three CTAs per SM); with many, one more CTA per SM does it better.
+template <int NT>
+int launch_rows(const CachedAttn& p, int batch, cudaStream_t st) {
+  const int64_t groups = int64_t(p.kv_heads) * batch;
+  const int steps = (p.extent + kRowsStep - 1) / kRowsStep + (p.sk + kRowsStep - 1) / kRowsStep;
+  RowsPlan deep, wide;
+  int rc = plan_rows<NT, 2>(groups, steps, &deep);
+  if (!rc) rc = plan_rows<NT, 1>(groups, steps, &wide);
+  if (rc) return rc;
+  return deep.cost <= wide.cost ? run_rows<NT, 2>(p, batch, deep.splits, st) : run_rows<NT, 1>(p, batch, wide.splits, st);
+}
+
 }  // namespace
 
 int launch_cached_rows(const CachedAttn& p, int batch, cudaStream_t st) {
-  static const int smem = [] {
-    return cudaFuncSetAttribute(cached_attn_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                int(sizeof(RowsSmem))) == cudaSuccess ? int(sizeof(RowsSmem)) : -1;
-  }();
-  if (smem < 0) return set_error(QIA_ERR_CUDA, "qia_cached_attention: cudaFuncSetAttribute failed");
-  const int64_t tiles = (int64_t(p.sq) * p.share + kRowsTile - 1) / kRowsTile;
-  const int64_t groups = tiles * p.kv_heads * batch;
-  const int steps = (p.extent + kRowsStep - 1) / kRowsStep + (p.sk + kRowsStep - 1) / kRowsStep;
-  // The keys are split as finely as leaves every warp two steps, up to a cluster
-  // of eight, but not into a second wave that would be nearly empty: past one
-  // wave (three CTAs per SM) only where that leaves several.
-  const int64_t slots = 3 * int64_t(sm_count());
-  int splits = 1;
-  for (int s = 2; s <= 8; ++s) {
-    if (steps < 2 * s * kRowsWarps) break;
-    if (groups * s <= slots || groups * s >= 2 * slots || groups * (s - 1) > slots) splits = s;
-  }
-  const int64_t gx = tiles * splits;
-  if (gx > 0x7fffffff) return set_error(QIA_ERR_UNSUPPORTED, "qia_cached_attention: too many query rows");
-  return launch_cluster("qia_cached_attention", cached_attn_rows_kernel,
-                        dim3(unsigned(gx), unsigned(p.kv_heads), unsigned(batch)), kRowsWarps * 32, size_t(smem),
-                        splits, st, p);
+  return int64_t(p.sq) * p.share <= 8 ? launch_rows<1>(p, batch, st) : launch_rows<2>(p, batch, st);
 }
 
 }  // namespace qia

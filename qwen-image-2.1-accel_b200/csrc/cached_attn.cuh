@@ -57,8 +57,11 @@ __device__ __forceinline__ KeyScalars key_scalars(const CachedAttn& p, float ks,
   // a zero row (scale 0) has zero codes: any vs gives the same value
   const float v = vs == 0.0f ? 1.0f : fmaxf(vs, 8.077935669e-28f);
   r.sk = valid ? p.scale_log2 * ks : 0.0f;
-  r.lsv = valid ? (vs == vs ? log2f(v) : vs) : -INFINITY;
-  r.rsv = valid ? 1.0f / v : 0.0f;
+  float lg, rc;                 // (relative errors below 2^-21)
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(v));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rc) : "f"(v));
+  r.lsv = valid ? (vs == vs ? lg : vs) : -INFINITY;
+  r.rsv = valid ? rc : 0.0f;
   return r;
 }
 

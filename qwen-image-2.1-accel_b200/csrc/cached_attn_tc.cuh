@@ -147,35 +147,6 @@ __device__ __forceinline__ void join_rows(const CachedAttn& p, const TileGrid& g
 }
 
 // ----------------------------------------------------------------------- host
-// Clusters of `size` CTAs of a kernel that the device holds at once (a cluster
-// stays within a GPU processing cluster, so this is less than SMs / size);
-// `cached`: nine zeros of static storage.
-template <class... KArgs>
-int resident_clusters(void (*kernel)(KArgs...), int threads, int smem, int size, int* cached) {
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lock(mu);
-  if (cached[size] == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(size));
-    cfg.blockDim = dim3(unsigned(threads));
-    cfg.dynamicSmemBytes = size_t(smem);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = unsigned(size);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
-      cudaGetLastError();
-      n = sm_count() / size > 0 ? sm_count() / size : 1;
-    }
-    cached[size] = n;
-  }
-  return cached[size];
-}
-
 // Runs `groups` groups of `tiles` key tiles: whole waves of one CTA per SM
 // unsplit; what is left over splits its keys so that it fills the device, when
 // that is shorter (in key tiles, with the fixed part of a CTA -- prologue and

@@ -2,6 +2,8 @@
 // memory (distributed shared memory), plus the host side of a cluster launch.
 #pragma once
 
+#include <mutex>
+
 #include "qia_common.cuh"
 
 namespace qia {
@@ -55,6 +57,35 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
 
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// Clusters of `size` CTAs of a kernel that the device holds at once (a cluster
+// stays within a GPU processing cluster, so this can be less than slots / size);
+// 0 where that size cannot run. `cached`: seventeen zeros of static storage.
+template <class... KArgs>
+int resident_clusters(void (*kernel)(KArgs...), int threads, int smem, int size, int* cached) {
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  if (cached[size] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(size));
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = size_t(smem);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(size);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = -1;
+    }
+    cached[size] = n;
+  }
+  return cached[size] > 0 ? cached[size] : 0;
 }
 
 // Launches `kernel` with clusters of `cluster` CTAs along x (grid.x a multiple
