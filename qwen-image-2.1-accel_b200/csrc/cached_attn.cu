@@ -533,7 +533,7 @@ int plan_rows(int64_t groups, int steps, RowsPlan* plan) {
   static const bool ready = cudaFuncSetAttribute(cached_attn_rows_kernel<NT, DEPTH>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess;
   if (!ready) return set_error(QIA_ERR_CUDA, "qia_cached_attention: cudaFuncSetAttribute failed");
-  static int resident[17] = {0};
+  static std::atomic<int> resident[17];
   *plan = {INT64_MAX, 1};
   for (int s = 1; s <= 8 && (s == 1 || s <= steps); ++s) {
     const int64_t slots = resident_clusters(cached_attn_rows_kernel<NT, DEPTH>, kRowsWarps * 32, smem, s, resident);

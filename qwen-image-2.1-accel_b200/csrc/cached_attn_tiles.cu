@@ -492,7 +492,7 @@ int launch_cached_tiles(const CachedAttn& p, int batch, cudaStream_t st) {
   TileGrid g = tile_grid(p);
   const int64_t groups = int64_t(g.pairs) * p.kv_heads * batch;
   if (groups > 0x0fffffff) return set_error(QIA_ERR_UNSUPPORTED, "qia_cached_attention: too many query rows");
-  static int resident[17] = {0};
+  static std::atomic<int> resident[17];
   return launch_waves(
       groups, (p.extent + 127) / 128 + (p.sk + 127) / 128,
       [&](int s) { return resident_clusters(cached_attn_tiles_kernel, kThreads, kSmemBytes, s, resident); },

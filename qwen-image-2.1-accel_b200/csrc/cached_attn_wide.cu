@@ -553,7 +553,7 @@ int launch_cached_wide(const CachedAttn& p, int batch, void* workspace, cudaStre
     rc = check_launch("cached_widen_kernel");
     if (rc) return rc;
   }
-  static int resident[17] = {0};
+  static std::atomic<int> resident[17];
   return launch_waves(
       groups, wd.tiles,
       [&](int s) { return resident_clusters(cached_attn_wide_kernel, kThreads, kSmemBytes, s, resident); },

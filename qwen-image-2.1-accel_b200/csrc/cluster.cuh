@@ -2,7 +2,7 @@
 // memory (distributed shared memory), plus the host side of a cluster launch.
 #pragma once
 
-#include <mutex>
+#include <atomic>
 
 #include "qia_common.cuh"
 
@@ -63,10 +63,9 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
 // stays within a GPU processing cluster, so this can be less than slots / size);
 // 0 where that size cannot run. `cached`: seventeen zeros of static storage.
 template <class... KArgs>
-int resident_clusters(void (*kernel)(KArgs...), int threads, int smem, int size, int* cached) {
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lock(mu);
-  if (cached[size] == 0) {
+int resident_clusters(void (*kernel)(KArgs...), int threads, int smem, int size, std::atomic<int>* cached) {
+  int n = cached[size].load(std::memory_order_relaxed);
+  if (n == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(size));
     cfg.blockDim = dim3(unsigned(threads));
@@ -78,14 +77,13 @@ int resident_clusters(void (*kernel)(KArgs...), int threads, int smem, int size,
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
       cudaGetLastError();
       n = -1;
     }
-    cached[size] = n;
+    cached[size].store(n, std::memory_order_relaxed);   // (every thread finds the same)
   }
-  return cached[size] > 0 ? cached[size] : 0;
+  return n > 0 ? n : 0;
 }
 
 // Launches `kernel` with clusters of `cluster` CTAs along x (grid.x a multiple

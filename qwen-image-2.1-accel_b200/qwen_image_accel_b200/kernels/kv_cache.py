@@ -9,15 +9,17 @@ the scores; `kv_cache_read` gives bf16 rows to an attention of another kind.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
 from .. import _lib
 
 HEAD_DIM = 128
-_Strides6 = ctypes.c_int64 * 6
-_Strides12 = ctypes.c_int64 * 12
+# stride arguments (int64[]) as bytes
+_strides6 = struct.Struct("6q").pack
+_strides12 = struct.Struct("12q").pack
+_NO_ROWS = (0,) * 6
 
 
 class QuantizedKV:
@@ -63,10 +65,11 @@ class QuantizedKV:
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
         self.lengths, self._tickets, self._parent = lengths, tickets, parent
         self.batch, self.kv_heads, self.capacity, self.extent = batch, heads, capacity, extent
-        self.device = k_codes.device
+        self.device, self._index = k_codes.device, k_codes.get_device()
         # the buffers' addresses, for the calls below
-        self._buffers = tuple(_lib.ptr(t) for t in (k_codes, v_codes, k_scales, v_scales, lengths))
-        self._ticket = _lib.ptr(tickets)
+        self._buffers = tuple(t.data_ptr() for t in (k_codes, v_codes, k_scales, v_scales, lengths))
+        self._ticket = tickets.data_ptr()
+        self._rows = torch.empty(0, dtype=torch.bfloat16, device=self.device)   # the type of rows read back
 
     def select(self, first: int, count: int = 1) -> "QuantizedKV":
         """Requests [first, first + count) of this cache, sharing its memory
@@ -94,7 +97,7 @@ def _check_rows(who: str, cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) 
                          f"{tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.stride(3) != 1 or v.stride(3) != 1:
         raise NotImplementedError(f"{who}: k and v must be bf16 with contiguous rows")
-    if k.device != cache.device or v.device != cache.device:
+    if k.get_device() != cache._index or v.get_device() != cache._index:
         raise ValueError(f"{who}: k, v and the cache are on different devices")
 
 
@@ -124,8 +127,8 @@ def kv_cache_append(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> Non
 def _write(cache, k, v, seq, start):
     kc, vc, ks, vs, lengths = cache._buffers
     _lib.call("qia_kv_cache_write", k.data_ptr(), v.data_ptr(), kc, vc, ks, vs, lengths, cache.batch, seq,
-              cache.kv_heads, HEAD_DIM, cache.capacity, start, _Strides6(*k.stride()[:3], *v.stride()[:3]),
-              cache._ticket, _lib.stream(cache.device))
+              cache.kv_heads, HEAD_DIM, cache.capacity, start, _strides6(*k.stride()[:3], *v.stride()[:3]),
+              cache._ticket, _lib.raw_stream(cache._index))
 
 
 def kv_cache_read(cache: QuantizedKV, first: int = 0, tokens: int | None = None, out_k: torch.Tensor | None = None,
@@ -139,16 +142,18 @@ def kv_cache_read(cache: QuantizedKV, first: int = 0, tokens: int | None = None,
     if first < 0 or tokens < 0 or first + tokens > cache.capacity:
         raise ValueError(f"kv_cache_read: tokens {first}+{tokens} of capacity {cache.capacity}")
     shape = (cache.batch, tokens, cache.kv_heads, HEAD_DIM)
+    given = out_k is not None or out_v is not None
     if out_k is None:
-        out_k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+        out_k = cache._rows.new_empty(shape)
     if out_v is None:
-        out_v = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
-    _check_rows("kv_cache_read", cache, out_k, out_v)
-    if out_k.shape != shape:
-        raise ValueError(f"kv_cache_read: the outputs must be {shape}, got {tuple(out_k.shape)}")
+        out_v = cache._rows.new_empty(shape) if given else torch.empty_like(out_k)
+    if given:
+        _check_rows("kv_cache_read", cache, out_k, out_v)
+        if out_k.shape != shape:
+            raise ValueError(f"kv_cache_read: the outputs must be {shape}, got {tuple(out_k.shape)}")
     _lib.call("qia_kv_cache_read", *cache._buffers, out_k.data_ptr(), out_v.data_ptr(), cache.batch, first, tokens,
-              cache.kv_heads, HEAD_DIM, cache.capacity, _Strides6(*out_k.stride()[:3], *out_v.stride()[:3]),
-              _lib.stream(cache.device))
+              cache.kv_heads, HEAD_DIM, cache.capacity, _strides6(*out_k.stride()[:3], *out_v.stride()[:3]),
+              _lib.raw_stream(cache._index))
     return out_k, out_v
 
 
@@ -166,43 +171,43 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
     gives zeros. scale defaults to 1/sqrt(128). Returns bf16 like q."""
     who = "cached_attention"
     _lib.require_cuda(q, key_valid)
-    if q.ndim != 4 or q.shape[0] != cache.batch or q.shape[3] != HEAD_DIM or q.shape[2] % cache.kv_heads:
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != cache.batch or shape[3] != HEAD_DIM or shape[2] % cache.kv_heads:
         raise ValueError(f"{who}: q must be [{cache.batch}, seq, a multiple of {cache.kv_heads}, {HEAD_DIM}], got "
-                         f"{tuple(q.shape)}")
-    if q.dtype != torch.bfloat16 or q.stride(3) != 1:
+                         f"{tuple(shape)}")
+    q_strides = q.stride()
+    if q.dtype != torch.bfloat16 or q_strides[3] != 1:
         raise NotImplementedError(f"{who}: q must be bf16 with contiguous rows")
-    if q.device != cache.device:
+    if q.get_device() != cache._index:
         raise ValueError(f"{who}: q and the cache are on different devices")
     if scale is not None and not scale > 0:
         raise ValueError(f"{who}: scale={scale} must be positive")
     if (k is None) != (v is None):
         raise ValueError(f"{who}: k and v come together")
-    fresh = 0
+    fresh, rows = 0, _NO_ROWS
     if k is not None:
         _check_rows(who, cache, k, v)
-        fresh = k.shape[1]
+        fresh, rows = k.shape[1], k.stride()[:3] + v.stride()[:3]
     mask_stride = 0
     if key_valid is not None:
         if key_valid.shape != (cache.batch, cache.extent + fresh) or key_valid.dtype != torch.bool:
             raise ValueError(f"{who}: key_valid must be bool [{cache.batch}, {cache.extent + fresh}], got "
                              f"{key_valid.dtype} {tuple(key_valid.shape)}")
-        if key_valid.stride(1) != 1 or key_valid.device != cache.device:
+        if key_valid.stride(1) != 1 or key_valid.get_device() != cache._index:
             raise NotImplementedError(f"{who}: key_valid must have contiguous rows on the cache's device")
         mask_stride = key_valid.stride(0)
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    elif (out.shape != q.shape or out.dtype != torch.bfloat16 or out.stride(3) != 1 or out.device != q.device):
+        out = torch.empty_like(q)
+    elif out.shape != shape or out.dtype != torch.bfloat16 or out.stride(3) != 1 or out.get_device() != cache._index:
         raise ValueError(f"{who}: out must be like q")
     if not out.numel():
         return out
-    size = _lib.load().qia_cached_attention_workspace_bytes(cache.batch, q.shape[1], fresh, q.shape[2], cache.kv_heads,
+    size = _lib.load().qia_cached_attention_workspace_bytes(cache.batch, shape[1], fresh, shape[2], cache.kv_heads,
                                                             cache.extent)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    kc, vc, ks, vs, lengths = cache._buffers
-    rows = (*k.stride()[:3], *v.stride()[:3]) if fresh else (0,) * 6
     _lib.call("qia_cached_attention", q.data_ptr(), k.data_ptr() if fresh else None, v.data_ptr() if fresh else None,
-              kc, vc, ks, vs, lengths, None if key_valid is None else key_valid.data_ptr(), out.data_ptr(),
-              cache.batch, q.shape[1], fresh, q.shape[2], cache.kv_heads, HEAD_DIM, cache.capacity, cache.extent,
-              _Strides12(*q.stride()[:3], *rows, *out.stride()[:3]), mask_stride,
-              0.0 if scale is None else float(scale), _lib.ptr(ws), _lib.stream(q.device))
+              *cache._buffers, None if key_valid is None else key_valid.data_ptr(), out.data_ptr(), cache.batch,
+              shape[1], fresh, shape[2], cache.kv_heads, HEAD_DIM, cache.capacity, cache.extent,
+              _strides12(*q_strides[:3], *rows, *out.stride()[:3]), mask_stride, 0.0 if scale is None else float(scale),
+              None if ws is None else ws.data_ptr(), _lib.raw_stream(cache._index))
     return out

@@ -7,14 +7,14 @@ linear or an MXFP8Linear).
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
 from .. import _lib
 
 MAX_RANK = 128
-_Strides6 = ctypes.c_int64 * 6
+_strides6 = struct.Struct("6q").pack      # stride arguments (int64[]) as bytes
 
 
 class LoraWeights:
@@ -47,8 +47,8 @@ class LoraWeights:
         self.ranks = torch.tensor(ranks, dtype=torch.int32, device=dev)
         self.scales = torch.tensor([float(s) for _, _, s in adapters], dtype=torch.float32, device=dev)
         _lib.require_cuda(self.a)
-        self.device = self.a.device
-        self._buffers = tuple(_lib.ptr(t) for t in (self.a, self.b, self.ranks, self.scales))
+        self.device, self._index = self.a.device, self.a.get_device()
+        self._buffers = tuple(t.data_ptr() for t in (self.a, self.b, self.ranks, self.scales))
 
 
 def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: torch.Tensor,
@@ -59,29 +59,32 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
     which may be `base` itself."""
     who = "lora_add"
     _lib.require_cuda(x, base, ids, out)
-    if x.ndim != 3 or x.shape[2] != weights.in_features or base.shape != (*x.shape[:2], weights.out_features):
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != weights.in_features or base.shape != (shape[0], shape[1], weights.out_features):
         raise ValueError(f"{who}: x {tuple(x.shape)} and base {tuple(base.shape)} do not fit a "
                          f"{weights.in_features} -> {weights.out_features} projection")
-    if x.dtype != torch.bfloat16 or base.dtype != torch.bfloat16 or x.stride(2) != 1 or base.stride(2) != 1:
+    batch, seq, _ = shape
+    x_strides, base_strides = x.stride(), base.stride()
+    if x.dtype != torch.bfloat16 or base.dtype != torch.bfloat16 or x_strides[2] != 1 or base_strides[2] != 1:
         raise NotImplementedError(f"{who}: x and base must be bf16 with contiguous rows")
-    batch, seq, _ = x.shape
     if ids.shape != (batch,) or ids.dtype != torch.int32 or not ids.is_contiguous():
         raise ValueError(f"{who}: ids must be int32 [{batch}], got {ids.dtype} {tuple(ids.shape)}")
     if out is None:
-        out = torch.empty(base.shape, dtype=torch.bfloat16, device=x.device)
-    elif out.shape != base.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1:
+        out = torch.empty_like(base)
+    elif out.shape != base.shape or out.dtype != torch.bfloat16:
         raise ValueError(f"{who}: out must be like base")
-    for t in (base, ids, out):
-        if t.device != x.device:
-            raise ValueError(f"{who}: tensors on different devices")
-    if x.device != weights.device:
-        raise ValueError(f"{who}: the adapters are on {weights.device}, x on {x.device}")
+    out_strides = out.stride()
+    if out_strides[2] != 1:
+        raise NotImplementedError(f"{who}: out must have contiguous rows")
+    index = weights._index
+    if x.get_device() != index or base.get_device() != index or ids.get_device() != index or out.get_device() != index:
+        raise ValueError(f"{who}: the adapters are on {weights.device}, x, base, ids or out are not")
     if not out.numel():
         return out
     size = _lib.load().qia_lora_workspace_bytes(batch, seq, weights.r_pad)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    a, b, ranks, scales = weights._buffers
-    _lib.call("qia_lora_add", x.data_ptr(), base.data_ptr(), out.data_ptr(), a, b, ranks, scales, ids.data_ptr(),
-              batch, seq, weights.in_features, weights.out_features, weights.count, weights.r_pad,
-              _Strides6(*x.stride()[:2], *base.stride()[:2], *out.stride()[:2]), _lib.ptr(ws), _lib.stream(x.device))
+    _lib.call("qia_lora_add", x.data_ptr(), base.data_ptr(), out.data_ptr(), *weights._buffers, ids.data_ptr(), batch,
+              seq, weights.in_features, weights.out_features, weights.count, weights.r_pad,
+              _strides6(*x_strides[:2], *base_strides[:2], *out_strides[:2]), None if ws is None else ws.data_ptr(),
+              _lib.raw_stream(index))
     return out
