@@ -5,12 +5,17 @@
 // columns past the adapter's own rank ignored. fp32 accumulation throughout,
 // one rounding of y to bf16. The padding of A and B holds zeros.
 //
-// Two forms. lora_tokens_kernel: few tokens per request. The weights are what is read (2
-// bytes per product), each by one CTA of a cluster that serves one request: the
-// cluster's warps share the rank rows of A (and, for small ranks, slices of the
-// contraction), every partial sum is stored into all CTAs' shared memory, and
-// after one cluster barrier each CTA computes its slice of the outputs. One
-// launch, fixed summation order.
+// Two forms. lora_tokens_kernel: up to eight tokens per request, which are the
+// columns of m16n8k16 products whose rows are weights: the weights are what is
+// read (2 bytes per product), straight from global memory into the operand
+// registers of the warp that uses them, and the call is a chain of latencies --
+// id, rows of A, exchange, rows of B (requested before the exchange), y. A cluster
+// of up to eight CTAs serves a request: its warps share the 16-row blocks of A
+// and slices of the contraction, every partial sum is stored into all CTAs'
+// shared memory, and after one cluster barrier each CTA computes its slice of the
+// outputs with t = scale A x as a sum of two bf16 numbers (2^-17 of t). One
+// launch, fixed summation order. (With one lane per weight row and fp32 FMAs the
+// same schedule executed ten times the instructions.)
 //
 // lora_shrink_kernel + lora_expand_kernel: many tokens per request, on tcgen05.
 // Both are bound by the bytes of x and of base and y, so a CTA is a stream of
@@ -60,114 +65,198 @@ __device__ __forceinline__ int lora_id(const Lora& p, int b, int* err) {
   return -1;
 }
 
-template <int TS>
-__global__ void __launch_bounds__(kTokWarps * 32) lora_tokens_kernel(const __grid_constant__ Lora p, int* err) {
-  // partial sums of A x: [slice of the contraction][token][rank]; slices x rank <= kTokWarps * cluster (or rank)
-  __shared__ float part[TS * (kLoraMaxRank > kTokWarps * 8 ? kLoraMaxRank : kTokWarps * 8)];
-  cluster_arrive();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ctas = int(cluster_size()), cta = int(cluster_rank());
-  const int chunk = blockIdx.x / ctas, b = blockIdx.y;
-  const int s0 = chunk * TS, live = min(TS, p.seq - s0);
-  const int id = lora_id(p, b, err);
-  const int rank = id < 0 ? 0 : min(max(__ldg(p.ranks + id), 0), p.r_pad);
-  const __nv_bfloat16* x = p.x + b * p.x_sb + int64_t(s0) * p.x_ss;
+constexpr int kTokens = 8;                      // tokens per cluster
+constexpr int kMaxSlices = 16;
+constexpr int kSums = kMaxSlices * 64;          // slices x ranks: at most 64 warps, 16 ranks each
 
-  int slices = 1;
-  while (slices < 8 && rank * slices * 2 <= kTokWarps * ctas) slices *= 2;
-  const int groups = p.in / 8;
-  cluster_wait();   // every CTA runs: its shared memory may be stored to
-  for (int item = warp * ctas + cta; item < rank * slices; item += kTokWarps * ctas) {
-    const int r = item / slices, slice = item % slices;
-    const uint4* arow = reinterpret_cast<const uint4*>(p.a + (int64_t(id) * p.r_pad + r) * p.in);
-    float acc[TS];
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+      "%2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Slices of the contraction: the cluster's warps over the 16-row blocks of A.
+__host__ __device__ __forceinline__ int token_slices(int r_pad, int ctas, int chunks) {
+  const int blocks = (r_pad + 15) / 16, n = kTokWarps * ctas / blocks, most = chunks < kMaxSlices ? chunks : kMaxSlices;
+  return n < 1 ? 1 : n < most ? n : most;
+}
+
+// kSteps: 16-rank steps of r_pad (2, 4 or 8); a warp has the rows of B of
+// up to four blocks of outputs in flight.
+template <int kSteps>
+__global__ void __launch_bounds__(kTokWarps * 32, 2) lora_tokens_kernel(const __grid_constant__ Lora p, int* err) {
+  constexpr int kPre = 8;                       // chunks of 32 channels (of 16 rows) in flight
+  constexpr int kRounds = kSteps == 8 ? 2 : 4;
+  __shared__ __align__(16) float part[kSums * kTokens];                       // [slice][rank][token]
+  __shared__ __align__(16) __nv_bfloat16 t_hi[kTokens][kLoraMaxRank + 8], t_lo[kTokens][kLoraMaxRank + 8];
+  __shared__ int col_b[kTokens], col_n;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int ctas = int(cluster_size()), cta = int(cluster_rank()), b = blockIdx.y;
+  // ---- the columns: eight tokens of request b, or, of single-token requests, b
+  // and the next seven with the same adapter (the others of the eight leave it to
+  // the first of them, so the weights are read once)
+  const int s0 = int(blockIdx.x) / ctas * kTokens;
+  const int raw = __ldg(p.ids + b);
+  if (p.seq == 1) {
+    if (warp == 0) {
+      int rank = 0, found = 0;
+      for (int i0 = 0; i0 < p.batch && found < kTokens; i0 += 32) {
+        const int i = i0 + lane, d = b - i0;
+        const uint32_t same = __ballot_sync(0xffffffffu, i < p.batch && __ldg(p.ids + i) == raw);
+        const uint32_t later = d <= 0 ? same : d >= 32 ? 0u : same & (0xffffffffu << d);
+        const int at = found + __popc(later & ((1u << lane) - 1u));
+        if (((later >> lane) & 1) && at < kTokens) col_b[at] = i;
+        rank += __popc(same ^ later);
+        found += __popc(later);
+      }
+      if (lane == 0) col_n = rank % kTokens ? 0 : min(found, kTokens);
+    }
+    __syncthreads();
+    if (col_n == 0) return;              // (the same in every CTA of the cluster)
+  } else {
+    if (threadIdx.x < kTokens) col_b[threadIdx.x] = b;
+    if (threadIdx.x == 0) col_n = min(kTokens, p.seq - s0);
+    __syncthreads();
+  }
+  cluster_arrive();
+  const int live = col_n, id = lora_id(p, b, err), at = max(id, 0);
+  // element offset of column `col` in a tensor of strides (sb, ss)
+  const auto column = [&](int col, int64_t sb, int64_t ss) {
+    return col_b[col] * sb + (p.seq == 1 ? int64_t(0) : int64_t(s0 + col) * ss);
+  };
+  const __nv_bfloat16* x = p.x + column(min(g, live - 1), p.x_sb, p.x_ss);
+
+  // ---- A x: 16 rows x this warp's slice; the products take channels 8 c .. 8 c + 7
+  // of a chunk from every c. The rows are requested before the adapter's rank is
+  // known (they exist up to r_pad).
+  const int blocks = (p.r_pad + 15) / 16, chunks = (p.in + 31) / 32, slices = token_slices(p.r_pad, ctas, chunks);
+  const int per = (chunks + slices - 1) / slices, ranks16 = blocks * 16;
+  const int items = id < 0 ? 0 : blocks * slices;
+  for (int item = warp * ctas + cta; item < items; item += kTokWarps * ctas) {
+    const int block = item % blocks, slice = item / blocks, end = min(chunks, (slice + 1) * per);
+    const uint4* row0 = reinterpret_cast<const uint4*>(p.a + (int64_t(at) * p.r_pad + min(16 * block + g, p.r_pad - 1)) * p.in);
+    const uint4* row1 =
+        reinterpret_cast<const uint4*>(p.a + (int64_t(at) * p.r_pad + min(16 * block + g + 8, p.r_pad - 1)) * p.in);
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = slice * per; k0 < end; k0 += kPre) {
+      uint4 a0[kPre], a1[kPre], xv[kPre];
 #pragma unroll
-    for (int t = 0; t < TS; ++t) acc[t] = 0.0f;
-    const int per = (groups + slices - 1) / slices;
-    const int end = min(groups, (slice + 1) * per);
-#pragma unroll 4
-    for (int i = slice * per + lane; i < end; i += 32) {
-      float w[8];
-      unpack8(__ldg(arow + i), w);
+      for (int k = 0; k < kPre; ++k) {
+        const int i = (k0 + k) * 4 + c;
+        const bool held = k0 + k < end && i * 8 < p.in;
+        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+        a0[k] = held ? __ldg(row0 + i) : zero;
+        a1[k] = held ? __ldg(row1 + i) : zero;
+        xv[k] = held && g < live ? __ldg(reinterpret_cast<const uint4*>(x) + i) : zero;
+      }
 #pragma unroll
-      for (int t = 0; t < TS; ++t) {
-        if (t < live) {
-          float f[8];
-          unpack8(__ldg(reinterpret_cast<const uint4*>(x + t * p.x_ss) + i), f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[t] = fmaf(w[e], f[e], acc[t]);
-        }
+      for (int k = 0; k < kPre; ++k) {
+        mma_bf16(acc, a0[k].x, a1[k].x, a0[k].y, a1[k].y, xv[k].x, xv[k].y);
+        mma_bf16(acc, a0[k].z, a1[k].z, a0[k].w, a1[k].w, xv[k].z, xv[k].w);
       }
     }
-#pragma unroll
-    for (int t = 0; t < TS; ++t) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], o);
-      if (lane < ctas) st_cluster_f32(cluster_map(&part[(slice * TS + t) * rank + r], lane), acc[t]);
+    if (item == warp * ctas + cta) cluster_wait();   // every CTA runs: its shared memory may be stored to
+    if (2 * c < live) {
+      float* dst = part + (slice * ranks16 + 16 * block + g) * kTokens + 2 * c;
+      for (int r = 0; r < ctas; ++r) {
+        const uint32_t peer = cluster_map(dst, uint32_t(r));
+        st_cluster_f32x2(peer, acc[0], acc[1]);
+        st_cluster_f32x2(peer + 8 * kTokens * 4, acc[2], acc[3]);
+      }
     }
   }
+  if (warp * ctas + cta >= items) cluster_wait();
+
+  // ---- rows of B and base of kRounds blocks of 16 outputs: channels 16 k + 4 c .. + 3 of every c
+  const int rank = id < 0 ? 0 : min(max(__ldg(p.ranks + at), 0), p.r_pad), steps = (rank + 15) / 16;
+  const float scale = __ldg(p.scales + at);
+  const int out_blocks = (p.out + 15) / 16, stride = ctas * kTokWarps;
+  int64_t col_base[2], col_y[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    col_base[e] = column(min(2 * c + e, live - 1), p.base_sb, p.base_ss);
+    col_y[e] = column(min(2 * c + e, live - 1), p.y_sb, p.y_ss);
+  }
+  uint2 w[kRounds][kSteps][2];
+  float base[kRounds][2][2];
+  const auto load = [&](int first) {
+#pragma unroll
+    for (int q = 0; q < kRounds; ++q)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int o = (first + q * stride) * 16 + g + 8 * h;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+          w[q][k][h] = k < steps && 16 * k + 4 * c < p.r_pad && o < p.out
+                           ? __ldg(reinterpret_cast<const uint2*>(p.b + (int64_t(at) * p.out + o) * p.r_pad + 16 * k + 4 * c))
+                           : make_uint2(0u, 0u);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          base[q][h][e] = o < p.out && 2 * c + e < live ? bf16_to_f32(p.base[col_base[e] + o]) : 0.0f;
+      }
+  };
+  int ob = cta * kTokWarps + warp;
+  load(ob);
   cluster_sync();
-  // the slices of a rank are added in order, into slice 0
-  for (int i = threadIdx.x; i < TS * rank; i += blockDim.x) {
-    float sum = part[i];
-    for (int k = 1; k < slices; ++k) sum += part[k * TS * rank + i];
-    part[i] = sum * __ldg(p.scales + id);
+  for (int i = threadIdx.x; i < ranks16 * kTokens; i += blockDim.x) {
+    const int r = i / kTokens, tok = i % kTokens;
+    float sum = 0.0f;
+    if (tok < live && r < rank)
+      for (int k = 0; k < slices; ++k) sum += part[(k * ranks16 + r) * kTokens + tok];
+    sum *= scale;
+    const __nv_bfloat16 hi = f32_to_bf16(sum);
+    t_hi[tok][r] = hi;
+    t_lo[tok][r] = f32_to_bf16(sum - bf16_to_f32(hi));
   }
   __syncthreads();
-
-  // ---- outputs: `lanes` lanes of eight ranks each per output, 32 outputs per warp and round
-  int lanes = 1;
-  while (lanes * 8 < rank) lanes *= 2;
-  const int per_round = 32 / lanes, group = lane / lanes, sub = lane % lanes;
-  const int blocks = (p.out + 31) / 32;
-  for (int ob = cta * kTokWarps + warp; ob < blocks; ob += ctas * kTokWarps) {
-    float mine[TS];
+  uint2 th[kSteps], tl[kSteps];
 #pragma unroll
-    for (int t = 0; t < TS; ++t) mine[t] = 0.0f;
-    if (rank) {
-      for (int j = 0; j < lanes; ++j) {
-        const int o = ob * 32 + j * per_round + group;
-        float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = 0.0f;
-        if (o < p.out && sub * 8 < rank)
-          unpack8(__ldg(reinterpret_cast<const uint4*>(p.b + (int64_t(id) * p.out + o) * p.r_pad) + sub), w);
-#pragma unroll
-        for (int t = 0; t < TS; ++t) {
-          float v = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (sub * 8 + e < rank) v = fmaf(w[e], part[t * rank + sub * 8 + e], v);
-          for (int k = 1; k < lanes; k *= 2) v += __shfl_xor_sync(0xffffffffu, v, k);
-          v = __shfl_sync(0xffffffffu, v, (lane % per_round) * lanes);
-          if (lane / per_round == j) mine[t] = v;
-        }
-      }
+  for (int k = 0; k < kSteps; ++k) {
+    th[k] = tl[k] = make_uint2(0u, 0u);
+    if (k < steps) {
+      th[k] = *reinterpret_cast<const uint2*>(&t_hi[g][16 * k + 4 * c]);
+      tl[k] = *reinterpret_cast<const uint2*>(&t_lo[g][16 * k + 4 * c]);
     }
-    const int o = ob * 32 + lane;
-    if (o < p.out) {
+  }
+  while (ob < out_blocks) {
 #pragma unroll
-      for (int t = 0; t < TS; ++t) {
-        if (t < live) {
-          const float v = bf16_to_f32(p.base[b * p.base_sb + int64_t(s0 + t) * p.base_ss + o]) + mine[t];
-          p.y[b * p.y_sb + int64_t(s0 + t) * p.y_ss + o] = f32_to_bf16(v);
+    for (int q = 0; q < kRounds; ++q) {
+      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+        if (k < steps) {
+          mma_bf16(acc, w[q][k][0].x, w[q][k][1].x, w[q][k][0].y, w[q][k][1].y, th[k].x, th[k].y);
+          mma_bf16(acc, w[q][k][0].x, w[q][k][1].x, w[q][k][0].y, w[q][k][1].y, tl[k].x, tl[k].y);
         }
-      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int o = (ob + q * stride) * 16 + g + 8 * h, tok = 2 * c + e;
+          if (o < p.out && tok < live)
+            p.y[col_y[e] + o] = f32_to_bf16(base[q][h][e] + acc[2 * h + e]);
+        }
     }
+    ob += kRounds * stride;
+    if (ob < out_blocks) load(ob);
   }
 }
 
 int launch_tokens(const Lora& p, cudaStream_t st) {
-  const bool one = p.seq == 1;
-  const int64_t chunks = one ? 1 : (int64_t(p.seq) + 7) / 8;
-  // four CTAs of 256 threads per SM at most; a cluster has work for at most out / 256 of them
+  const int64_t chunks = (int64_t(p.seq) + kTokens - 1) / kTokens;
+  // two CTAs of 256 threads per SM; a CTA has work for its warps down to 128 outputs or 256 channels
   int ctas = 1;
-  while (ctas < 8 && chunks * p.batch * ctas < 4 * sm_count() && ctas * kTokWarps * 32 < p.out) ctas *= 2;
+  while (ctas < 8 && chunks * p.batch * ctas < 2 * sm_count() &&
+         (ctas * kTokWarps * 16 < p.out || ctas * kTokWarps * 32 < p.in))
+    ctas *= 2;
   const dim3 grid(unsigned(chunks * ctas), unsigned(p.batch));
-  if (one) return launch_cluster("qia_lora_add", lora_tokens_kernel<1>, grid, kTokWarps * 32, 0, ctas, st, p,
-                                 device_error_word());
-  return launch_cluster("qia_lora_add", lora_tokens_kernel<8>, grid, kTokWarps * 32, 0, ctas, st, p,
-                        device_error_word());
+  const auto run = [&](auto kernel) {
+    return launch_cluster("qia_lora_add", kernel, grid, kTokWarps * 32, 0, ctas, st, p, device_error_word());
+  };
+  return p.r_pad <= 32 ? run(lora_tokens_kernel<2>) : p.r_pad <= 64 ? run(lora_tokens_kernel<4>) : run(lora_tokens_kernel<8>);
 }
 
 // ------------------------------------------------------------------ many tokens
@@ -452,6 +541,7 @@ int launch_tiles(const Lora& p, void* workspace, cudaStream_t st) {
   static const bool ready =
       cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            shrink_smem(kLoraMaxRank)) == cudaSuccess &&
+      cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
       cudaFuncSetAttribute(lora_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            expand_smem(kLoraMaxRank)) == cudaSuccess;
   if (!ready) return set_error(QIA_ERR_CUDA, "qia_lora_add: cudaFuncSetAttribute failed");
@@ -468,7 +558,7 @@ int launch_tiles(const Lora& p, void* workspace, cudaStream_t st) {
   const int blocks = (p.in + 63) / 64;
   // the contraction is split until the CTAs fill the device, down to two stages' worth each
   int splits = 1;
-  while (splits < 8 && tiles * p.batch * splits < sm_count() && blocks >= 4 * splits * 2) splits *= 2;
+  while (splits < 16 && tiles * p.batch * splits < sm_count() && blocks >= 4 * splits * 2) splits *= 2;
   rc = launch_cluster("lora_shrink_kernel", lora_shrink_kernel, dim3(unsigned(tiles * splits), unsigned(p.batch)), 192,
                       size_t(shrink_smem(p.r_pad)), splits, st, tm_x, tm_a, p, t, device_error_word());
   if (rc) return rc;
