@@ -4,6 +4,7 @@
 // requests of at most two query tiles, cached_attn_wide.cu for larger ones.)
 #pragma once
 
+#include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
 #include <mutex>
@@ -43,12 +44,95 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
   return out;
 }
 
+// The numerics of both forms. Keys are f16 rows, each tile of 128 keys scaled by
+// powers of two of its own:
+//   kw_j = ks_j kc_j 2^-e,  vw_j = vs_j vc_j 2^-f     (masked keys: zeros)
+// with the tile's largest |ks|, |vs| just inside 2^14. f16 keeps eleven bits down
+// to 2^-28 of that, an eighth of bf16's rounding, and no factor is left per key:
+// with x = q_i . kw_j (q_i scaled by a power of two per row),
+//   t_ij = x c_i + f,  c_i = c log2e 2^(e + e_i)        log2 of the weight of vw_j
+//   w_ij = 2^(t_ij - M_i + 8)
+//   o_i  = sum_j w_ij vw_j / sum_tiles 2^-f sum_j w_ij
+// so a score costs half a maximum, half a multiply-add, one exponential, half an
+// addition and half a conversion, and the softmax reads 32 bytes per tile. (With
+// the scales as per-key numbers in shared memory, a step of 256 x 128 scores took
+// 5700 cycles instead of 4200: the broadcast reads compete with the MMA operands.)
+// The accumulators are rescaled only when a row's maximum grew by more than 2^7
+// (f16 weights are at most 2^15).
+constexpr float kBias = 8.0f, kLag = 7.0f;
+constexpr uint32_t kIdescS = (1u << 4) | (uint32_t(128 >> 3) << 17) | (uint32_t(128 >> 4) << 24);   // f16 x f16 -> f32
+constexpr uint32_t kIdescO = kIdescS | (1u << 16);   // B (V) is MN-major
+
+// A tile of 128 keys: the softmax's numbers and which keys take part.
+constexpr int kInfoBytes = 32;
+struct __align__(16) TileInfo {
+  float c, f, inv_f;     // c log2e 2^e, f, 2^-f
+  uint32_t all;          // every key takes part
+  uint32_t valid[4];
+};
+static_assert(sizeof(TileInfo) == kInfoBytes, "bulk copy size");
+
+__device__ __forceinline__ uint32_t cvt_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Four codes (a word of INT8) times a -> four f16: byte u = code + 128 under
+// 0x4B0000 is the float 2^23 + u.
+__device__ __forceinline__ uint2 widen4(uint32_t w, float a) {
+  const uint32_t u = w ^ 0x80808080u;
+  const uint64_t off = f2_pack(-8388736.0f, -8388736.0f), a2 = f2_pack(a, a);
+  float x[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t t = f2_pack(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + 2 * i)),
+                               __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7541 + 2 * i)));
+    f2_unpack(f2_mul(f2_add(t, off), a2), x[2 * i], x[2 * i + 1]);
+  }
+  return make_uint2(cvt_f16x2(x[0], x[1]), cvt_f16x2(x[2], x[3]));
+}
+
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
+
+// Exponent e with max 2^-e in [2^13, 2^14) for a maximum given as bits; kept in
+// a range where c 2^(e + e_i) and 2^+-f stay normal (rows beyond it only lose
+// bits: below 2^-44 they no longer matter to a score, above they saturate f16
+// to infinity at 2^106). Of INT8 rows: the maximum scale, |code| < 2^7.
+__device__ __forceinline__ int tile_exponent(uint32_t bits, int lo) {
+  return min(max(int(bits >> 23) - 127 - 13, lo), 90);
+}
+constexpr int kLowK = -30, kLowV = -90;
+__device__ __forceinline__ int code_exponent(uint32_t scale_bits, int lo) { return tile_exponent(scale_bits + (7u << 23), lo); }
+
+// |x| as bits of a number that may set a tile's exponent: a NaN does not.
+__device__ __forceinline__ uint32_t magnitude(float x) { return x == x ? __float_as_uint(x) & 0x7fffffffu : 0u; }
+
+// The largest finite magnitude of eight bf16 values.
+__device__ __forceinline__ uint32_t finite_max8(const uint4& v, uint32_t m) {
+  const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t lo = (x[q] << 16) & 0x7fffffffu, hi = x[q] & 0x7fff0000u;
+    m = max(m, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+  }
+  return m;
+}
+
+__device__ __forceinline__ uint4 narrow8(const uint4& v, float a) {   // eight bf16 values times a -> f16
+  float f[8];
+  unpack8(v, f);
+  return make_uint4(cvt_f16x2(f[0] * a, f[1] * a), cvt_f16x2(f[2] * a, f[3] * a), cvt_f16x2(f[4] * a, f[5] * a),
+                    cvt_f16x2(f[6] * a, f[7] * a));
+}
+
 // Query tiles and groups: a tile is 128 / share tokens of all heads that share a
 // K/V head; a group is a pair of tiles of one (request, K/V head).
 struct TileGrid {
   int tokens_per_tile;
   int q_tiles, pairs;    // tiles of a request, and pairs of them
   int first_group;       // group = (request, K/V head, pair), pairs fastest
+  uint32_t share_inv;    // 2^16 / share rounded up: (row * share_inv) >> 16 = row / share for rows below 128
 };
 
 inline TileGrid tile_grid(const CachedAttn& p) {
@@ -56,7 +140,124 @@ inline TileGrid tile_grid(const CachedAttn& p) {
   g.tokens_per_tile = kTileRows / p.share;
   g.q_tiles = (p.sq + g.tokens_per_tile - 1) / g.tokens_per_tile;
   g.pairs = (g.q_tiles + 1) / 2;
+  g.share_inv = uint32_t((65536 + p.share - 1) / p.share);
   return g;
+}
+
+// A query tile into shared memory as f16, each row scaled by a power of two 2^e_i
+// (rows past the end are zeros), by the 128 threads of a softmax group (`t`; eight
+// rows per step, sixteen threads per row); 2^e_i into scale[128]. Announced on
+// q_full (four arrivals per tile).
+__device__ __forceinline__ void load_queries(const CachedAttn& p, const TileGrid& g, uint32_t slot, float* scale, int tile,
+                                             int t, int kvh, int b, uint64_t* q_full) {
+  const int tile_rows = g.tokens_per_tile * p.share, piece = t & 15;
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    uint4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = half * 64 + i * 8 + (t >> 4), part = int((uint32_t(row) * g.share_inv) >> 16);
+      const int token = tile * g.tokens_per_tile + part;
+      v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < tile_rows && token < p.sq)
+        v[i] = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_sb + int64_t(token) * p.q_ss +
+                                                    int64_t(kvh * p.share + row - part * p.share) * p.q_sh) + piece);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = half * 64 + i * 8 + (t >> 4);
+      float f[8];
+      unpack8(v[i], f);
+      uint32_t mx = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(f[e]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const int e = min(max(int(mx >> 23) - 127, -80), 120);
+      if (piece == 0) scale[row] = pow2f(e);
+      const uint4 h = narrow8(v[i], pow2f(-e));
+      st_shared_v4(slot + tile_offset(row, piece), h.x, h.y, h.z, h.w);
+    }
+  }
+  fence_proxy_async_shared();
+  __syncwarp();
+  if ((t & 31) == 0) mbar_arrive(smem_u32(q_full));
+}
+
+struct RowState {
+  float m, l;
+};
+
+// One softmax step of a thread's row: the 128 scores at TMEM column t_s -> f16
+// weights over the first 64 columns, each half announced on p_full[h]; `fresh`:
+// the row's accumulators (t_o) hold nothing yet.
+__device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, const TileInfo* info, float q_up, bool fresh,
+                                             RowState& st, uint64_t* p_full, int lane) {
+  uint32_t s[128];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    tc_ld_32x32b_x32(t_s + uint32_t(q * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[q * 32]));
+  const float4 num = *reinterpret_cast<const float4*>(info);
+  const float c = num.x * q_up, f = num.y;
+  tc_wait_ld();
+  if (!__float_as_uint(num.w)) {         // some keys take no part
+    const uint4 bits = *reinterpret_cast<const uint4*>(info->valid);
+    const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+    for (int i = 0; i < 128; ++i)
+      if (!((word[i >> 5] >> (i & 31)) & 1)) s[i] = 0xff800000u;
+  }
+  float mx[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s[i]);
+#pragma unroll
+  for (int i = 4; i < 124; i += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
+#pragma unroll
+  for (int k = 0; k < 2; ++k) mx[k] = max3(mx[k], __uint_as_float(s[124 + 2 * k]), __uint_as_float(s[125 + 2 * k]));
+  const float top = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), c, f);
+  const bool grow = top > st.m + kLag;
+  if (__any_sync(0xffffffffu, grow)) {
+    const float r = grow ? ex2_ftz(st.m - top) : 1.0f;   // (m = -inf: 0)
+    if (grow) st.m = top;
+    st.l *= r;
+    if (!fresh) {
+#pragma unroll 1
+      for (int q = 0; q < 8; ++q) {
+        uint32_t o[16];
+        tc_ld_32x32b_x16(t_o + uint32_t(q * 16), o);
+        tc_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * r);
+        tc_st_32x32b_x16(t_o + uint32_t(q * 16), o);
+      }
+    }
+  }
+  const float n1 = f + kBias - (st.m == -INFINITY ? 0.0f : st.m);
+  const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(n1, n1);
+  uint64_t sum[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t x[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      float a, b;
+      f2_unpack(f2_fma(f2_pack(__uint_as_float(s[64 * h + 2 * i]), __uint_as_float(s[64 * h + 2 * i + 1])), c2, n2), a, b);
+      a = ex2_ftz(a);
+      b = ex2_ftz(b);
+      sum[i & 1] = f2_add(sum[i & 1], f2_pack(a, b));
+      x[i] = cvt_f16x2(a, b);
+    }
+    tc_st_32x32b_x32(t_s + uint32_t(32 * h), x);
+    tc_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&p_full[h]));
+  }
+  float a, b;
+  f2_unpack(f2_add(sum[0], sum[1]), a, b);
+  st.l = fmaf(a + b, num.z, st.l);
 }
 
 // A softmax thread's row of accumulators (128 TMEM columns from t_o) / l -> out.

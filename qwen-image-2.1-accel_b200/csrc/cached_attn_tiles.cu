@@ -1,33 +1,25 @@
 // Attention of some tens to some hundreds of query rows over the INT8 prefix
-// cache (at most two tiles of 128 rows per request and K/V head), on tcgen05.
+// cache (at most two tiles of 128 rows per request and K/V head), on tcgen05,
+// converting the codes as it goes: numerics, tiles and joining as in
+// cached_attn_tc.cuh.
 //
 // Roles (512 threads, one CTA per SM):
 //   warps 0-3, 4-7  softmax groups 0 and 1 (a query row per thread): scores from
 //                   TMEM, weights back into TMEM;
 //   warp 8          issues the MMAs;
-//   warps 9-15      operand writers: INT8 codes -> bf16 (exact), fresh bf16 rows
-//                   copied, into the swizzled shared-memory tiles, and the
-//                   per-key numbers of the softmax.
+//   warps 9-15      operand writers: codes and fresh rows -> f16 in the swizzled
+//                   shared-memory tiles, and the tiles' numbers.
 // A key tile is 128 keys. K and V tiles (32 KB each) have two stages. TMEM:
-// scores of group i at columns [128 i, +128), its bf16 weights over the first 64
-// of them (the A operand of P.V), accumulators at 256 + 128 i. The groups own
-// the two query tiles of the CTA and see every key tile, or, when there is only
-// one query tile, both work on it with the even and the odd key tiles.
+// scores of group i at columns [128 i, +128), its weights over the first 64 of
+// them (the A operand of P.V), accumulators at 256 + 128 i. The groups own the two
+// query tiles of the CTA and see every key tile, or, when there is only one query
+// tile, both work on it with the even and the odd key tiles.
 //
 // The issuer runs, per softmax group: P(j).V(j), as each half of P(j) is stored,
 // then Q.K of the group's next key tile, so while one group's products run, the
 // other group's softmax works. MMAs of one thread complete in order: the next
 // Q.K may overwrite the scores that hold P(j), and once its scores are there,
-// the accumulators hold all of P.V up to j and the softmax may rescale them
-// (only when a row's maximum grew by more than 2^8, see cached_attn.cuh).
-//
-// Both products take the codes themselves; the softmax multiplies scores by
-// c log2e ks_j and weights by vs_j in fp32. Tiles whose keys all take part skip
-// the mask; fresh ones have no scales and touch no per-key number at all (the
-// broadcast reads of those share the shared-memory port with the operands).
-//
-// INT8 -> bf16: byte b under exponent byte 0x43; x = 128 + (b & 0x7f) and
-// c = 128 (b >= 0) or 256 (b < 0, exponent + 1) are bf16 patterns, x - c = b.
+// the accumulators hold all of P.V up to j and the softmax may rescale them.
 //
 // Keys may be split over a cluster, which joins through distributed shared
 // memory in rank order (no workspace, fixed order). Every wait is bounded (1 s)
@@ -39,89 +31,21 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWriters = 7;                     // operand-writer warps: arrivals of a written tile
-constexpr int kScalarBytes = 3 * 128 * 4;       // [sk | vs | bias][128] f32
-constexpr int kSmemML = kSmemTail + kScalarRing * kScalarBytes;   // m, l of 256 rows (joining)
-constexpr int kSmemBars = kSmemML + 2 * 256 * 4;
+constexpr int kSmemQScale = kSmemTail + kScalarRing * kInfoBytes;   // 2^e_i of 256 rows
+constexpr int kSmemML = kSmemQScale + 256 * 4;                      // m, l of 256 rows (joining)
+constexpr int kSmemFactor = kSmemML + 2 * 256 * 4;                  // [writer][K, V][128] scale 2^-e of a tile's keys
+constexpr int kSmemSlots = kSmemFactor + kWriters * 2 * 128 * 4;    // [writer] maxima
+constexpr int kSmemStage = kSmemSlots + 64;                         // codes of half a tile in flight
+constexpr int kStageBytes = kTileRows * kCaD;
+constexpr int kSmemBars = kSmemStage + kStageBytes;
 constexpr int kSmemBytes = kSmemBars + 256 + 1024;
 // registers of a softmax thread and of any other: 256 x 160 + 256 x 96 = 512 x 128, what the block starts with
 constexpr int kSoftmaxRegs = 160, kOtherRegs = 96;
-constexpr float kTilesLag = 8.0f;
-constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(128 >> 3) << 17) | (uint32_t(128 >> 4) << 24);
-constexpr uint32_t kIdescO = kIdescS | (1u << 16);   // B (V) is MN-major
-// kinds of a key tile, in the order of what the softmax has to read
-constexpr int kFreshFull = 0, kCachedFull = 1, kMasked = 2;
 
-__device__ __forceinline__ void cp_async16_zfill(uint32_t smem, const void* gmem, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
 }
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
-// bf16 pair of two codes of `w` (bytes picked by `sel`)
-__device__ __forceinline__ uint32_t codes_bf16x2(uint32_t w, uint32_t sel) {
-  const uint32_t t = __byte_perm(w, 0x43434343u, sel);
-  uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t & 0xff7fff7fu), "r"(t & 0xff80ff80u));
-  return r;
-}
-
-// The 128 scores of a row in registers -> their maximum, and for tiles with
-// per-key numbers also t = s * sk (+ bias) in place.
-template <int KIND>
-__device__ __forceinline__ float row_scores(uint32_t (&s)[128], const float* scal, float c) {
-  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int i = 0; i < 128; i += 4) {
-    if (KIND != kFreshFull) {
-      const float4 sk = *reinterpret_cast<const float4*>(scal + i);
-      uint64_t t0 = f2_pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-      uint64_t t1 = f2_pack(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
-      if (KIND == kMasked) {
-        const float4 bias = *reinterpret_cast<const float4*>(scal + 256 + i);
-        t0 = f2_fma(t0, f2_pack(sk.x, sk.y), f2_pack(bias.x, bias.y));
-        t1 = f2_fma(t1, f2_pack(sk.z, sk.w), f2_pack(bias.z, bias.w));
-      } else {
-        t0 = f2_mul(t0, f2_pack(sk.x, sk.y));
-        t1 = f2_mul(t1, f2_pack(sk.z, sk.w));
-      }
-      float a, b;
-      f2_unpack(t0, a, b);
-      s[i] = __float_as_uint(a);
-      s[i + 1] = __float_as_uint(b);
-      f2_unpack(t1, a, b);
-      s[i + 2] = __float_as_uint(a);
-      s[i + 3] = __float_as_uint(b);
-    }
-    mx[(i / 4) & 3] = max3(mx[(i / 4) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-    mx[(i / 4 + 2) & 3] = max3(mx[(i / 4 + 2) & 3], __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
-  }
-  const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-  return KIND == kFreshFull ? top * c : top;
-}
-
-// Weights of 64 keys (half h): w = 2^(t - m), their sum into l, and w (times vs
-// of cached keys) as bf16 pairs.
-template <int KIND>
-__device__ __forceinline__ void row_weights(const uint32_t (&s)[128], int h, const float* scal, float c, float neg_m,
-                                            uint64_t (&l)[2], uint32_t (&w)[32]) {
-  const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(neg_m, neg_m);
-#pragma unroll
-  for (int k = 0; k < 64; k += 4) {
-    const int i = h * 64 + k;
-    float4 vs;
-    if (KIND != kFreshFull) vs = *reinterpret_cast<const float4*>(scal + 128 + i);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const uint64_t x = f2_pack(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
-      float a, b;
-      f2_unpack(KIND == kFreshFull ? f2_fma(x, c2, n2) : f2_add(x, n2), a, b);
-      a = ex2_ftz(a);
-      b = ex2_ftz(b);
-      l[e] = f2_add(l[e], f2_pack(a, b));
-      if (KIND != kFreshFull) f2_unpack(f2_mul(f2_pack(a, b), e ? f2_pack(vs.z, vs.w) : f2_pack(vs.x, vs.y)), a, b);
-      w[k / 2 + e] = cvt_bf16x2(a, b);
-    }
-  }
-}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 __global__ void __launch_bounds__(kThreads, 1)
 cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_constant__ TileGrid tp, int* err) {
@@ -133,12 +57,13 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
   uint64_t* v_full = bars + 2;        // [2]
   uint64_t* k_empty = bars + 4;       // [2] issuer -> operand writers
   uint64_t* v_empty = bars + 6;       // [2]
-  uint64_t* scal_full = bars + 8;     // [4] operand writers -> softmax
+  uint64_t* info_full = bars + 8;     // [4] first operand writer -> softmax
   uint64_t* s_full = bars + 12;       // [2] scores of group i
   uint64_t* p_full = bars + 14;       // [2][2] weights of group i, half h, stored
   uint64_t* o_full = bars + 18;
   uint64_t* drain = bars + 19;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t* q_full = bars + 20;       // softmax -> issuer
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = int(cluster_size()), split = int(cluster_rank());
@@ -161,30 +86,17 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
       mbar_init(smem_u32(&s_full[i]), 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&p_full[i]), 4);
-    for (int i = 0; i < kScalarRing; ++i) mbar_init(smem_u32(&scal_full[i]), kWriters);
+    for (int i = 0; i < kScalarRing; ++i) mbar_init(smem_u32(&info_full[i]), 1);
     mbar_init(smem_u32(o_full), 1);
     mbar_init(smem_u32(drain), 1);
+    mbar_init(smem_u32(q_full), 4 * n_tiles);
     fence_barrier_init();
   }
   if (warp == 8) tmem_alloc(smem_u32(tmem_slot), 512);
-  // ---- query tiles (rows past the end are zeros)
-  const int tile_rows = tp.tokens_per_tile * p.share;
-  for (int i = threadIdx.x; i < n_tiles * kTileRows * 16; i += kThreads) {
-    const int tile = i >> 11, row = (i >> 4) & 127, piece = i & 15;
-    const int token = (2 * pair + tile) * tp.tokens_per_tile + row / p.share;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (row < tile_rows && token < p.sq)
-      v = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_sb + int64_t(token) * p.q_ss +
-                                               int64_t(kvh * p.share + row % p.share) * p.q_sh) + piece);
-    st_shared_v4(sbase + kSmemQ + tile * kTileBytes + tile_offset(row, piece), v.x, v.y, v.z, v.w);
-  }
-  fence_proxy_async_shared();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // key tiles of softmax group w: the it-th is it (both groups), or 2 it + w
-  const auto tiles_of = [&](int w) { return duo ? (n - w + 1) / 2 : n; };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -231,7 +143,7 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
           }
           return true;
         };
-        bool ok = true;
+        bool ok = wait(q_full, 0);
         if (duo) {
           for (int j = 0; j < 2 && j < n && ok; ++j) {
             ok = wait_k(j);
@@ -250,7 +162,7 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
             }
           }
         } else {
-          ok = wait_k(0);
+          ok = ok && wait_k(0);
           if (ok) {
             qk(0, 0);
             qk(1, 0);
@@ -277,201 +189,236 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
       }
     } else {
       // ------------------------------------------------------- operand writers
-      const int t = threadIdx.x - 32 * 9;
+      const int t = threadIdx.x - 32 * 9, writer = warp - 9;
       const int64_t head_row = (int64_t(b) * p.kv_heads + kvh) * p.capacity;
       const uint8_t* mask = p.key_valid ? p.key_valid + b * p.mask_sb : nullptr;
       const int cached_n = max(0, min(n, cached_tiles - first));   // cached tiles of this CTA
-      // codes of half tile u (2 j: K of tile j, 2 j + 1: V): eight threads per
-      // row, 28 rows per step
+      float* factor = reinterpret_cast<float*>(smem + kSmemFactor) + writer * 256;
+      // z: 0 K, 1 V. Codes: eight threads per row, 28 rows per step, through
+      // pieces of a staging buffer private to the warp, with cp.async: two halves of a
+      // tile in flight where the second query tile's space is free, one otherwise.
+      // (With plain loads a warp waits for all of its outstanding loads at the
+      // first use of any: 5300 cycles per tile.)
       constexpr int kSteps = 5;
-      const int trow = t >> 3;
-      const auto load_codes = [&](int u, uint4 (&c)[kSteps]) {
-        const int k0 = (first + (u >> 1)) * 128;
-        const int8_t* src = ((u & 1) ? p.vc : p.kc) + head_row * kCaD + (t & 7) * 16;
+      const int trow = t >> 3, depth = duo ? 2 : 1;
+      const uint32_t stage = duo ? sbase + kSmemQ + kTileBytes : sbase + kSmemStage;
+      const auto issue = [&](int u) {      // half u: K (even) or V of tile u / 2
+        if (u < 2 * cached_n) {
+          const int k0 = (first + (u >> 1)) * 128;
+          const int8_t* src = ((u & 1) ? p.vc : p.kc) + head_row * kCaD + (t & 7) * 16;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const int key = min(k0 + i * 28 + trow, len - 1);   // (past the length: any held row, weight 0)
-          c[i] = __ldg(reinterpret_cast<const uint4*>(src + int64_t(key) * kCaD));
-        }
-      };
-      const auto store_codes = [&](uint32_t slot, const uint4 (&c)[kSteps]) {
-        const int piece = (t & 7) * 2;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const int row = i * 28 + trow;
-          if (row >= kTileRows) break;
-          const uint32_t a0 = codes_bf16x2(c[i].x, 0x4140), a1 = codes_bf16x2(c[i].x, 0x4342);
-          const uint32_t a2 = codes_bf16x2(c[i].y, 0x4140), a3 = codes_bf16x2(c[i].y, 0x4342);
-          const uint32_t b0 = codes_bf16x2(c[i].z, 0x4140), b1 = codes_bf16x2(c[i].z, 0x4342);
-          const uint32_t b2 = codes_bf16x2(c[i].w, 0x4140), b3 = codes_bf16x2(c[i].w, 0x4342);
-          // the upper four lanes of a row write their second piece first: the
-          // eight lanes of a store phase then hit eight different bank groups
-          const bool up = t & 4;
-          st_shared_v4(slot + tile_offset(row, piece + up), up ? b0 : a0, up ? b1 : a1, up ? b2 : a2, up ? b3 : a3);
-          st_shared_v4(slot + tile_offset(row, piece + !up), up ? a0 : b0, up ? a1 : b1, up ? a2 : b2, up ? a3 : b3);
-        }
-      };
-      // the softmax's numbers of key tile j, one key per thread
-      float ks = 1.0f, vs = 1.0f;
-      bool valid = false;
-      const auto load_scalars = [&](int j) {
-        const int tile = first + j;
-        ks = vs = 1.0f;
-        if (tile < cached_tiles) {
-          const int key = tile * 128 + t;
-          valid = key < len && t < 128;
-          if (valid) {
-            ks = __ldg(p.ks + head_row + key);
-            vs = __ldg(p.vs + head_row + key);
-            valid = !mask || __ldg(mask + key) != 0;
+          for (int i = 0; i < kSteps; ++i) {
+            const int row = i * 28 + trow;
+            if (row < kTileRows)   // (past the length: any held row, factor 0)
+              cp_async16(stage + uint32_t(duo ? (u & 1) * kStageBytes : 0) + uint32_t(row * kCaD + (t & 7) * 16),
+                         src + int64_t(min(k0 + row, len - 1)) * kCaD);
           }
-        } else {
-          const int key = (tile - cached_tiles) * 128 + t;
-          valid = key < p.sk && t < 128 && (!mask || __ldg(mask + p.extent + key) != 0);
         }
+        cp_async_commit();      // (an empty group keeps the count)
       };
-      const auto store_scalars = [&](int j) {
-        if (t < 128) {
-          float* dst = reinterpret_cast<float*>(smem + kSmemTail + (j % kScalarRing) * kScalarBytes) + t;
-          dst[0] = valid ? p.scale_log2 * ks : 0.0f;
-          dst[128] = valid ? vs : 0.0f;
-          dst[256] = valid ? 0.0f : -INFINITY;
+      // Eight codes (one 16-byte f16 piece) per thread and row: sixteen threads per
+      // row read what their warp staged.
+      const auto take_codes = [&](int u, uint2 (&c)[2 * kSteps]) {
+        if (duo) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2 * kSteps; ++i) {
+          const int row = (i >> 1) * 28 + writer * 4 + (i & 1) * 2 + (lane >> 4);
+          const uint32_t at = stage + uint32_t(duo ? (u & 1) * kStageBytes : 0) + uint32_t(row * kCaD + (lane & 15) * 8);
+          c[i] = make_uint2(0u, 0u);
+          if (row < kTileRows)
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(c[i].x), "=r"(c[i].y) : "r"(at) : "memory");
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&scal_full[j % kScalarRing]));
+        issue(u + depth);
       };
-      const auto publish = [&](int u) {
+      const auto slot_of = [&](int j, int z) { return sbase + kSmemKV + uint32_t((j & 1) * 2 + z) * kTileBytes; };
+      const auto store_codes = [&](int j, int z, const uint2 (&c)[2 * kSteps]) {
+        const uint32_t slot = slot_of(j, z);
+#pragma unroll
+        for (int i = 0; i < 2 * kSteps; ++i) {
+          const int row = (i >> 1) * 28 + writer * 4 + (i & 1) * 2 + (lane >> 4);
+          if (row >= kTileRows) break;
+          const float a = factor[z * 128 + row];
+          const uint2 x = widen4(c[i].x, a), y = widen4(c[i].y, a);
+          st_shared_v4(slot + tile_offset(row, lane & 15), x.x, x.y, y.x, y.y);
+        }
+      };
+      const auto publish = [&](int j, int z) {
         fence_proxy_async_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32((u & 1) ? &v_full[(u >> 1) & 1] : &k_full[(u >> 1) & 1]));
+        if (lane == 0) mbar_arrive(smem_u32(z ? &v_full[j & 1] : &k_full[j & 1]));
       };
-      const auto wait_slot = [&](int u) {
-        const int j = u >> 1;
-        return __all_sync(0xffffffffu, mbar_wait(smem_u32((u & 1) ? &v_empty[j & 1] : &k_empty[j & 1]),
-                                                 ((j >> 1) & 1) ^ 1, err));
+      const auto wait_slot = [&](int j, int z) {
+        return __all_sync(0xffffffffu, mbar_wait(smem_u32(z ? &v_empty[j & 1] : &k_empty[j & 1]), ((j >> 1) & 1) ^ 1, err));
       };
-      uint4 cur[kSteps];
-      bool ok = true;
-      if (n > 0) load_scalars(0);
-      if (cached_n > 0) load_codes(0, cur);
-      int u = 0;
-      for (; u < 2 * cached_n && ok; ++u) {
-        uint4 next[kSteps];
-        if (u + 1 < 2 * cached_n) load_codes(u + 1, next);
-        const int j = u >> 1;
-        ok = wait_slot(u);
-        if (!ok) break;
-        store_codes(sbase + kSmemKV + uint32_t((j & 1) * 2 + (u & 1)) * kTileBytes, cur);
-        publish(u);
-        if (!(u & 1)) {
-          store_scalars(j);
-        } else if (j + 1 < n) {
-          load_scalars(j + 1);
-        }
+      // (ring slot j % 4: tile j - 4 was done before V of j - 3 left)
+      const auto store_info = [&](int j, int e, int f, const uint32_t (&bits)[4]) {
+        if (writer == 0 && lane == 0) {
+          TileInfo* info = reinterpret_cast<TileInfo*>(smem + kSmemTail + (j % kScalarRing) * kInfoBytes);
+          info->c = p.scale_log2 * pow2f(e);
+          info->f = float(f);
+          info->inv_f = pow2f(-f);
+          info->all = (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) cur[i] = next[i];
-      }
-      // fresh tiles: bf16 rows copied as they are (masked and missing rows as
-      // zeros); a tile is published one step later, when its copies have landed
-      bool pending = false;
-      for (; u < 2 * n && ok; ++u) {
-        const int j = u >> 1, k0 = (first + j - cached_tiles) * 128;
-        ok = wait_slot(u);
+          for (int i = 0; i < 4; ++i) info->valid[i] = bits[i];
+          mbar_arrive(smem_u32(&info_full[j % kScalarRing]));
+        }
+      };
+      // ---- cached tiles. Every writer warp keeps the scales of the tile's keys
+      // (keys lane + 32 i), so that no writer waits for another.
+      float ks[4], vs[4];
+      bool valid[4];
+      const auto load_scales = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = (first + j) * 128 + 32 * i + lane;
+          ks[i] = __ldg(p.ks + head_row + min(key, len - 1));
+          vs[i] = __ldg(p.vs + head_row + min(key, len - 1));
+          valid[i] = key < len && (!mask || __ldg(mask + key) != 0);
+        }
+      };
+      uint2 codes[2 * kSteps];
+      bool ok = true;
+      for (int u = 0; u < depth; ++u) issue(u);
+      if (cached_n > 0) load_scales(0);
+      int j = 0;
+      for (; j < cached_n; ++j) {
+        uint32_t mk = 0, mv = 0, bits[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          bits[i] = __ballot_sync(0xffffffffu, valid[i]);
+          if (!valid[i]) ks[i] = vs[i] = 0.0f;
+          mk = max(mk, magnitude(ks[i]));
+          mv = max(mv, magnitude(vs[i]));
+        }
+        const int e = code_exponent(__reduce_max_sync(0xffffffffu, mk), kLowK);
+        const int f = code_exponent(__reduce_max_sync(0xffffffffu, mv), kLowV);
+        store_info(j, e, f, bits);
+        __syncwarp();                        // (the previous tile's factors were read)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          factor[32 * i + lane] = ks[i] * pow2f(-e);
+          factor[128 + 32 * i + lane] = vs[i] * pow2f(-f);
+        }
+        __syncwarp();
+        if (j + 1 < cached_n) load_scales(j + 1);
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          take_codes(2 * j + z, codes);
+          ok = ok && wait_slot(j, z);
+          if (ok) {
+            store_codes(j, z, codes);
+            publish(j, z);
+          }
+        }
         if (!ok) break;
-        if (pending) {
-          cp_async_wait();
-          publish(u - 1);
-        }
-        const uint32_t slot = sbase + kSmemKV + uint32_t((j & 1) * 2 + (u & 1)) * kTileBytes;
-        const __nv_bfloat16* src = (u & 1) ? p.v + b * p.v_sb + kvh * p.v_sh : p.k + b * p.k_sb + kvh * p.k_sh;
-        const int64_t ss = (u & 1) ? p.v_ss : p.k_ss;
-        for (int row = t >> 4; row < kTileRows; row += 14) {
-          const int piece = t & 15, key = k0 + row;
-          const bool held = key < p.sk && (!mask || __ldg(mask + p.extent + key) != 0);
-          cp_async16_zfill(slot + tile_offset(row, piece), src + int64_t(held ? key : 0) * ss + piece * 8, held);
-        }
-        pending = true;
-        if (!(u & 1)) {
-          store_scalars(j);
-          if (j + 1 < n) load_scalars(j + 1);
-        }
       }
-      cp_async_wait();
-      if (pending && ok) publish(u - 1);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      // ---- fresh tiles: the exponents come from the rows themselves (sixteen
+      // threads per row, 14 rows per step)
+      constexpr int kFresh = 10;
+      uint32_t* slots = reinterpret_cast<uint32_t*>(smem + kSmemSlots);
+      for (; j < n && ok; ++j) {
+        const int k0 = (first + j - cached_tiles) * 128, piece = t & 15;
+        uint32_t bits[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = k0 + 32 * i + lane;
+          bits[i] = __ballot_sync(0xffffffffu, key < p.sk && (!mask || __ldg(mask + p.extent + key) != 0));
+        }
+        const auto load_rows = [&](int z, uint4 (&c)[kFresh]) {
+          const __nv_bfloat16* src = z ? p.v + b * p.v_sb + kvh * p.v_sh : p.k + b * p.k_sb + kvh * p.k_sh;
+          const int64_t ss = z ? p.v_ss : p.k_ss;
+#pragma unroll
+          for (int i = 0; i < kFresh; ++i) {
+            const int row = i * 14 + (t >> 4);
+            const uint32_t word = row < 32 ? bits[0] : row < 64 ? bits[1] : row < 96 ? bits[2] : bits[3];
+            c[i] = row < kTileRows && ((word >> (row & 31)) & 1)
+                       ? __ldg(reinterpret_cast<const uint4*>(src + int64_t(k0 + row) * ss) + piece)
+                       : make_uint4(0u, 0u, 0u, 0u);
+          }
+        };
+        const auto exponent = [&](const uint4 (&c)[kFresh], int lo) {
+          uint32_t m = 0;
+#pragma unroll
+          for (int i = 0; i < kFresh; ++i) m = finite_max8(c[i], m);
+          m = __reduce_max_sync(0xffffffffu, m);
+          asm volatile("bar.sync 1, 224;" ::: "memory");      // (the slots' last readers are done)
+          if (lane == 0) slots[writer] = m;
+          asm volatile("bar.sync 1, 224;" ::: "memory");
+#pragma unroll
+          for (int i = 0; i < kWriters; ++i) m = max(m, slots[i]);
+          return tile_exponent(m, lo);
+        };
+        const auto store_rows = [&](int z, const uint4 (&c)[kFresh], float a) {
+          const uint32_t slot = slot_of(j, z);
+#pragma unroll
+          for (int i = 0; i < kFresh; ++i) {
+            const int row = i * 14 + (t >> 4);
+            const uint4 h = narrow8(c[i], a);
+            if (row < kTileRows) st_shared_v4(slot + tile_offset(row, piece), h.x, h.y, h.z, h.w);
+          }
+        };
+        uint4 c[kFresh];
+        load_rows(1, c);
+        const int f = exponent(c, kLowV);
+        load_rows(0, c);
+        const int e = exponent(c, kLowK);
+        store_info(j, e, f, bits);
+        // (a warp whose wait gives up leaves the others: their named barriers do
+        // not depend on it beyond this tile's, which it has passed)
+        ok = wait_slot(j, 0);
+        if (ok) {
+          store_rows(0, c, pow2f(-e));
+          publish(j, 0);
+          load_rows(1, c);
+          ok = wait_slot(j, 1);
+        }
+        if (ok) {
+          store_rows(1, c, pow2f(-f));
+          publish(j, 1);
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      for (; j < n; ++j)    // the barriers of tiles that were given up
+        if (j >= cached_n)
+          for (int i = 0; i < 4; ++i) asm volatile("bar.sync 1, 224;" ::: "memory");
     }
   } else {
     // ----------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    const int w = warp >> 2;
+    const int w = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + t_lane + uint32_t(128 * w), t_o = tmem + t_lane + uint32_t(256 + 128 * w);
-    const float c = p.scale_log2;
-    const int count = tiles_of(w);
+    const int q_tile = duo ? 0 : w;
+    float* scale = reinterpret_cast<float*>(smem + kSmemQScale) + q_tile * kTileRows;
+    if (w == q_tile)
+      load_queries(p, tp, sbase + kSmemQ + w * kTileBytes, scale, 2 * pair + w, threadIdx.x & 127, kvh, b, q_full);
+    asm volatile("bar.sync 2, 256;" ::: "memory");       // (the rows' scales)
+    const float q_up = scale[row];
+    const int count = duo ? (n - w + 1) / 2 : n;       // key tiles of this group
     bool ok = true;
-    float m = -INFINITY;
-    uint64_t l2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+    RowState st = {-INFINITY, 0.0f};
     for (int it = 0; it < count; ++it) {
       const int j = duo ? 2 * it + w : it;
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[w]), it & 1, err) &&
-                                       mbar_wait(smem_u32(&scal_full[j % kScalarRing]), (j / kScalarRing) & 1, err));
+                                       mbar_wait(smem_u32(&info_full[j % kScalarRing]), (j / kScalarRing) & 1, err));
       if (!ok) break;
       tc_fence_after();
-      uint32_t s[128];
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        tc_ld_32x32b_x32(t_s + uint32_t(q * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[q * 32]));
-      const float* scal = reinterpret_cast<const float*>(smem + kSmemTail + (j % kScalarRing) * kScalarBytes);
-      const int tile = first + j, tail = tile < cached_tiles ? len - tile * 128 : p.sk - (tile - cached_tiles) * 128;
-      const int kind = p.key_valid || tail < 128 ? kMasked : tile < cached_tiles ? kCachedFull : kFreshFull;
-      tc_wait_ld();
-      const float top = kind == kFreshFull    ? row_scores<kFreshFull>(s, scal, c)
-                        : kind == kCachedFull ? row_scores<kCachedFull>(s, scal, c)
-                                              : row_scores<kMasked>(s, scal, c);
-      const bool grow = top > m + kTilesLag;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float f = grow ? ex2_ftz(m - top) : 1.0f;   // (m = -inf: 0)
-        if (grow) m = top;
-        l2[0] = f2_mul(l2[0], f2_pack(f, f));
-        l2[1] = f2_mul(l2[1], f2_pack(f, f));
-        if (it > 0) {
-#pragma unroll 1
-          for (int q = 0; q < 8; ++q) {
-            uint32_t o[16];
-            tc_ld_32x32b_x16(t_o + uint32_t(q * 16), o);
-            tc_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tc_st_32x32b_x16(t_o + uint32_t(q * 16), o);
-          }
-        }
-      }
-      const float neg_m = m == -INFINITY ? 0.0f : -m;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t x[32];
-        if (kind == kFreshFull) row_weights<kFreshFull>(s, h, scal, c, neg_m, l2, x);
-        else row_weights<kCachedFull>(s, h, scal, c, neg_m, l2, x);
-        tc_st_32x32b_x32(t_s + uint32_t(32 * h), x);
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&p_full[2 * w + h]));
-      }
+      softmax_tile(t_s, t_o, reinterpret_cast<const TileInfo*>(smem + kSmemTail + (j % kScalarRing) * kInfoBytes), q_up,
+                   it == 0, st, &p_full[2 * w], lane);
     }
-    float la, lb;
-    f2_unpack(f2_add(l2[0], l2[1]), la, lb);
-    const float l = la + lb;
     bool have = ok && count > 0;       // the accumulators hold something
     if (ok && n > 0) have = __all_sync(0xffffffffu, mbar_wait(smem_u32(o_full), 0, err)) && have;
     tc_fence_after();
-    // ------------------------------------------------------------------ output
-    const int row = (warp & 3) * 32 + lane;
     const int token = (2 * pair + w) * tp.tokens_per_tile + row / p.share;
     if (splits == 1 && !duo)
-      store_row(t_o, have, l, row < tile_rows && token < p.sq,
+      store_row(t_o, have, st.l, row < tp.tokens_per_tile * p.share && token < p.sq,
                 p.out + b * p.o_sb + int64_t(token) * p.o_ss + int64_t(kvh * p.share + row % p.share) * p.o_sh);
     else
-      stage_row(t_o, have, m, l, sbase, reinterpret_cast<float*>(smem + kSmemML), w * kTileRows + row);
+      stage_row(t_o, have, st.m, st.l, sbase, reinterpret_cast<float*>(smem + kSmemML), w * kTileRows + row);
   }
   tc_fence_before();
   __syncthreads();

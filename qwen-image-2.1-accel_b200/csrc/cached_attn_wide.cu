@@ -3,20 +3,8 @@
 // of 256 query rows streams them by TMA.
 //
 // cached_widen_kernel writes, per (request, K/V head), the cached and the fresh
-// keys as f16 rows, each tile of 128 keys scaled by powers of two of its own:
-//   kw_j = ks_j kc_j 2^-e,  vw_j = vs_j vc_j 2^-f     (masked keys: zeros)
-// with the tile's largest |ks|, |vs| just inside 2^14. f16 keeps eleven bits down
-// to 2^-28 of that, an eighth of bf16's rounding, and no factor is left per key:
-// with x = q_i . kw_j (q_i scaled by a power of two per row),
-//   t_ij = x c_i + f,  c_i = c log2e 2^(e + e_i)        log2 of the weight of vw_j
-//   w_ij = 2^(t_ij - M_i + 8)
-//   o_i  = sum_j w_ij vw_j / sum_tiles 2^-f sum_j w_ij
-// so a score costs half a maximum, half a multiply-add, one exponential, half an
-// addition and half a conversion, and the softmax reads 32 bytes per tile. (With
-// the scales as per-key numbers in shared memory it took 5700 cycles a step of
-// 256 x 128 scores instead of 4200: the broadcast reads compete with the MMA
-// operands.) The widening moves 3 bytes per code, once, instead of converting
-// them again in every CTA.
+// keys as the f16 rows of cached_attn_tc.cuh and their tiles' numbers. It moves 3
+// bytes per code, once, instead of converting the codes again in every CTA.
 //
 // Roles (384 threads, one CTA per SM): warps 0-3 and 4-7 softmax of the two query
 // tiles (a row per thread), warp 8 issues the MMAs, warp 9 the TMA loads. TMEM:
@@ -31,62 +19,24 @@
 //
 // What bounds it: per key tile 4 x 512 tensor cycles and 2 x 1024 cycles of
 // exponentials per SM.
-#include <cuda_fp16.h>
-
 #include "cached_attn_tc.cuh"
 
 namespace qia {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kInfoBytes = 32;
 constexpr int kSmemQScale = kSmemTail + kScalarRing * kInfoBytes;   // 2^e_i of 256 rows
 constexpr int kSmemML = kSmemQScale + 256 * 4;                      // m, l of 256 rows (joining)
 constexpr int kSmemBars = kSmemML + 2 * 256 * 4;
 constexpr int kSmemBytes = kSmemBars + 256 + 1024;
 // registers of a softmax thread and of any other: 256 x 208 + 128 x 88 = 384 x 168, what the block starts with
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
-constexpr float kBias = 8.0f, kLag = 7.0f;
-constexpr uint32_t kIdescS = (1u << 4) | (uint32_t(128 >> 3) << 17) | (uint32_t(128 >> 4) << 24);   // f16 x f16 -> f32
-constexpr uint32_t kIdescO = kIdescS | (1u << 16);   // B (V) is MN-major
-
-// A tile of 128 keys: the softmax's numbers and which keys take part.
-struct __align__(16) TileInfo {
-  float c, f, inv_f;     // c log2e 2^e, f, 2^-f
-  uint32_t all;          // every key takes part
-  uint32_t valid[4];
-};
-static_assert(sizeof(TileInfo) == kInfoBytes, "bulk copy size");
-
 struct Widened {
   __half* k;             // [B Hkv, tiles * 128, 128]: cached_cap cached tiles, then the fresh ones
   __half* v;
   TileInfo* info;        // [B Hkv, tiles]
   int cached_cap, tiles;
 };
-
-__device__ __forceinline__ uint32_t cvt_f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
-// Four codes (a word of INT8) times a -> four f16: byte u = code + 128 under
-// 0x4B0000 is the float 2^23 + u.
-__device__ __forceinline__ uint2 widen4(uint32_t w, float a) {
-  const uint32_t u = w ^ 0x80808080u;
-  const uint64_t off = f2_pack(-8388736.0f, -8388736.0f), a2 = f2_pack(a, a);
-  float x[4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint64_t t = f2_pack(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + 2 * i)),
-                               __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7541 + 2 * i)));
-    f2_unpack(f2_mul(f2_add(t, off), a2), x[2 * i], x[2 * i + 1]);
-  }
-  return make_uint2(cvt_f16x2(x[0], x[1]), cvt_f16x2(x[2], x[3]));
-}
-
-__device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
 
 // Maximum of |x| over the block as bits (NaN and infinity above every number); 256 threads.
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* slots) {
@@ -97,14 +47,6 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* slots) {
 #pragma unroll
   for (int i = 1; i < 8; ++i) m = max(m, slots[i]);
   return m;
-}
-
-// Exponent e with max 2^-e in [2^13, 2^14) for a maximum given as bits; kept in
-// a range where c 2^(e + e_i) and 2^+-f stay normal (rows beyond it only lose
-// bits: below 2^-44 they no longer matter to a score, above they saturate f16
-// to infinity at 2^106).
-__device__ __forceinline__ int tile_exponent(uint32_t bits, int lo) {
-  return min(max(int(bits >> 23) - 127 - 13, lo), 90);
 }
 
 // One CTA per (tile, K/V head, request).
@@ -143,11 +85,10 @@ __global__ void __launch_bounds__(256) cached_widen_kernel(const __grid_constant
     const float s = key < end ? __ldg((t < 128 ? p.ks : p.vs) + head_row + key) : 0.0f;
     __syncthreads();
     const float mine = (valid_bits[(t & 127) >> 5] >> (t & 31)) & 1 ? s : 0.0f;
-    // (a NaN scale takes no part in the maximum)
-    const uint32_t mag = mine == mine ? __float_as_uint(fabsf(mine)) : 0u;
+    const uint32_t mag = magnitude(mine);
     const uint32_t mk = block_max(t < 128 ? mag : 0u, slots[0]), mv = block_max(t < 128 ? 0u : mag, slots[1]);
-    e[0] = tile_exponent(mk + (7u << 23), -30);     // (|code| < 2^7)
-    e[1] = tile_exponent(mv + (7u << 23), -90);
+    e[0] = code_exponent(mk, kLowK);
+    e[1] = code_exponent(mv, kLowV);
     factor[t >> 7][t & 127] = mine * pow2f(-e[t >> 7]);
     __syncthreads();
 #pragma unroll
@@ -177,24 +118,13 @@ __global__ void __launch_bounds__(256) cached_widen_kernel(const __grid_constant
                    : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t x[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t lo = (x[q] << 16) & 0x7fffffffu, hi = x[q] & 0x7fff0000u;
-          m = max(m, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));   // finite values
-        }
-      }
-      e[z] = tile_exponent(block_max(m, slots[z]), z ? -90 : -30);
+      for (int i = 0; i < 8; ++i) m = finite_max8(c[i], m);
+      e[z] = tile_exponent(block_max(m, slots[z]), z ? kLowV : kLowK);
       const float a = pow2f(-e[z]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int row = i * 16 + (t >> 4);
-        float f[8];
-        unpack8(c[i], f);
-        reinterpret_cast<uint4*>((z ? w.v : w.k) + (out_row + row) * kCaD)[t & 15] =
-            make_uint4(cvt_f16x2(f[0] * a, f[1] * a), cvt_f16x2(f[2] * a, f[3] * a), cvt_f16x2(f[4] * a, f[5] * a),
-                       cvt_f16x2(f[6] * a, f[7] * a));
+        reinterpret_cast<uint4*>((z ? w.v : w.k) + (out_row + row) * kCaD)[t & 15] = narrow8(c[i], a);
       }
     }
   }
@@ -227,7 +157,8 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
   uint64_t* p_full = bars + 14;       // [2][2] weights of query tile i, half h, stored
   uint64_t* o_full = bars + 18;
   uint64_t* drain = bars + 19;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t* q_full = bars + 20;       // softmax -> issuer
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = int(cluster_size()), split = int(cluster_rank());
@@ -246,35 +177,12 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
     for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&p_full[i]), 4);
     mbar_init(smem_u32(o_full), 1);
     mbar_init(smem_u32(drain), 1);
+    mbar_init(smem_u32(q_full), 4 * n_tiles);
     fence_barrier_init();
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
   }
   if (warp == 8) tmem_alloc(smem_u32(tmem_slot), 512);
-  // ---- query rows as f16, scaled by a power of two each (sixteen threads per
-  // row; rows past the end are zeros)
-  const int tile_rows = tp.tokens_per_tile * p.share;
-  for (int i = threadIdx.x; i < n_tiles * kTileRows * 16; i += kThreads) {
-    const int tile = i >> 11, row = (i >> 4) & 127, piece = i & 15;
-    const int token = (2 * pair + tile) * tp.tokens_per_tile + row / p.share;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (row < tile_rows && token < p.sq)
-      v = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_sb + int64_t(token) * p.q_ss +
-                                               int64_t(kvh * p.share + row % p.share) * p.q_sh) + piece);
-    float f[8];
-    unpack8(v, f);
-    uint32_t mx = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(f[e]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const int e = min(max(int(mx >> 23) - 127, -80), 120);
-    const float inv = pow2f(-e);
-    if (piece == 0) reinterpret_cast<float*>(smem + kSmemQScale)[tile * kTileRows + row] = pow2f(e);
-    st_shared_v4(sbase + kSmemQ + tile * kTileBytes + tile_offset(row, piece), cvt_f16x2(f[0] * inv, f[1] * inv),
-                 cvt_f16x2(f[2] * inv, f[3] * inv), cvt_f16x2(f[4] * inv, f[5] * inv), cvt_f16x2(f[6] * inv, f[7] * inv));
-  }
-  fence_proxy_async_shared();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -321,7 +229,7 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
         const auto commit = [&](uint64_t* bar) {
           if (lead) tc_commit(smem_u32(bar));
         };
-        bool ok = wait(&k_full[0], 0);
+        bool ok = wait(q_full, 0) && wait(&k_full[0], 0);
         if (ok) {
           for (int i = 0; i < n_tiles; ++i) qk(i, 0);
           commit(&k_empty[0]);
@@ -388,92 +296,30 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
     const int w = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = uint32_t((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + t_lane + uint32_t(128 * w), t_o = tmem + t_lane + uint32_t(256 + 128 * w);
-    const float q_up = reinterpret_cast<const float*>(smem + kSmemQScale)[w < n_tiles ? w * kTileRows + row : 0];
+    float* scale = reinterpret_cast<float*>(smem + kSmemQScale) + w * kTileRows;
+    if (w < n_tiles)
+      load_queries(p, tp, sbase + kSmemQ + w * kTileBytes, scale, 2 * pair + w, threadIdx.x & 127, kvh, b, q_full);
     bool ok = w < n_tiles;
-    float m = -INFINITY, l = 0.0f;
+    if (ok) asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");   // (the rows' scales)
+    const float q_up = scale[row];
+    RowState st = {-INFINITY, 0.0f};
     for (int j = 0; j < n && ok; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[w]), j & 1, err) &&
                                        mbar_wait(smem_u32(&info_full[j % kScalarRing]), (j / kScalarRing) & 1, err));
       if (!ok) break;
       tc_fence_after();
-      uint32_t s[128];
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        tc_ld_32x32b_x32(t_s + uint32_t(q * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[q * 32]));
-      const TileInfo* info = reinterpret_cast<const TileInfo*>(smem + kSmemTail + (j % kScalarRing) * kInfoBytes);
-      const float4 num = *reinterpret_cast<const float4*>(info);
-      const float c = num.x * q_up, f = num.y;
-      tc_wait_ld();
-      if (!__float_as_uint(num.w)) {         // some keys take no part
-        const uint4 bits = *reinterpret_cast<const uint4*>(info->valid);
-        const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
-#pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (!((word[i >> 5] >> (i & 31)) & 1)) s[i] = 0xff800000u;
-      }
-      float mx[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s[i]);
-#pragma unroll
-      for (int i = 4; i < 124; i += 8)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mx[k] = max3(mx[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        mx[k] = max3(mx[k], __uint_as_float(s[124 + 2 * k]), __uint_as_float(s[125 + 2 * k]));
-      const float top = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), c, f);
-      const bool grow = top > m + kLag;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float r = grow ? ex2_ftz(m - top) : 1.0f;   // (m = -inf: 0)
-        if (grow) m = top;
-        l *= r;
-        if (j > 0) {
-#pragma unroll 1
-          for (int q = 0; q < 8; ++q) {
-            uint32_t o[16];
-            tc_ld_32x32b_x16(t_o + uint32_t(q * 16), o);
-            tc_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * r);
-            tc_st_32x32b_x16(t_o + uint32_t(q * 16), o);
-          }
-        }
-      }
-      const float n1 = f + kBias - (m == -INFINITY ? 0.0f : m);
-      const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(n1, n1);
-      uint64_t sum[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t x[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float a, b2;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[64 * h + 2 * i]), __uint_as_float(s[64 * h + 2 * i + 1])), c2, n2), a, b2);
-          a = ex2_ftz(a);
-          b2 = ex2_ftz(b2);
-          sum[i & 1] = f2_add(sum[i & 1], f2_pack(a, b2));
-          x[i] = cvt_f16x2(a, b2);
-        }
-        tc_st_32x32b_x32(t_s + uint32_t(32 * h), x);
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&p_full[2 * w + h]));
-      }
-      float a, b2;
-      f2_unpack(f2_add(sum[0], sum[1]), a, b2);
-      l = fmaf(a + b2, num.z, l);
+      softmax_tile(t_s, t_o, reinterpret_cast<const TileInfo*>(smem + kSmemTail + (j % kScalarRing) * kInfoBytes), q_up,
+                   j == 0, st, &p_full[2 * w], lane);
     }
     const bool have = ok && n > 0 && __all_sync(0xffffffffu, mbar_wait(smem_u32(o_full), 0, err));
     tc_fence_after();
     if (w < n_tiles) {
       const int token = (2 * pair + w) * tp.tokens_per_tile + row / p.share;
       if (splits == 1)
-        store_row(t_o, have, l, row < tile_rows && token < p.sq,
+        store_row(t_o, have, st.l, row < tp.tokens_per_tile * p.share && token < p.sq,
                   p.out + b * p.o_sb + int64_t(token) * p.o_ss + int64_t(kvh * p.share + row % p.share) * p.o_sh);
       else
-        stage_row(t_o, have, m, l, sbase, reinterpret_cast<float*>(smem + kSmemML), w * kTileRows + row);
+        stage_row(t_o, have, st.m, st.l, sbase, reinterpret_cast<float*>(smem + kSmemML), w * kTileRows + row);
     }
   }
   tc_fence_before();
