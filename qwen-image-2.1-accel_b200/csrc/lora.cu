@@ -260,16 +260,20 @@ int launch_tokens(const Lora& p, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ many tokens
-constexpr int kShrinkStages = 5;
 constexpr int kShrinkX = 128 * 64 * 2;    // x tile of a stage: 128 tokens x 64 channels
 
 __host__ __device__ constexpr int shrink_rank(int r_pad) { return (r_pad + 15) / 16 * 16; }   // N of the product
 __host__ __device__ constexpr int shrink_stage(int r_pad) { return kShrinkX + shrink_rank(r_pad) * 128; }
 __host__ __device__ constexpr int shrink_sums(int r_pad) { return 128 * (shrink_rank(r_pad) + 4) * 4; }
-__host__ __device__ constexpr int shrink_smem(int r_pad) {
-  return kShrinkStages * ((shrink_stage(r_pad) + 1023) / 1024 * 1024) + 256 + 1024;
+// Stages of a CTA: two CTAs per SM.
+__host__ __device__ constexpr int shrink_stages(int r_pad) {
+  return 110 * 1024 / shrink_stage(r_pad) < 6 ? 110 * 1024 / shrink_stage(r_pad) : 6;
 }
-static_assert(shrink_sums(kLoraMaxRank) <= kShrinkStages * kShrinkX, "the sums reuse the stages");
+__host__ __device__ constexpr int shrink_smem(int r_pad) { return shrink_stages(r_pad) * shrink_stage(r_pad) + 256 + 1024; }
+static_assert(shrink_sums(kLoraMaxRank) <= shrink_stages(kLoraMaxRank) * shrink_stage(kLoraMaxRank) &&
+                  shrink_sums(64) <= shrink_stages(64) * shrink_stage(64),
+              "the sums reuse the stages");
+static_assert(shrink_stage(8) % 1024 == 0 && shrink_stage(kLoraMaxRank) % 1024 == 0, "swizzled tiles are 1 KB aligned");
 
 constexpr uint32_t idesc_bf16(int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
@@ -282,10 +286,10 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                    const __grid_constant__ Lora p, __nv_bfloat16* t, int* err) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int n = shrink_rank(p.r_pad), stage_bytes = (shrink_stage(p.r_pad) + 1023) / 1024 * 1024;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kShrinkStages * stage_bytes);
-  uint64_t* empty = full + kShrinkStages;
-  uint64_t* acc_full = empty + kShrinkStages;
+  const int n = shrink_rank(p.r_pad), stage_bytes = shrink_stage(p.r_pad), stages = shrink_stages(p.r_pad);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + stages * stage_bytes);
+  uint64_t* empty = full + stages;
+  uint64_t* acc_full = empty + stages;
   uint64_t* drain = acc_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -298,7 +302,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
   const int first = min(blocks, split * per), count = min(blocks, first + per) - first;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kShrinkStages; ++i) {
+    for (int i = 0; i < stages; ++i) {
       mbar_init(smem_u32(&full[i]), 1);
       mbar_init(smem_u32(&empty[i]), 1);
     }
@@ -313,35 +317,38 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
   const uint32_t tmem = *tmem_slot;
   if (warp == 4) {
     if (lane == 0) {
-      int issued = 0;
+      int st = 0, issued = 0;
+      uint32_t phase = 0;
       bool ok = true;
       for (int i = 0; i < count; ++i) {
-        const int st = i % kShrinkStages;
-        if (!mbar_wait(smem_u32(&empty[st]), ((i / kShrinkStages) & 1) ^ 1, err)) { ok = false; break; }
+        if (!mbar_wait(smem_u32(&empty[st]), phase ^ 1, err)) { ok = false; break; }
         const uint32_t dst = smem_u32(smem + st * stage_bytes), bar = smem_u32(&full[st]);
         mbar_arrive_expect_tx(bar, uint32_t(kShrinkX + n * 128));
         tma_load_3d(dst, &tm_x, bar, (first + i) * 64, s0, b);
         tma_load_3d(dst + kShrinkX, &tm_a, bar, (first + i) * 64, 0, id);
-        issued = i + 1;
+        ++issued;
+        if (++st == stages) { st = 0; phase ^= 1; }
       }
       if (!ok)   // let queued copies land before the shared memory is released
-        for (int i = max(0, issued - kShrinkStages); i < issued; ++i)
-          mbar_wait(smem_u32(&full[i % kShrinkStages]), (i / kShrinkStages) & 1, nullptr, 100000000ull);
+        for (int i = max(0, issued - stages); i < issued; ++i)
+          mbar_wait(smem_u32(&full[i % stages]), (i / stages) & 1, nullptr, 100000000ull);
     }
     __syncwarp();
   } else if (warp == 5) {
     if (lane == 0) {
       bool ok = true;
+      int st = 0;
+      uint32_t phase = 0;
       const uint32_t idesc = idesc_bf16(0) | (uint32_t(n >> 3) << 17);
       for (int i = 0; i < count; ++i) {
-        const int st = i % kShrinkStages;
-        if (!mbar_wait(smem_u32(&full[st]), (i / kShrinkStages) & 1, err)) { ok = false; break; }
+        if (!mbar_wait(smem_u32(&full[st]), phase, err)) { ok = false; break; }
         tc_fence_after();
         const uint64_t xd = smem_desc_k_sw128(smem_u32(smem + st * stage_bytes));
         const uint64_t ad = smem_desc_k_sw128(smem_u32(smem + st * stage_bytes + kShrinkX));
 #pragma unroll
         for (int k = 0; k < 4; ++k) tc_mma_f16_ss(tmem, xd + uint64_t(2 * k), ad + uint64_t(2 * k), idesc, (i | k) != 0);
         tc_commit(smem_u32(&empty[st]));
+        if (++st == stages) { st = 0; phase ^= 1; }
       }
       if (ok) tc_commit(smem_u32(acc_full));
       tc_commit(smem_u32(drain));
@@ -540,7 +547,7 @@ int make_map(CUtensorMap* map, const void* base, int64_t d0, int64_t d1, int64_t
 int launch_tiles(const Lora& p, void* workspace, cudaStream_t st) {
   static const bool ready =
       cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           shrink_smem(kLoraMaxRank)) == cudaSuccess &&
+                           112 * 1024) == cudaSuccess &&
       cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
       cudaFuncSetAttribute(lora_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            expand_smem(kLoraMaxRank)) == cudaSuccess;
