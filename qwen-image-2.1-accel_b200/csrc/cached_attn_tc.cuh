@@ -120,10 +120,16 @@ __device__ __forceinline__ uint32_t finite_max8(const uint4& v, uint32_t m) {
 }
 
 __device__ __forceinline__ uint4 narrow8(const uint4& v, float a) {   // eight bf16 values times a -> f16
-  float f[8];
-  unpack8(v, f);
-  return make_uint4(cvt_f16x2(f[0] * a, f[1] * a), cvt_f16x2(f[2] * a, f[3] * a), cvt_f16x2(f[4] * a, f[5] * a),
-                    cvt_f16x2(f[6] * a, f[7] * a));
+  const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+  const uint64_t a2 = f2_pack(a, a);
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    f2_unpack(f2_mul(f2_pack(bf16_lo(x[i]), bf16_hi(x[i])), a2), lo, hi);
+    h[i] = cvt_f16x2(lo, hi);
+  }
+  return make_uint4(h[0], h[1], h[2], h[3]);
 }
 
 // Query tiles and groups: a tile is 128 / share tokens of all heads that share a
@@ -145,39 +151,34 @@ inline TileGrid tile_grid(const CachedAttn& p) {
 }
 
 // A query tile into shared memory as f16, each row scaled by a power of two 2^e_i
-// (rows past the end are zeros), by the 128 threads of a softmax group (`t`; eight
-// rows per step, sixteen threads per row); 2^e_i into scale[128]. Announced on
-// q_full (four arrivals per tile).
+// (rows past the end are zeros), by THREADS threads (`t`; sixteen per row, every
+// load of a thread in flight at once); 2^e_i into scale[128]. Announced on q_full
+// by every warp.
+template <int THREADS>
 __device__ __forceinline__ void load_queries(const CachedAttn& p, const TileGrid& g, uint32_t slot, float* scale, int tile,
                                              int t, int kvh, int b, uint64_t* q_full) {
+  constexpr int kRows = THREADS / 16, kLoads = kTileRows / kRows;
   const int tile_rows = g.tokens_per_tile * p.share, piece = t & 15;
-#pragma unroll 1
-  for (int half = 0; half < 2; ++half) {
-    uint4 v[8];
+  const __nv_bfloat16* src = p.q + b * p.q_sb + int64_t(kvh * p.share) * p.q_sh + 8 * piece;
+  uint4 v[kLoads];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = half * 64 + i * 8 + (t >> 4), part = int((uint32_t(row) * g.share_inv) >> 16);
-      const int token = tile * g.tokens_per_tile + part;
-      v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (row < tile_rows && token < p.sq)
-        v[i] = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_sb + int64_t(token) * p.q_ss +
-                                                    int64_t(kvh * p.share + row - part * p.share) * p.q_sh) + piece);
-    }
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = i * kRows + (t >> 4), part = int((uint32_t(row) * g.share_inv) >> 16);
+    const int token = tile * g.tokens_per_tile + part;
+    v[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (row < tile_rows && token < p.sq)
+      v[i] = __ldg(reinterpret_cast<const uint4*>(src + int64_t(token) * p.q_ss + int64_t(row - part * p.share) * p.q_sh));
+  }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = half * 64 + i * 8 + (t >> 4);
-      float f[8];
-      unpack8(v[i], f);
-      uint32_t mx = 0;
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = i * kRows + (t >> 4);
+    uint32_t m = __vmaxu2(__vmaxu2(abs_bf16x2(v[i].x), abs_bf16x2(v[i].y)), __vmaxu2(abs_bf16x2(v[i].z), abs_bf16x2(v[i].w)));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(f[e]) & 0x7fffffffu);
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const int e = min(max(int(mx >> 23) - 127, -80), 120);
-      if (piece == 0) scale[row] = pow2f(e);
-      const uint4 h = narrow8(v[i], pow2f(-e));
-      st_shared_v4(slot + tile_offset(row, piece), h.x, h.y, h.z, h.w);
-    }
+    for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const int e = min(max(int(max(m & 0xffffu, m >> 16) >> 7) - 127, -80), 120);
+    if (piece == 0) scale[row] = pow2f(e);
+    const uint4 h = narrow8(v[i], pow2f(-e));
+    st_shared_v4(slot + tile_offset(row, piece), h.x, h.y, h.z, h.w);
   }
   fence_proxy_async_shared();
   __syncwarp();

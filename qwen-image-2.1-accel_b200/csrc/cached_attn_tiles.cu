@@ -89,7 +89,7 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
     for (int i = 0; i < kScalarRing; ++i) mbar_init(smem_u32(&info_full[i]), 1);
     mbar_init(smem_u32(o_full), 1);
     mbar_init(smem_u32(drain), 1);
-    mbar_init(smem_u32(q_full), 4 * n_tiles);
+    mbar_init(smem_u32(q_full), 8);
     fence_barrier_init();
   }
   if (warp == 8) tmem_alloc(smem_u32(tmem_slot), 512);
@@ -394,8 +394,8 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
     const uint32_t t_s = tmem + t_lane + uint32_t(128 * w), t_o = tmem + t_lane + uint32_t(256 + 128 * w);
     const int q_tile = duo ? 0 : w;
     float* scale = reinterpret_cast<float*>(smem + kSmemQScale) + q_tile * kTileRows;
-    if (w == q_tile)
-      load_queries(p, tp, sbase + kSmemQ + w * kTileBytes, scale, 2 * pair + w, threadIdx.x & 127, kvh, b, q_full);
+    if (duo) load_queries<256>(p, tp, sbase + kSmemQ, scale, 2 * pair, threadIdx.x, kvh, b, q_full);
+    else load_queries<128>(p, tp, sbase + kSmemQ + w * kTileBytes, scale, 2 * pair + w, threadIdx.x & 127, kvh, b, q_full);
     asm volatile("bar.sync 2, 256;" ::: "memory");       // (the rows' scales)
     const float q_up = scale[row];
     const int count = duo ? (n - w + 1) / 2 : n;       // key tiles of this group

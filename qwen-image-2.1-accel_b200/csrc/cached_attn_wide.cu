@@ -50,7 +50,7 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* slots) {
 }
 
 // One CTA per (tile, K/V head, request).
-__global__ void __launch_bounds__(256) cached_widen_kernel(const __grid_constant__ CachedAttn p,
+__global__ void __launch_bounds__(256, 3) cached_widen_kernel(const __grid_constant__ CachedAttn p,
                                                            const __grid_constant__ Widened w) {
   __shared__ float factor[2][128];
   __shared__ uint32_t slots[2][8], valid_bits[4];
@@ -298,7 +298,7 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
     const uint32_t t_s = tmem + t_lane + uint32_t(128 * w), t_o = tmem + t_lane + uint32_t(256 + 128 * w);
     float* scale = reinterpret_cast<float*>(smem + kSmemQScale) + w * kTileRows;
     if (w < n_tiles)
-      load_queries(p, tp, sbase + kSmemQ + w * kTileBytes, scale, 2 * pair + w, threadIdx.x & 127, kvh, b, q_full);
+      load_queries<128>(p, tp, sbase + kSmemQ + w * kTileBytes, scale, 2 * pair + w, threadIdx.x & 127, kvh, b, q_full);
     bool ok = w < n_tiles;
     if (ok) asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");   // (the rows' scales)
     const float q_up = scale[row];
