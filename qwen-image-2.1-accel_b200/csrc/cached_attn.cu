@@ -530,9 +530,9 @@ struct RowsPlan {
 template <int NT, int DEPTH>
 int plan_rows(int64_t groups, int steps, RowsPlan* plan) {
   constexpr int smem = int(sizeof(RowsSmem<8 * NT, DEPTH>));
-  static const bool ready = cudaFuncSetAttribute(cached_attn_rows_kernel<NT, DEPTH>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess;
-  if (!ready) return set_error(QIA_ERR_CUDA, "qia_cached_attention: cudaFuncSetAttribute failed");
+  static std::atomic<uint64_t> allowed;
+  const int rc = allow_launch("qia_cached_attention", cached_attn_rows_kernel<NT, DEPTH>, smem, &allowed);
+  if (rc) return rc;
   static std::atomic<int> resident[17];
   *plan = {INT64_MAX, 1};
   for (int s = 1; s <= 8 && (s == 1 || s <= steps); ++s) {

@@ -433,9 +433,9 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
 }  // namespace
 
 int launch_cached_tiles(const CachedAttn& p, int batch, cudaStream_t st) {
-  static const bool ready = cudaFuncSetAttribute(cached_attn_tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 kSmemBytes) == cudaSuccess;
-  if (!ready) return set_error(QIA_ERR_CUDA, "qia_cached_attention: cudaFuncSetAttribute failed");
+  static std::atomic<uint64_t> allowed;
+  const int rc = allow_launch("qia_cached_attention", cached_attn_tiles_kernel, kSmemBytes, &allowed);
+  if (rc) return rc;
   TileGrid g = tile_grid(p);
   const int64_t groups = int64_t(g.pairs) * p.kv_heads * batch;
   if (groups > 0x0fffffff) return set_error(QIA_ERR_UNSUPPORTED, "qia_cached_attention: too many query rows");

@@ -374,9 +374,9 @@ int64_t cached_wide_workspace(int64_t batch, int64_t seq_k, int64_t kv_heads, in
 
 int launch_cached_wide(const CachedAttn& p, int batch, void* workspace, cudaStream_t st) {
   const char* who = "qia_cached_attention";
-  static const bool ready = cudaFuncSetAttribute(cached_attn_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 kSmemBytes) == cudaSuccess;
-  if (!ready) return set_error(QIA_ERR_CUDA, "%s: cudaFuncSetAttribute failed", who);
+  static std::atomic<uint64_t> allowed;
+  int rc = allow_launch(who, cached_attn_wide_kernel, kSmemBytes, &allowed);
+  if (rc) return rc;
   TileGrid g = tile_grid(p);
   const int64_t groups = int64_t(g.pairs) * p.kv_heads * batch, heads = int64_t(batch) * p.kv_heads;
   Widened wd;
@@ -392,7 +392,7 @@ int launch_cached_wide(const CachedAttn& p, int batch, void* workspace, cudaStre
     wd.k = (__half*)workspace;
     wd.v = wd.k + rows * kCaD;
     wd.info = (TileInfo*)(wd.v + rows * kCaD);
-    int rc = make_rows_map(&tm_k, wd.k, rows);
+    rc = make_rows_map(&tm_k, wd.k, rows);
     if (!rc) rc = make_rows_map(&tm_v, wd.v, rows);
     if (rc) return rc;
     cached_widen_kernel<<<dim3(unsigned(wd.tiles), unsigned(p.kv_heads), unsigned(batch)), 256, 0, st>>>(p, wd);

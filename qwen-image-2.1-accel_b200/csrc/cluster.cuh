@@ -86,6 +86,25 @@ int resident_clusters(void (*kernel)(KArgs...), int threads, int smem, int size,
   return n > 0 ? n : 0;
 }
 
+// Lets `kernel` use `smem` bytes of dynamic shared memory (and clusters of more
+// than eight CTAs) on the current device, once per device: `done` is static
+// storage, one bit per device.
+template <class... KArgs>
+int allow_launch(const char* what, void (*kernel)(KArgs...), int smem, std::atomic<uint64_t>* done, bool big_clusters = false) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return set_error(QIA_ERR_CUDA, "%s: no device", what);
+  const uint64_t bit = uint64_t(1) << dev;
+  if (done->load(std::memory_order_acquire) & bit) return QIA_OK;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && big_clusters) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(QIA_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
+  }
+  done->fetch_or(bit, std::memory_order_release);
+  return QIA_OK;
+}
+
 // Launches `kernel` with clusters of `cluster` CTAs along x (grid.x a multiple
 // of it).
 template <class... KArgs, class... Args>

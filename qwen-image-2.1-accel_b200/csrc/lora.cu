@@ -545,16 +545,13 @@ int make_map(CUtensorMap* map, const void* base, int64_t d0, int64_t d1, int64_t
 }
 
 int launch_tiles(const Lora& p, void* workspace, cudaStream_t st) {
-  static const bool ready =
-      cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           112 * 1024) == cudaSuccess &&
-      cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-      cudaFuncSetAttribute(lora_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           expand_smem(kLoraMaxRank)) == cudaSuccess;
-  if (!ready) return set_error(QIA_ERR_CUDA, "qia_lora_add: cudaFuncSetAttribute failed");
+  static std::atomic<uint64_t> shrink_allowed, expand_allowed;
+  int rc = allow_launch("qia_lora_add", lora_shrink_kernel, 112 * 1024, &shrink_allowed, true);
+  if (!rc) rc = allow_launch("qia_lora_add", lora_expand_kernel, expand_smem(kLoraMaxRank), &expand_allowed);
+  if (rc) return rc;
   __nv_bfloat16* t = (__nv_bfloat16*)workspace;
   CUtensorMap tm_x, tm_a, tm_t, tm_b, tm_base, tm_y;
-  int rc = make_map(&tm_x, p.x, p.in, p.seq, p.batch, p.x_ss, p.x_sb, 128);
+  rc = make_map(&tm_x, p.x, p.in, p.seq, p.batch, p.x_ss, p.x_sb, 128);
   if (!rc) rc = make_map(&tm_a, p.a, p.in, p.r_pad, p.adapters, p.in, int64_t(p.r_pad) * p.in, shrink_rank(p.r_pad));
   if (!rc) rc = make_map(&tm_t, t, p.r_pad, p.seq, p.batch, p.r_pad, int64_t(p.seq) * p.r_pad, 128);
   if (!rc) rc = make_map(&tm_b, p.b, p.r_pad, p.out, p.adapters, p.r_pad, int64_t(p.out) * p.r_pad, kExpandN);

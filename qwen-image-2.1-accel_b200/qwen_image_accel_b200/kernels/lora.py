@@ -73,14 +73,16 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
         out = torch.empty_like(base)
     elif out.shape != base.shape or out.dtype != torch.bfloat16:
         raise ValueError(f"{who}: out must be like base")
+    if not out.numel():
+        return out
+    if out.data_ptr() == x.data_ptr():
+        raise ValueError(f"{who}: out may be base, not x")
     out_strides = out.stride()
     if out_strides[2] != 1:
         raise NotImplementedError(f"{who}: out must have contiguous rows")
     index = weights._index
     if x.get_device() != index or base.get_device() != index or ids.get_device() != index or out.get_device() != index:
         raise ValueError(f"{who}: the adapters are on {weights.device}, x, base, ids or out are not")
-    if not out.numel():
-        return out
     size = _lib.load().qia_lora_workspace_bytes(batch, seq, weights.r_pad)
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     _lib.call("qia_lora_add", x.data_ptr(), base.data_ptr(), out.data_ptr(), *weights._buffers, ids.data_ptr(), batch,

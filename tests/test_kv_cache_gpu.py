@@ -192,6 +192,7 @@ SHAPES = [  # batch, queries, heads, kv_heads, lengths, fresh
     (1, 1, 8, 1, [8193], 0), (2, 3, 12, 4, [65, 64], 3), (1, 16, 4, 4, [127], 16), (2, 17, 4, 2, [129, 16], 17),
     (1, 77, 6, 2, [300], 77), (2, 128, 2, 2, [256, 255], 0), (1, 129, 2, 1, [1], 129), (1, 300, 3, 3, [0], 300),
     (2, 257, 14, 2, [640, 12], 257), (1, 1000, 2, 2, [777], 1000), (1, 40, 5, 1, [2000], 7), (1, 513, 1, 1, [64], 1),
+    (1, 5, 100, 1, [200], 5), (2, 90, 9, 3, [70, 2], 0), (1, 700, 16, 1, [1, ], 33),
 ]
 
 
@@ -280,6 +281,20 @@ def test_strided_inputs_head_major_views_and_out():
         got = cached_attention(q, cache, k, v, key_valid=mask, out=out[:, :sq, :, :128])
         assert_attention(got, *attention64(q, cache, k, v, mask))
         assert (out[:, sq:] == 7).all() and (out[..., 128:] == 7).all()
+
+
+def test_broadcast_keys():
+    """Fresh rows shared by all requests, or by all heads: zero strides."""
+    from qwen_image_accel_b200.kernels.kv_cache import cached_attention, kv_cache_read, kv_cache_write
+    g = gen(19)
+    for sq in (2, 50, 300):
+        cache = make_cache(g, 3, 4, 64, [64, 9, 30])
+        k, v = rows(g, 1, 40, 4, 128).expand(3, -1, -1, -1), rows(g, 3, 40, 1, 128).expand(-1, -1, 4, -1)
+        q = rows(g, 3, sq, 4, 128)
+        assert_attention(cached_attention(q, cache, k, v), *attention64(q, cache, k, v, None))
+        kv_cache_write(cache, k, v)
+        rk, rv = kv_cache_read(cache)
+        assert torch.equal(rk[0], rk[1]) and torch.equal(rv[:, :, 0], rv[:, :, 3])
 
 
 def test_same_bits_twice_and_on_another_stream():

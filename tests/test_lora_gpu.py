@@ -103,6 +103,19 @@ def test_strides_and_streams(s):
     assert torch.equal(both[..., :384], left)
 
 
+@pytest.mark.parametrize("s", [3, 40])
+def test_broadcast_inputs(s):
+    """One activation, and one base row, for all requests: zero strides."""
+    from qwen_image_accel_b200.kernels.lora import LoraWeights, lora_add
+    g = gen(s)
+    items = adapters(g, 128, 256, [16, 8])
+    x, base = rand(g, 1, s, 128).expand(3, -1, -1), rand(g, 3, 1, 256).expand(-1, s, -1)
+    ids = [1, 0, -1]
+    out = torch.empty(3, s, 256, dtype=torch.bfloat16, device=DEV)
+    got = lora_add(x, base, LoraWeights(items), torch.tensor(ids, dtype=torch.int32, device=DEV), out=out)
+    check(got, lora64(x, base, items, ids))
+
+
 @pytest.mark.parametrize("s", [1, 150])
 def test_padding_of_smaller_ranks_is_not_read_and_unused_adapters_do_not_matter(s):
     from qwen_image_accel_b200.kernels.lora import LoraWeights, lora_add
@@ -155,6 +168,8 @@ def test_refusals():
         lora_add(x.float(), base, w, ids)
     with pytest.raises(ValueError, match="CUDA"):
         lora_add(x.cpu(), base.cpu(), w, ids)
+    with pytest.raises(ValueError, match="not x"):
+        lora_add(x, base, w, ids, out=x)
     with pytest.raises(_lib.QiaError, match="multiple of 8"):
         lora_add(rand(g, 2, 3, 68)[..., :64], base, w, ids)
     assert lora_add(x[:, :0], base[:, :0], w, ids).shape == (2, 0, 64)
