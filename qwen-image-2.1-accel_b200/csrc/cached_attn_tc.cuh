@@ -189,25 +189,7 @@ struct RowState {
   float m, l;
 };
 
-// One softmax step of a thread's row: the 128 scores at TMEM column t_s -> f16
-// weights over the first 64 columns, each half announced on p_full[h]; `fresh`:
-// the row's accumulators (t_o) hold nothing yet.
-__device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, const TileInfo* info, float q_up, bool fresh,
-                                             RowState& st, uint64_t* p_full, int lane) {
-  uint32_t s[128];
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    tc_ld_32x32b_x32(t_s + uint32_t(q * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[q * 32]));
-  const float4 num = *reinterpret_cast<const float4*>(info);
-  const float c = num.x * q_up, f = num.y;
-  tc_wait_ld();
-  if (!__float_as_uint(num.w)) {         // some keys take no part
-    const uint4 bits = *reinterpret_cast<const uint4*>(info->valid);
-    const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
-#pragma unroll
-    for (int i = 0; i < 128; ++i)
-      if (!((word[i >> 5] >> (i & 31)) & 1)) s[i] = 0xff800000u;
-  }
+__device__ __forceinline__ float max_of(const uint32_t (&s)[128]) {
   float mx[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s[i]);
@@ -217,7 +199,41 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, const T
     for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
 #pragma unroll
   for (int k = 0; k < 2; ++k) mx[k] = max3(mx[k], __uint_as_float(s[124 + 2 * k]), __uint_as_float(s[125 + 2 * k]));
-  const float top = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), c, f);
+  return fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+}
+
+// One softmax step of a thread's row: the 128 scores at TMEM column t_s -> f16
+// weights over the first 64 columns, each half announced on p_full[h]; `fresh`:
+// the row's accumulators (t_o) hold nothing yet.
+//
+// Keys that take no part have zero rows, so their score is exactly 0 and their
+// weight 2^(f - M + 8) changes nothing but the sum: where every row of the warp
+// has a positive score -- its maximum is then a key's that takes part -- they cost
+// one subtraction per tile (at most 128 times the largest weight: seven bits of
+// fp32). Otherwise their scores are set to -infinity (450 cycles a tile more).
+__device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, const TileInfo* info, float q_up, bool fresh,
+                                             RowState& st, uint64_t* p_full, int lane) {
+  uint32_t s[128];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    tc_ld_32x32b_x32(t_s + uint32_t(q * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[q * 32]));
+  const float4 num = *reinterpret_cast<const float4*>(info);
+  const float c = num.x * q_up, f = num.y;
+  tc_wait_ld();
+  float raw = max_of(s), missing = 0.0f;
+  if (!__float_as_uint(num.w)) {         // some keys take no part
+    const uint4 bits = *reinterpret_cast<const uint4*>(info->valid);
+    if (__all_sync(0xffffffffu, raw > 0.0f)) {
+      missing = float(128 - __popc(bits.x) - __popc(bits.y) - __popc(bits.z) - __popc(bits.w));
+    } else {
+      const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+      for (int i = 0; i < 128; ++i)
+        if (!((word[i >> 5] >> (i & 31)) & 1)) s[i] = 0xff800000u;
+      raw = max_of(s);
+    }
+  }
+  const float top = fmaf(raw, c, f);
   const bool grow = top > st.m + kLag;
   if (__any_sync(0xffffffffu, grow)) {
     const float r = grow ? ex2_ftz(st.m - top) : 1.0f;   // (m = -inf: 0)
@@ -258,7 +274,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, const T
   }
   float a, b;
   f2_unpack(f2_add(sum[0], sum[1]), a, b);
-  st.l = fmaf(a + b, num.z, st.l);
+  st.l = fmaf(fmaf(-missing, ex2_ftz(n1), a + b), num.z, st.l);
 }
 
 // A softmax thread's row of accumulators (128 TMEM columns from t_o) / l -> out.
