@@ -3,17 +3,23 @@
 // converting the codes as it goes: numerics, tiles and joining as in
 // cached_attn_tc.cuh.
 //
-// Roles (512 threads, one CTA per SM):
+// Roles (896 threads, one CTA per SM):
 //   warps 0-3, 4-7  softmax groups 0 and 1 (a query row per thread): scores from
 //                   TMEM, weights back into TMEM;
-//   warp 8          issues the MMAs;
-//   warps 9-15      operand writers: codes and fresh rows -> f16 in the swizzled
-//                   shared-memory tiles, and the tiles' numbers.
-// A key tile is 128 keys. K and V tiles (32 KB each) have two stages. TMEM:
+//   warps 8-15, 16-23  operand writers of K and of V: codes and fresh rows -> f16 in
+//                   the swizzled shared-memory tiles;
+//   warp 24         issues the MMAs;
+//   warp 25         copies the codes to shared memory ahead of the writers, 64 keys of
+//                   K or V (8 KB, contiguous) per bulk copy;
+//   warp 26         the cached tiles' numbers and the factors of their keys.
+// A key tile is 128 keys; the fresh tiles come first, converted while the query
+// rows load and the first codes are on their way (7000 cycles at the end of a CTA
+// otherwise). K and V tiles (32 KB each) have two stages. TMEM:
 // scores of group i at columns [128 i, +128), its weights over the first 64 of
 // them (the A operand of P.V), accumulators at 256 + 128 i. The groups own the two
 // query tiles of the CTA and see every key tile, or, when there is only one query
-// tile, both work on it with the even and the odd key tiles.
+// tile, both work on it with the even and the odd key tiles (and the second query
+// tile's space holds more copies in flight).
 //
 // The issuer runs, per softmax group: P(j).V(j), as each half of P(j) is stored,
 // then Q.K of the group's next key tile, so while one group's products run, the
@@ -24,28 +30,38 @@
 // Keys may be split over a cluster, which joins through distributed shared
 // memory in rank order (no workspace, fixed order). Every wait is bounded (1 s)
 // and reports QIA_ERR_TIMEOUT through the device error word.
+//
+// What bounds it: with one query tile, the writers and the softmax about equally
+// (2250 cycles of work per operand tile, 4200 for the softmax of every second key
+// tile: 3100 cycles per 128 keys, 2.4 TB/s of codes); with two, the softmax, which
+// sees every tile. Both are instruction issue: seven warps per scheduler, nine
+// instructions per four codes. Four requests of 77 rows, 32 heads, on a B200: 8192
+// cached tokens 117 us, 1024 25 us, 16 13 us (seven writer warps, each with its own
+// copies and factors in unrolled code: 150, 28 and 13 us; eight in one team: 155,
+// 30 and 15 us; pieces of the scores read ahead while others are used: 119, 25 and
+// 14 us).
 #include "cached_attn_tc.cuh"
 
 namespace qia {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWriters = 7;                     // operand-writer warps: arrivals of a written tile
-constexpr int kSmemQScale = kSmemTail + kScalarRing * kInfoBytes;   // 2^e_i of 256 rows
+constexpr int kThreads = 896;
+constexpr int kWriters = 8;                     // operand-writer warps of K, and of V: arrivals of a written tile
+constexpr int kInfoRing = 8;
+constexpr int kUnitKeys = 64, kUnitBytes = kUnitKeys * kCaD;        // codes per bulk copy
+constexpr int kUnits = 3, kDuoUnits = kUnits + kTileBytes / kUnitBytes;
+constexpr int kSmemQScale = kSmemTail + kInfoRing * kInfoBytes;     // 2^e_i of 256 rows
 constexpr int kSmemML = kSmemQScale + 256 * 4;                      // m, l of 256 rows (joining)
-constexpr int kSmemFactor = kSmemML + 2 * 256 * 4;                  // [writer][K, V][128] scale 2^-e of a tile's keys
-constexpr int kSmemSlots = kSmemFactor + kWriters * 2 * 128 * 4;    // [writer] maxima
-constexpr int kSmemStage = kSmemSlots + 64;                         // codes of half a tile in flight
-constexpr int kStageBytes = kTileRows * kCaD;
-constexpr int kSmemBars = kSmemStage + kStageBytes;
-constexpr int kSmemBytes = kSmemBars + 256 + 1024;
-// registers of a softmax thread and of any other: 256 x 160 + 256 x 96 = 512 x 128, what the block starts with
-constexpr int kSoftmaxRegs = 160, kOtherRegs = 96;
-
-__device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+constexpr int kSmemFactor = kSmemML + 2 * 256 * 4;                  // [2 tiles][K, V][128] scale 2^-e of a tile's keys
+constexpr int kSmemSlots = kSmemFactor + 2 * 256 * 4;               // [2 tiles][K, V][writer] maxima
+constexpr int kSmemBars = kSmemSlots + 2 * 2 * kWriters * 4;
+constexpr int kSmemStage = kSmemBars + 384;                         // codes in flight
+constexpr int kSmemBytes = kSmemStage + kUnits * kUnitBytes + 1024;
+static_assert(kSmemStage % 16 == 0 && kSmemBytes <= 227 * 1024, "shared memory");
+// registers of a softmax thread, a writer and any other: 256 x 112 + 512 x 56 + 128 x 48 = 63488 of the
+// 896 x 72 that the block starts with
+constexpr int kSoftmaxRegs = 112, kWriterRegs = 56, kOtherRegs = 48;
+static_assert(256 * kSoftmaxRegs + 512 * kWriterRegs + 128 * kOtherRegs <= kThreads * 72, "register split");
 
 __global__ void __launch_bounds__(kThreads, 1)
 cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_constant__ TileGrid tp, int* err) {
@@ -57,13 +73,18 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
   uint64_t* v_full = bars + 2;        // [2]
   uint64_t* k_empty = bars + 4;       // [2] issuer -> operand writers
   uint64_t* v_empty = bars + 6;       // [2]
-  uint64_t* info_full = bars + 8;     // [4] first operand writer -> softmax
+  uint64_t* info_full = bars + 40;    // [8] a tile's numbers -> softmax
   uint64_t* s_full = bars + 12;       // [2] scores of group i
   uint64_t* p_full = bars + 14;       // [2][2] weights of group i, half h, stored
   uint64_t* o_full = bars + 18;
   uint64_t* drain = bars + 19;
   uint64_t* q_full = bars + 20;       // softmax -> issuer
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  uint64_t* stage_full = bars + 21;   // [7] bulk copies -> operand writers
+  uint64_t* stage_empty = bars + 28;  // [7] operand writers -> bulk copies
+  uint64_t* factor_full = bars + 35;  // [2] factors of tile j % 2
+  uint64_t* factor_empty = bars + 37; // [2]
+  uint64_t* fresh_done = bars + 39;   // K and V writers are past the fresh tiles
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 48);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = int(cluster_size()), split = int(cluster_rank());
@@ -76,6 +97,30 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
   const int all_tiles = cached_tiles + (p.sk + 127) / 128;
   const int per = (all_tiles + splits - 1) / splits;
   const int first = min(all_tiles, split * per), n = min(all_tiles, first + per) - first;   // this CTA's key tiles
+  const int cached_n = max(0, min(n, cached_tiles - first)), fresh_n = n - cached_n;         // tiles 0 .. fresh_n - 1: fresh
+  const int64_t head_row = (int64_t(b) * p.kv_heads + kvh) * p.capacity;
+  const uint8_t* mask = p.key_valid ? p.key_valid + b * p.mask_sb : nullptr;
+  const int units = duo ? kDuoUnits : kUnits;
+  const auto unit_at = [&](int s) {
+    return s < kUnits ? sbase + uint32_t(kSmemStage + s * kUnitBytes)
+                      : sbase + uint32_t(kSmemQ + kTileBytes + (s - kUnits) * kUnitBytes);
+  };
+  // The numbers of tile j that come from K (z = 0) or V, by one thread each. Ring
+  // slot j % 8: K of tile j - 1 (for a cached tile, K and V of j - 2) is written, so
+  // Q.K of j - 4 was issued, after P.V of j - 6: the softmax has read those of j - 8.
+  const auto store_info = [&](int j, int z, int e, const uint32_t (&bits)[4]) {
+    TileInfo* info = reinterpret_cast<TileInfo*>(smem + kSmemTail + (j % kInfoRing) * kInfoBytes);
+    if (z) {
+      info->f = float(e);
+      info->inv_f = pow2f(-e);
+    } else {
+      info->c = p.scale_log2 * pow2f(e);
+      info->all = (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) info->valid[i] = bits[i];
+    }
+    mbar_arrive(smem_u32(&info_full[j % kInfoRing]));
+  };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -86,21 +131,30 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
       mbar_init(smem_u32(&s_full[i]), 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&p_full[i]), 4);
-    for (int i = 0; i < kScalarRing; ++i) mbar_init(smem_u32(&info_full[i]), 1);
+    for (int i = 0; i < kInfoRing; ++i) mbar_init(smem_u32(&info_full[i]), 2);
     mbar_init(smem_u32(o_full), 1);
     mbar_init(smem_u32(drain), 1);
+    mbar_init(smem_u32(fresh_done), 2);
     mbar_init(smem_u32(q_full), 8);
+    for (int i = 0; i < kDuoUnits; ++i) {
+      mbar_init(smem_u32(&stage_full[i]), 1);
+      mbar_init(smem_u32(&stage_empty[i]), kWriters);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&factor_full[i]), 1);
+      mbar_init(smem_u32(&factor_empty[i]), 2 * kWriters);
+    }
     fence_barrier_init();
   }
-  if (warp == 8) tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == 24) tmem_alloc(smem_u32(tmem_slot), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 8) {
+  if (warp >= 24) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 8) {
+    if (warp == 24) {
       // ------------------------------------------------------------ MMA issuer
       // (warp-uniform control, one elected lane: see cached_attn_wide.cu)
       if (n > 0) {
@@ -187,104 +241,43 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
         commit(drain);
         mbar_wait(smem_u32(drain), 0, ok ? err : nullptr, 100000000ull);
       }
-    } else {
-      // ------------------------------------------------------- operand writers
-      const int t = threadIdx.x - 32 * 9, writer = warp - 9;
-      const int64_t head_row = (int64_t(b) * p.kv_heads + kvh) * p.capacity;
-      const uint8_t* mask = p.key_valid ? p.key_valid + b * p.mask_sb : nullptr;
-      const int cached_n = max(0, min(n, cached_tiles - first));   // cached tiles of this CTA
-      float* factor = reinterpret_cast<float*>(smem + kSmemFactor) + writer * 256;
-      // z: 0 K, 1 V. Codes: eight threads per row, 28 rows per step, through
-      // pieces of a staging buffer private to the warp, with cp.async: two halves of a
-      // tile in flight where the second query tile's space is free, one otherwise.
-      // (With plain loads a warp waits for all of its outstanding loads at the
-      // first use of any: 5300 cycles per tile.)
-      constexpr int kSteps = 5;
-      const int trow = t >> 3, depth = duo ? 2 : 1;
-      const uint32_t stage = duo ? sbase + kSmemQ + kTileBytes : sbase + kSmemStage;
-      const auto issue = [&](int u) {      // half u: K (even) or V of tile u / 2
-        if (u < 2 * cached_n) {
-          const int k0 = (first + (u >> 1)) * 128;
-          const int8_t* src = ((u & 1) ? p.vc : p.kc) + head_row * kCaD + (t & 7) * 16;
-#pragma unroll
-          for (int i = 0; i < kSteps; ++i) {
-            const int row = i * 28 + trow;
-            if (row < kTileRows)   // (past the length: any held row, factor 0)
-              cp_async16(stage + uint32_t(duo ? (u & 1) * kStageBytes : 0) + uint32_t(row * kCaD + (t & 7) * 16),
-                         src + int64_t(min(k0 + row, len - 1)) * kCaD);
-          }
-        }
-        cp_async_commit();      // (an empty group keeps the count)
-      };
-      // Eight codes (one 16-byte f16 piece) per thread and row: sixteen threads per
-      // row read what their warp staged.
-      const auto take_codes = [&](int u, uint2 (&c)[2 * kSteps]) {
-        if (duo) asm volatile("cp.async.wait_group 1;" ::: "memory");
-        else asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 2 * kSteps; ++i) {
-          const int row = (i >> 1) * 28 + writer * 4 + (i & 1) * 2 + (lane >> 4);
-          const uint32_t at = stage + uint32_t(duo ? (u & 1) * kStageBytes : 0) + uint32_t(row * kCaD + (lane & 15) * 8);
-          c[i] = make_uint2(0u, 0u);
-          if (row < kTileRows)
-            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(c[i].x), "=r"(c[i].y) : "r"(at) : "memory");
-        }
-        __syncwarp();
-        issue(u + depth);
-      };
-      const auto slot_of = [&](int j, int z) { return sbase + kSmemKV + uint32_t((j & 1) * 2 + z) * kTileBytes; };
-      const auto store_codes = [&](int j, int z, const uint2 (&c)[2 * kSteps]) {
-        const uint32_t slot = slot_of(j, z);
-#pragma unroll
-        for (int i = 0; i < 2 * kSteps; ++i) {
-          const int row = (i >> 1) * 28 + writer * 4 + (i & 1) * 2 + (lane >> 4);
-          if (row >= kTileRows) break;
-          const float a = factor[z * 128 + row];
-          const uint2 x = widen4(c[i].x, a), y = widen4(c[i].y, a);
-          st_shared_v4(slot + tile_offset(row, lane & 15), x.x, x.y, y.x, y.y);
-        }
-      };
-      const auto publish = [&](int j, int z) {
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(z ? &v_full[j & 1] : &k_full[j & 1]));
-      };
-      const auto wait_slot = [&](int j, int z) {
-        return __all_sync(0xffffffffu, mbar_wait(smem_u32(z ? &v_empty[j & 1] : &k_empty[j & 1]), ((j >> 1) & 1) ^ 1, err));
-      };
-      // (ring slot j % 4: tile j - 4 was done before V of j - 3 left)
-      const auto store_info = [&](int j, int e, int f, const uint32_t (&bits)[4]) {
-        if (writer == 0 && lane == 0) {
-          TileInfo* info = reinterpret_cast<TileInfo*>(smem + kSmemTail + (j % kScalarRing) * kInfoBytes);
-          info->c = p.scale_log2 * pow2f(e);
-          info->f = float(f);
-          info->inv_f = pow2f(-f);
-          info->all = (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) info->valid[i] = bits[i];
-          mbar_arrive(smem_u32(&info_full[j % kScalarRing]));
-        }
-      };
-      // ---- cached tiles. Every writer warp keeps the scales of the tile's keys
-      // (keys lane + 32 i), so that no writer waits for another.
+    } else if (warp == 25 && lane == 0) {
+      // ------------------------------------------------------------ bulk copies
+      // (only held rows are read; what the buffer keeps past the length has factor 0)
+      int st = 0, u = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (; u < 4 * cached_n; ++u) {          // K, V of tile u / 4 in halves
+        ok = mbar_wait(smem_u32(&stage_empty[st]), phase ^ 1, err);
+        if (!ok) break;
+        const int k0 = (first + (u >> 2)) * kTileRows + (u & 1) * kUnitKeys, rows = max(0, min(len - k0, kUnitKeys));
+        mbar_arrive_expect_tx(smem_u32(&stage_full[st]), uint32_t(rows * kCaD));
+        if (rows > 0)
+          bulk_load(unit_at(st), ((u & 2) ? p.vc : p.kc) + (head_row + k0) * kCaD, uint32_t(rows * kCaD),
+                    smem_u32(&stage_full[st]));
+        if (++st == units) { st = 0; phase ^= 1; }
+      }
+      if (!ok)   // let queued copies land before the shared memory is released
+        for (int i = max(0, u - units); i < u; ++i)
+          mbar_wait(smem_u32(&stage_full[i % units]), uint32_t((i / units) & 1), nullptr, 100000000ull);
+    } else if (warp == 26) {
+      // ---------------------------------------- numbers and factors of cached tiles
+      // (keys lane + 32 i; the next tile's scales are requested before this one's are used)
+      float* factors = reinterpret_cast<float*>(smem + kSmemFactor);
       float ks[4], vs[4];
       bool valid[4];
       const auto load_scales = [&](int j) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = (first + j) * 128 + 32 * i + lane;
+          const int key = (first + j) * kTileRows + 32 * i + lane;
           ks[i] = __ldg(p.ks + head_row + min(key, len - 1));
           vs[i] = __ldg(p.vs + head_row + min(key, len - 1));
           valid[i] = key < len && (!mask || __ldg(mask + key) != 0);
         }
       };
-      uint2 codes[2 * kSteps];
-      bool ok = true;
-      for (int u = 0; u < depth; ++u) issue(u);
       if (cached_n > 0) load_scales(0);
-      int j = 0;
-      for (; j < cached_n; ++j) {
+#pragma unroll 1
+      for (int j = 0; j < cached_n; ++j) {
         uint32_t mk = 0, mv = 0, bits[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -295,96 +288,127 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
         }
         const int e = code_exponent(__reduce_max_sync(0xffffffffu, mk), kLowK);
         const int f = code_exponent(__reduce_max_sync(0xffffffffu, mv), kLowV);
-        store_info(j, e, f, bits);
-        __syncwarp();                        // (the previous tile's factors were read)
+        // (the factors of tile j - 2 were used; the ring of numbers is not more than its length ahead)
+        bool ok = mbar_wait(smem_u32(&factor_empty[j & 1]), ((j >> 1) & 1) ^ 1, err);
+        if (j == 0 && fresh_n > kInfoRing / 2) ok = ok && mbar_wait(smem_u32(fresh_done), 0, err);
+        if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          factor[32 * i + lane] = ks[i] * pow2f(-e);
-          factor[128 + 32 * i + lane] = vs[i] * pow2f(-f);
+          factors[(j & 1) * 256 + 32 * i + lane] = code_factor(ks[i] * pow2f(-e));
+          factors[(j & 1) * 256 + 128 + 32 * i + lane] = code_factor(vs[i] * pow2f(-f));
         }
         __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&factor_full[j & 1]));
+          store_info(fresh_n + j, 0, e, bits);
+          store_info(fresh_n + j, 1, f, bits);
+        }
         if (j + 1 < cached_n) load_scales(j + 1);
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          take_codes(2 * j + z, codes);
-          ok = ok && wait_slot(j, z);
-          if (ok) {
-            store_codes(j, z, codes);
-            publish(j, z);
-          }
-        }
-        if (!ok) break;
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      // ---- fresh tiles: the exponents come from the rows themselves (sixteen
-      // threads per row, 14 rows per step)
-      constexpr int kFresh = 10;
-      uint32_t* slots = reinterpret_cast<uint32_t*>(smem + kSmemSlots);
-      for (; j < n && ok; ++j) {
-        const int k0 = (first + j - cached_tiles) * 128, piece = t & 15;
-        uint32_t bits[4];
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    // --------------------------------------------------------- operand writers
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWriterRegs));
+    const int writer = (warp - 8) & 7, z = (warp - 8) >> 3, t = writer * 32 + lane, piece = lane & 15;   // z: 0 K, 1 V
+    uint64_t* full = z ? v_full : k_full;
+    uint64_t* empty = z ? v_empty : k_empty;
+    const uint32_t slots0 = sbase + uint32_t(kSmemKV + z * kTileBytes);      // tile j in stage j % 2
+    const auto publish = [&](int j) {
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&full[j & 1]));
+    };
+    bool ok = true;
+    // ---- fresh tiles: the exponent comes from the rows themselves (sixteen
+    // threads per row, 16 rows per step; one named barrier per tile and operand, passed
+    // whether or not a wait gave up)
+    uint32_t* slots = reinterpret_cast<uint32_t*>(smem + kSmemSlots);
+    const __nv_bfloat16* src = z ? p.v + b * p.v_sb + kvh * p.v_sh : p.k + b * p.k_sb + kvh * p.k_sh;
+    const int64_t ss = z ? p.v_ss : p.k_ss;
+#pragma unroll 1
+    for (int j = 0; j < fresh_n; ++j) {
+      const int k0 = (first + cached_n + j - cached_tiles) * kTileRows;
+      uint32_t bits[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = k0 + 32 * i + lane;
-          bits[i] = __ballot_sync(0xffffffffu, key < p.sk && (!mask || __ldg(mask + p.extent + key) != 0));
-        }
-        const auto load_rows = [&](int z, uint4 (&c)[kFresh]) {
-          const __nv_bfloat16* src = z ? p.v + b * p.v_sb + kvh * p.v_sh : p.k + b * p.k_sb + kvh * p.k_sh;
-          const int64_t ss = z ? p.v_ss : p.k_ss;
-#pragma unroll
-          for (int i = 0; i < kFresh; ++i) {
-            const int row = i * 14 + (t >> 4);
-            const uint32_t word = row < 32 ? bits[0] : row < 64 ? bits[1] : row < 96 ? bits[2] : bits[3];
-            c[i] = row < kTileRows && ((word >> (row & 31)) & 1)
-                       ? __ldg(reinterpret_cast<const uint4*>(src + int64_t(k0 + row) * ss) + piece)
-                       : make_uint4(0u, 0u, 0u, 0u);
-          }
-        };
-        const auto exponent = [&](const uint4 (&c)[kFresh], int lo) {
-          uint32_t m = 0;
-#pragma unroll
-          for (int i = 0; i < kFresh; ++i) m = finite_max8(c[i], m);
-          m = __reduce_max_sync(0xffffffffu, m);
-          asm volatile("bar.sync 1, 224;" ::: "memory");      // (the slots' last readers are done)
-          if (lane == 0) slots[writer] = m;
-          asm volatile("bar.sync 1, 224;" ::: "memory");
-#pragma unroll
-          for (int i = 0; i < kWriters; ++i) m = max(m, slots[i]);
-          return tile_exponent(m, lo);
-        };
-        const auto store_rows = [&](int z, const uint4 (&c)[kFresh], float a) {
-          const uint32_t slot = slot_of(j, z);
-#pragma unroll
-          for (int i = 0; i < kFresh; ++i) {
-            const int row = i * 14 + (t >> 4);
-            const uint4 h = narrow8(c[i], a);
-            if (row < kTileRows) st_shared_v4(slot + tile_offset(row, piece), h.x, h.y, h.z, h.w);
-          }
-        };
-        uint4 c[kFresh];
-        load_rows(1, c);
-        const int f = exponent(c, kLowV);
-        load_rows(0, c);
-        const int e = exponent(c, kLowK);
-        store_info(j, e, f, bits);
-        // (a warp whose wait gives up leaves the others: their named barriers do
-        // not depend on it beyond this tile's, which it has passed)
-        ok = wait_slot(j, 0);
-        if (ok) {
-          store_rows(0, c, pow2f(-e));
-          publish(j, 0);
-          load_rows(1, c);
-          ok = wait_slot(j, 1);
-        }
-        if (ok) {
-          store_rows(1, c, pow2f(-f));
-          publish(j, 1);
-        }
-        ok = __all_sync(0xffffffffu, ok);
+      for (int i = 0; i < 4; ++i) {
+        const int key = k0 + 32 * i + lane;
+        bits[i] = __ballot_sync(0xffffffffu, key < p.sk && (!mask || __ldg(mask + p.extent + key) != 0));
       }
-      for (; j < n; ++j)    // the barriers of tiles that were given up
-        if (j >= cached_n)
-          for (int i = 0; i < 4; ++i) asm volatile("bar.sync 1, 224;" ::: "memory");
+      uint4 c[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = i * 16 + (t >> 4);
+        c[i] = (bits[i >> 1] >> (row & 31)) & 1
+                   ? __ldg(reinterpret_cast<const uint4*>(src + int64_t(k0 + row) * ss) + piece)
+                   : make_uint4(0u, 0u, 0u, 0u);
+      }
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = finite_max8(c[i], m);
+      m = __reduce_max_sync(0xffffffffu, m);
+      // (a slot is written again two tiles on: every writer has read it before the barrier between)
+      uint32_t* mine = slots + ((j & 1) * 2 + z) * kWriters;
+      if (lane == 0) mine[writer] = m;
+      asm volatile("bar.sync %0, 256;" ::"r"(3 + z) : "memory");
+#pragma unroll
+      for (int i = 0; i < kWriters; ++i) m = max(m, mine[i]);
+      const int e = tile_exponent(m, z ? kLowV : kLowK);
+      if (ok && t == 0) store_info(j, z, e, bits);
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[j & 1]), ((j >> 1) & 1) ^ 1, err));
+      if (ok) {
+        const uint32_t slot = slots0 + uint32_t((j & 1) * 2 * kTileBytes);
+        const float a = pow2f(-e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint4 x = narrow8(c[i], a);
+          st_shared_v4(slot + tile_offset(i * 16 + (t >> 4), piece), x.x, x.y, x.z, x.w);
+        }
+        publish(j);
+      }
+    }
+    if (fresh_n > 0 && t == 0) mbar_arrive(smem_u32(fresh_done));
+    // ---- cached tiles: eight rows per warp and unit, sixteen threads (of eight
+    // codes, one 16-byte piece) per row, in a short loop: the instruction cache has to
+    // hold it beside the softmax. Its steps are latencies (waits, loads, the proxy
+    // fence), which sixteen warps hide.
+    const int row0 = 8 * writer + (lane >> 4);
+    const uint32_t code_at = uint32_t(row0 * kCaD + piece * 8);
+    const float* factors = reinterpret_cast<const float*>(smem + kSmemFactor) + z * 128 + row0;
+    int st = 2 * z;
+    uint32_t phase = 0;
+#pragma unroll 1
+    for (int u = 0; u < 2 * cached_n; ++u) {
+      const int i0 = u >> 1, j = fresh_n + i0, h = u & 1;
+      if (h == 0)
+        ok = ok && mbar_wait(smem_u32(&factor_full[i0 & 1]), (i0 >> 1) & 1, err) &&
+             mbar_wait(smem_u32(&empty[j & 1]), ((j >> 1) & 1) ^ 1, err);
+      ok = ok && mbar_wait(smem_u32(&stage_full[st]), phase, err);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      const uint32_t from = unit_at(st) + code_at;
+      uint2 codes[4];
+      float a[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(codes[i].x), "=r"(codes[i].y) : "r"(from + uint32_t(i * 2 * kCaD))
+                     : "memory");
+        a[i] = factors[(i0 & 1) * 256 + h * kUnitKeys + 2 * i];
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&stage_empty[st]));
+        if (h == 1) mbar_arrive(smem_u32(&factor_empty[i0 & 1]));
+      }
+      const uint32_t slot = slots0 + uint32_t((j & 1) * 2 * kTileBytes + h * kUnitKeys * 128);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float off = widen_offset(a[i]);
+        const uint2 x = widen4(codes[i].x, a[i], off), y = widen4(codes[i].y, a[i], off);
+        st_shared_v4(slot + tile_offset(row0 + 2 * i, piece), x.x, x.y, y.x, y.y);
+      }
+      if (h == 1) publish(j);
+      st += h ? 3 : 1;                       // (the other operand's units lie between)
+      if (st >= units) { st -= units; phase ^= 1; }
     }
   } else {
     // ----------------------------------------------------------------- softmax
@@ -404,25 +428,23 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
     for (int it = 0; it < count; ++it) {
       const int j = duo ? 2 * it + w : it;
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[w]), it & 1, err) &&
-                                       mbar_wait(smem_u32(&info_full[j % kScalarRing]), (j / kScalarRing) & 1, err));
+                                       mbar_wait(smem_u32(&info_full[j % kInfoRing]), (j / kInfoRing) & 1, err));
       if (!ok) break;
       tc_fence_after();
-      softmax_tile(t_s, t_o, reinterpret_cast<const TileInfo*>(smem + kSmemTail + (j % kScalarRing) * kInfoBytes), q_up,
+      softmax_tile<false>(t_s, t_o, reinterpret_cast<const TileInfo*>(smem + kSmemTail + (j % kInfoRing) * kInfoBytes), q_up,
                    it == 0, st, &p_full[2 * w], lane);
     }
     bool have = ok && count > 0;       // the accumulators hold something
     if (ok && n > 0) have = __all_sync(0xffffffffu, mbar_wait(smem_u32(o_full), 0, err)) && have;
     tc_fence_after();
-    const int token = (2 * pair + w) * tp.tokens_per_tile + row / p.share;
     if (splits == 1 && !duo)
-      store_row(t_o, have, st.l, row < tp.tokens_per_tile * p.share && token < p.sq,
-                p.out + b * p.o_sb + int64_t(token) * p.o_ss + int64_t(kvh * p.share + row % p.share) * p.o_sh);
+      store_rows(p, tp, sbase + uint32_t(kSmemQ + w * kTileBytes), t_o, have, st.l, 2 * pair + w, row, kvh, b);
     else
       stage_row(t_o, have, st.m, st.l, sbase, reinterpret_cast<float*>(smem + kSmemML), w * kTileRows + row);
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 24) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

@@ -89,15 +89,16 @@ __global__ void __launch_bounds__(256, 3) cached_widen_kernel(const __grid_const
     const uint32_t mk = block_max(t < 128 ? mag : 0u, slots[0]), mv = block_max(t < 128 ? 0u : mag, slots[1]);
     e[0] = code_exponent(mk, kLowK);
     e[1] = code_exponent(mv, kLowV);
-    factor[t >> 7][t & 127] = mine * pow2f(-e[t >> 7]);
+    factor[t >> 7][t & 127] = code_factor(mine * pow2f(-e[t >> 7]));
     __syncthreads();
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = i * 32 + (t >> 3);
-        const float a = factor[z][row];
-        const uint2 x = widen4(c[z][i].x, a), y = widen4(c[z][i].y, a), u = widen4(c[z][i].z, a), v = widen4(c[z][i].w, a);
+        const float a = factor[z][row], off = widen_offset(a);
+        const uint2 x = widen4(c[z][i].x, a, off), y = widen4(c[z][i].y, a, off);
+        const uint2 u = widen4(c[z][i].z, a, off), v = widen4(c[z][i].w, a, off);
         st_global_v8((z ? w.v : w.k) + (out_row + row) * kCaD + 16 * (t & 7), make_uint4(x.x, x.y, y.x, y.y),
                      make_uint4(u.x, u.y, v.x, v.y));
       }
@@ -308,16 +309,14 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
                                        mbar_wait(smem_u32(&info_full[j % kScalarRing]), (j / kScalarRing) & 1, err));
       if (!ok) break;
       tc_fence_after();
-      softmax_tile(t_s, t_o, reinterpret_cast<const TileInfo*>(smem + kSmemTail + (j % kScalarRing) * kInfoBytes), q_up,
+      softmax_tile<true>(t_s, t_o, reinterpret_cast<const TileInfo*>(smem + kSmemTail + (j % kScalarRing) * kInfoBytes), q_up,
                    j == 0, st, &p_full[2 * w], lane);
     }
     const bool have = ok && n > 0 && __all_sync(0xffffffffu, mbar_wait(smem_u32(o_full), 0, err));
     tc_fence_after();
     if (w < n_tiles) {
-      const int token = (2 * pair + w) * tp.tokens_per_tile + row / p.share;
       if (splits == 1)
-        store_row(t_o, have, st.l, row < tp.tokens_per_tile * p.share && token < p.sq,
-                  p.out + b * p.o_sb + int64_t(token) * p.o_ss + int64_t(kvh * p.share + row % p.share) * p.o_sh);
+        store_rows(p, tp, sbase + uint32_t(kSmemQ + w * kTileBytes), t_o, have, st.l, 2 * pair + w, row, kvh, b);
       else
         stage_row(t_o, have, st.m, st.l, sbase, reinterpret_cast<float*>(smem + kSmemML), w * kTileRows + row);
     }
