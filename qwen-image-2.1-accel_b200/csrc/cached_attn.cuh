@@ -7,17 +7,18 @@
 // vc_j with INT8 codes kc, vc) and its fresh bf16 tokens, each only where
 // key_valid is set. A query with no key writes zeros.
 //
-// The codes are the tensor-core operands (every INT8 value is exact in bf16 and
-// f16), and both scales move into the exponent, so that a key costs one fused
-// multiply-add per score and masks cost nothing:
+// No scale is left in the inner loop of either kind of kernel, and masks cost
+// (almost) nothing. On the tensor cores of the larger forms the keys are f16 rows
+// scaled by powers of two per tile (cached_attn_tc.cuh). In the 16-row form the codes
+// themselves are the operands (every INT8 value is exact in f16) and both scales
+// move into the exponent, so that a key costs one fused multiply-add per score:
 //   t_ij = (c log2e ks_j) (q_i.kc_j) + log2 vs_j
 //   w_ij = 2^(t_ij - M_i)               the weight of the code vc_j
 //   o_i  = sum_j w_ij vc_j / sum_j w_ij / vs_j
-// A masked or missing key has (0, -inf, 0) for (c log2e ks, log2 vs, 1/vs) and
+// There a masked or missing key has (0, -inf, 0) for (c log2e ks, log2 vs, 1/vs) and
 // zero rows, so its w is exactly 0 whatever its memory holds.
-// M_i is a running maximum that may lag the true one by a bounded factor (the
-// weights then exceed 1, which both operand types hold), so the accumulators
-// are rescaled rarely.
+// M_i is a running maximum that may lag the true one by 2^7 (the weights then
+// exceed 1, which f16 holds), so the accumulators are rescaled rarely.
 #pragma once
 
 #include "qia_common.cuh"
@@ -66,12 +67,12 @@ __device__ __forceinline__ KeyScalars key_scalars(const CachedAttn& p, float ks,
 }
 
 // The forms by query rows per K/V head (seq_q * share): one 16-row tile
-// (cached_attn.cu), up to two 128-row tiles (cached_attn_tiles.cu), more
-// (cached_attn_wide.cu, which needs a workspace).
+// (cached_attn.cu); up to two 128-row tiles over many keys (cached_attn_tiles.cu);
+// more, or few keys (cached_attn_wide.cu, which needs a workspace).
 int launch_cached_rows(const CachedAttn& p, int batch, cudaStream_t st);
 int launch_cached_tiles(const CachedAttn& p, int batch, cudaStream_t st);
 int launch_cached_wide(const CachedAttn& p, int batch, void* workspace, cudaStream_t st);
-bool cached_use_wide(int64_t seq_q, int64_t share);
+bool cached_use_wide(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t kv_heads, int64_t share, int64_t extent);
 int64_t cached_wide_workspace(int64_t batch, int64_t seq_k, int64_t kv_heads, int64_t extent);
 
 __device__ __forceinline__ float ex2_ftz(float x) {

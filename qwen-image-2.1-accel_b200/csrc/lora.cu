@@ -1,25 +1,29 @@
 // Low-rank adapters of many requests beside a shared projection:
 //   y[b, s] = base[b, s] + scale_i * B_i (A_i x[b, s]),   i = ids[b]
 // with A_i [r_i, in], B_i [out, r_i] of adapter i; ids[b] < 0: y = base.
-// A is stored [adapters, r_pad, in] and B [adapters, out, r_pad], bf16, rows and
-// columns past the adapter's own rank ignored. fp32 accumulation throughout,
-// one rounding of y to bf16. The padding of A and B holds zeros.
+// A is stored [adapters, r_pad, in] and B [adapters, out, r_pad], bf16, with zeros
+// past an adapter's own rank. fp32 accumulation throughout, one rounding of y to bf16.
 //
-// Two forms. lora_tokens_kernel: up to eight tokens per request, which are the
-// columns of m16n8k16 products whose rows are weights: the weights are what is
-// read (2 bytes per product), straight from global memory into the operand
-// registers of the warp that uses them, and the call is a chain of latencies --
-// id, rows of A, exchange, rows of B (requested before the exchange), y. A cluster
-// of up to eight CTAs serves a request: its warps share the 16-row blocks of A
-// and slices of the contraction, every partial sum is stored into all CTAs'
-// shared memory, and after one cluster barrier each CTA computes its slice of the
-// outputs with t = scale A x as a sum of two bf16 numbers (2^-17 of t). One
+// Two forms, chosen by their estimated times (plan_tokens, tiles_us).
+// lora_tokens_kernel: eight tokens of a request, or eight single-token requests of
+// one adapter, are the columns of m16n8k16 products whose rows are weights: the
+// weights are what is read (2 bytes per product), straight from global memory into
+// the operand registers of the warp that uses them, and the call is a chain of
+// latencies -- id, rows of A, exchange, rows of B (requested before the exchange), y.
+// A cluster of up to eight CTAs serves eight tokens: its warps share the 16-row
+// blocks of A and slices of the contraction, every partial sum is stored into all
+// CTAs' shared memory, and after one cluster barrier each CTA computes its slice of
+// the outputs with t = scale A x as a sum of two bf16 numbers (2^-17 of t). One
 // launch, fixed summation order. (With one lane per weight row and fp32 FMAs the
-// same schedule executed ten times the instructions.)
+// same schedule executed ten times the instructions.) 32 single tokens, 4096 -> 4096,
+// rank 64, eight adapters: 9.3 us, 5 us of them launch and latency; 4 x 77 tokens,
+// 12288 -> 4096, rank 16: 11.3 us.
 //
 // lora_shrink_kernel + lora_expand_kernel: many tokens per request, on tcgen05.
 // Both are bound by the bytes of x and of base and y, so a CTA is a stream of
-// TMA tiles with as much in flight as fits, and the products hide behind it:
+// TMA tiles with as much in flight as fits, and the products hide behind it (four
+// requests of 4096 tokens, 4096 -> 12288, rank 64: 170 us, 85 % of the copy's rate:
+// shrink 31 us, its bytes 21; expand 139, its bytes 123):
 //   shrink  t = scale_i A_i x for 128 tokens, the contraction split over a
 //           cluster until the CTAs fill the device; partial sums are added
 //           through distributed shared memory in rank order; t is rounded to
@@ -33,6 +37,7 @@
 // never crosses into another request and ragged edges are zero-filled or cut.
 #include <cudaTypedefs.h>
 
+#include <cmath>
 #include <mutex>
 
 #include "cluster.cuh"
@@ -173,7 +178,10 @@ __global__ void __launch_bounds__(kTokWarps * 32, 2) lora_tokens_kernel(const __
   // ---- rows of B and base of kRounds blocks of 16 outputs: channels 16 k + 4 c .. + 3 of every c
   const int rank = id < 0 ? 0 : min(max(__ldg(p.ranks + at), 0), p.r_pad), steps = (rank + 15) / 16;
   const float scale = __ldg(p.scales + at);
-  const int out_blocks = (p.out + 15) / 16, stride = ctas * kTokWarps;
+  // (this cluster's share of the outputs: blockIdx.z of gridDim.z)
+  const int all_blocks = (p.out + 15) / 16, share = (all_blocks + int(gridDim.z) - 1) / int(gridDim.z);
+  const int first_block = int(blockIdx.z) * share, out_blocks = min(all_blocks, first_block + share);
+  const int out_end = min(p.out, out_blocks * 16), stride = ctas * kTokWarps;
   int64_t col_base[2], col_y[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -190,15 +198,15 @@ __global__ void __launch_bounds__(kTokWarps * 32, 2) lora_tokens_kernel(const __
         const int o = (first + q * stride) * 16 + g + 8 * h;
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
-          w[q][k][h] = k < steps && 16 * k + 4 * c < p.r_pad && o < p.out
+          w[q][k][h] = k < steps && 16 * k + 4 * c < p.r_pad && o < out_end
                            ? __ldg(reinterpret_cast<const uint2*>(p.b + (int64_t(at) * p.out + o) * p.r_pad + 16 * k + 4 * c))
                            : make_uint2(0u, 0u);
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          base[q][h][e] = o < p.out && 2 * c + e < live ? bf16_to_f32(p.base[col_base[e] + o]) : 0.0f;
+          base[q][h][e] = o < out_end && 2 * c + e < live ? bf16_to_f32(p.base[col_base[e] + o]) : 0.0f;
       }
   };
-  int ob = cta * kTokWarps + warp;
+  int ob = first_block + cta * kTokWarps + warp;
   load(ob);
   cluster_sync();
   for (int i = threadIdx.x; i < ranks16 * kTokens; i += blockDim.x) {
@@ -236,7 +244,7 @@ __global__ void __launch_bounds__(kTokWarps * 32, 2) lora_tokens_kernel(const __
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int o = (ob + q * stride) * 16 + g + 8 * h, tok = 2 * c + e;
-          if (o < p.out && tok < live)
+          if (o < out_end && tok < live)
             p.y[col_y[e] + o] = f32_to_bf16(base[q][h][e] + acc[2 * h + e]);
         }
     }
@@ -245,16 +253,44 @@ __global__ void __launch_bounds__(kTokWarps * 32, 2) lora_tokens_kernel(const __
   }
 }
 
-int launch_tokens(const Lora& p, cudaStream_t st) {
+// How the token form would run: CTAs of a cluster, clusters that share the outputs
+// of a group of eight tokens (each computes t), and about how long, in us. A
+// cluster takes 5 us and its weights, 31 MB / ms and CTA; beyond four fifths of an SM's
+// worth of CTAs two share an SM (1.4 times as long), beyond 1.85 there is another
+// wave; and L2 gives about 4 MB / us. On a B200, 4096 -> 12288 at rank 128, one token:
+// 22 us without sharing, 10 with six clusters; 12288 -> 4096 at rank 16, 4 x 77
+// tokens: 15.8 us in clusters of eight (two waves), 11.3 in clusters of four.
+struct TokenPlan {
+  int ctas, shares;
+  float us;
+};
+
+TokenPlan plan_tokens(const Lora& p) {
+  int64_t groups = int64_t(p.batch) * ((p.seq + kTokens - 1) / kTokens);
+  if (p.seq == 1) {      // requests of one adapter go together
+    const int64_t most = int64_t(p.batch) / kTokens + p.adapters + 1;
+    groups = groups < most ? groups : most;
+  }
+  TokenPlan best = {1, 1, INFINITY};
+  // (a CTA has work for its warps down to 128 outputs or 256 channels)
+  for (int ctas = 1; ctas <= 8 && (ctas == 1 || ctas * kTokWarps * 8 < p.out || ctas * kTokWarps * 16 < p.in); ctas *= 2) {
+    const int pass = ctas * kTokWarps * (p.r_pad <= 64 ? 4 : 2) * 16;     // outputs that a cluster has in flight
+    for (int shares = 1; shares <= 8 && (shares - 1) * pass < p.out; ++shares) {
+      const float n = float(groups) * ctas * shares, sms = float(sm_count());
+      const float mb = p.r_pad * 2e-6f * (p.in + float(p.out) / shares);
+      const float us = fmaxf((n <= 0.8f * sms ? 1.0f : 1.4f * ceilf(n / (1.85f * sms))) * (5.0f + 32.0f * mb / ctas),
+                             5.0f + 0.25f * float(groups) * shares * mb);
+      if (us < best.us) best = {ctas, shares, us};
+    }
+  }
+  return best;
+}
+
+int launch_tokens(const Lora& p, const TokenPlan& plan, cudaStream_t st) {
   const int64_t chunks = (int64_t(p.seq) + kTokens - 1) / kTokens;
-  // two CTAs of 256 threads per SM; a CTA has work for its warps down to 128 outputs or 256 channels
-  int ctas = 1;
-  while (ctas < 8 && chunks * p.batch * ctas < 2 * sm_count() &&
-         (ctas * kTokWarps * 16 < p.out || ctas * kTokWarps * 32 < p.in))
-    ctas *= 2;
-  const dim3 grid(unsigned(chunks * ctas), unsigned(p.batch));
+  const dim3 grid(unsigned(chunks * plan.ctas), unsigned(p.batch), unsigned(plan.shares));
   const auto run = [&](auto kernel) {
-    return launch_cluster("qia_lora_add", kernel, grid, kTokWarps * 32, 0, ctas, st, p, device_error_word());
+    return launch_cluster("qia_lora_add", kernel, grid, kTokWarps * 32, 0, plan.ctas, st, p, device_error_word());
   };
   return p.r_pad <= 32 ? run(lora_tokens_kernel<2>) : p.r_pad <= 64 ? run(lora_tokens_kernel<4>) : run(lora_tokens_kernel<8>);
 }
@@ -560,9 +596,19 @@ int launch_tiles(const Lora& p, void* workspace, cudaStream_t st) {
   if (rc) return rc;
   const int64_t tiles = (int64_t(p.seq) + 127) / 128;
   const int blocks = (p.in + 63) / 64;
-  // the contraction is split until the CTAs fill the device, down to two stages' worth each
+  // The contraction is split until the CTAs fill the device, down to eight
+  // 64-channel blocks each, while the clusters run at once: two CTAs per SM, one
+  // with clusters of sixteen (4096 -> 4096 at rank 64, eight requests of 333 tokens:
+  // 24.2 us, 21.4 in fewer CTAs; sixteen of 77: 19.5 us, 27.1 in clusters of
+  // sixteen, which take two waves; 12288 -> 4096, four of 77: 14.2 us in sixteen
+  // splits, 16.3 in eight).
+  static std::atomic<int> resident[17];
+  const int64_t requests = tiles * p.batch;
   int splits = 1;
-  while (splits < 16 && tiles * p.batch * splits < sm_count() && blocks >= 4 * splits * 2) splits *= 2;
+  while (splits < 16 && requests * splits < sm_count() && blocks >= 8 * splits * 2 &&
+         requests <= (splits < 8 ? 2 : 1) *
+                         resident_clusters(lora_shrink_kernel, 192, shrink_smem(p.r_pad), 2 * splits, resident))
+    splits *= 2;
   rc = launch_cluster("lora_shrink_kernel", lora_shrink_kernel, dim3(unsigned(tiles * splits), unsigned(p.batch)), 192,
                       size_t(shrink_smem(p.r_pad)), splits, st, tm_x, tm_a, p, t, device_error_word());
   if (rc) return rc;
@@ -585,12 +631,22 @@ int launch_tiles(const Lora& p, void* workspace, cudaStream_t st) {
   return QIA_OK;
 }
 
-// Few tokens per request, or a broadcast row or request (a zero stride, which
-// a tensor map does not take).
-bool use_tokens(int64_t batch, int64_t seq, const Lora& p) {
-  if (seq <= 8) return true;
+// A broadcast row or request: a zero stride, which a tensor map does not take.
+bool broadcast(const Lora& p) {
   return p.x_ss <= 0 || p.base_ss <= 0 || p.y_ss <= 0 ||
-         (batch > 1 && (p.x_sb <= 0 || p.base_sb <= 0 || p.y_sb <= 0));
+         (p.batch > 1 && (p.x_sb <= 0 || p.base_sb <= 0 || p.y_sb <= 0));
+}
+
+// About how long the two kernels take, in us: two launches, the contraction's
+// length, the 128-token tiles and their weights, and the tokens of a tile. Measured on a B200
+// (us, token form / two kernels): 12288 -> 4096, rank 16, 64 tokens: one request 7.2 /
+// 13.5, four 8.4 / 14.1, sixteen 22.4 / 21.8; 4096 -> 4096, rank 64: one 9.0 / 12.3,
+// four 13.7 / 12.9, eight 25.6 / 13.6; 4096 -> 12288, rank 128, one request: 16 tokens
+// 10.3 / 12.6, 64 18.0 / 14.8. Up to eight tokens the token form was never slower.
+float tiles_us(const Lora& p) {
+  const float tiles = float(int64_t(p.batch) * ((p.seq + 127) / 128));
+  return 8.0f + 3e-4f * p.in + tiles * (0.25f + 0.33f * (p.r_pad * 2e-6f * (float(p.in) + p.out))) +
+         0.027f * float(p.seq < 128 ? p.seq : 128);
 }
 
 }  // namespace
@@ -643,9 +699,11 @@ extern "C" int qia_lora_add(const void* x, const void* base, void* y, const void
   p.out = int(out_features);
   p.adapters = int(adapters);
   p.r_pad = int(r_pad);
-  if (use_tokens(batch, seq, p)) return launch_tokens(p, as_stream(stream));
+  const TokenPlan plan = plan_tokens(p);
+  if (seq <= kTokens || broadcast(p)) return launch_tokens(p, plan, as_stream(stream));
   if (!workspace || !aligned(workspace, 16))
     return set_error(QIA_ERR_INVALID, "%s: the workspace is null or misaligned", who);
+  if (plan.us <= tiles_us(p)) return launch_tokens(p, plan, as_stream(stream));
   // (a request that is alone needs no request stride: any value that a map takes)
   if (batch == 1) p.x_sb = p.base_sb = p.y_sb = 8;
   return launch_tiles(p, workspace, as_stream(stream));
