@@ -363,17 +363,27 @@ cached_attn_rows_kernel(const __grid_constant__ CachedAttn p) {
     const auto row_of = [&](int z, int key) {
       return z ? p.v + b * p.v_sb + int64_t(key) * p.v_ss + kvh * p.v_sh : p.k + b * p.k_sb + int64_t(key) * p.k_ss + kvh * p.k_sh;
     };
-    // lane j holds key j's scales: they are found first, row by row
+    // lane j holds key j's scales: they are found first, four rows at a time, eight
+    // lanes per row (a row at a time, sixteen fresh keys took 7 us)
     float up[2] = {1.0f, 1.0f}, inv[2] = {1.0f, 1.0f};
-    for (int j = 0; j < min(kRowsStep, p.sk - k0); ++j) {
-      if (!fresh_ok(k0 + j)) continue;
+#pragma unroll 1
+    for (int j0 = 0; j0 < min(kRowsStep, p.sk - k0); j0 += 4) {
+      const int key = k0 + j0 + (lane >> 3);
+      const bool held = fresh_ok(key);
+      uint4 x[2][2];
+#pragma unroll
+      for (int z = 0; z < 2; ++z)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          x[z][i] = held ? __ldg(reinterpret_cast<const uint4*>(row_of(z, key)) + 2 * (lane & 7) + i)
+                         : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        const uint2 x = __ldg(reinterpret_cast<const uint2*>(row_of(z, k0 + j)) + lane);
-        const uint32_t mx = absmax8(make_uint4(x.x, x.y, 0u, 0u), 0u);
-        float u, v;
-        pow2_scale(__reduce_max_sync(0xffffffffu, mx), u, v);
-        if (lane == j) up[z] = u, inv[z] = v;
+        uint32_t m = absmax8(x[z][1], absmax8(x[z][0], 0u));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        m = __shfl_sync(0xffffffffu, m, 8 * (lane & 3));
+        if (lane >> 2 == j0 >> 2) pow2_scale(m, up[z], inv[z]);
       }
     }
     float s[NT][2][4];
