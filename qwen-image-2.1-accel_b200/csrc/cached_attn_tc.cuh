@@ -280,9 +280,10 @@ __device__ __forceinline__ void weigh64(const uint32_t* s, float c, float n1, ui
 // has a positive score -- its maximum is then a key's that takes part -- they cost
 // one subtraction per tile (at most 128 times the largest weight: seven bits of
 // fp32). Otherwise their scores are set to -infinity (450 cycles a tile more).
-template <bool kHold>
+// begin() comes before the exponentials, end() after them.
+template <bool kHold, class Begin, class End>
 __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, const TileInfo* info, float q_up, bool fresh,
-                                             RowState& st, uint64_t* p_full, int lane) {
+                                             RowState& st, uint64_t* p_full, int lane, Begin&& begin, End&& end) {
   uint32_t s[kHold ? 128 : 64];
   bool drop = false;
   const auto load = [&](int h, uint32_t* dst) {       // 64 scores
@@ -352,10 +353,12 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, const T
   }
   const float n1 = f + kBias - (st.m == -INFINITY ? 0.0f : st.m);
   uint64_t sum[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+  begin();
 #pragma unroll(kHold ? 2 : 1)
   for (int h = 0; h < 2; ++h) {
     if constexpr (!kHold) reload(h);
     weigh64(kHold ? s + 64 * h : s, c, n1, sum, t_s + uint32_t(32 * h));
+    if (h == 1) end();
     tc_wait_st();
     tc_fence_before();
     __syncwarp();

@@ -432,7 +432,7 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
       if (!ok) break;
       tc_fence_after();
       softmax_tile<false>(t_s, t_o, reinterpret_cast<const TileInfo*>(smem + kSmemTail + (j % kInfoRing) * kInfoBytes), q_up,
-                   it == 0, st, &p_full[2 * w], lane);
+                   it == 0, st, &p_full[2 * w], lane, [] {}, [] {});
     }
     bool have = ok && count > 0;       // the accumulators hold something
     if (ok && n > 0) have = __all_sync(0xffffffffu, mbar_wait(smem_u32(o_full), 0, err)) && have;

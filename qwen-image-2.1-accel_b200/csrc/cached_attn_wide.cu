@@ -17,8 +17,20 @@
 // may rescale them (only when a row's maximum grew by more than 2^7; f16 weights
 // are at most 2^15).
 //
-// What bounds it: per key tile 4 x 512 tensor cycles and 2 x 1024 cycles of
-// exponentials per SM.
+// The warps of the two groups that share a scheduler take their exponentials in
+// turn: both at once, each runs at half the unit's rate and then both wait for the
+// tensor cores (4096 rows over 8325 keys, 32 heads: 559 us without turns, 530 to 547
+// with).
+//
+// What bounds it: the chain scores, softmax, weights, product of each query tile. Per
+// key tile and SM the tensor cores need 2050 cycles for both, the exponentials 2048;
+// a tile's softmax takes about 2050 and its next scores come some 1300 later (they
+// overwrite the weights, so Q.K has to wait for P.V). On a B200, 4096 rows over
+// 4229 + 4096 keys, 32 heads: 1.1 PFLOP/s after 37 us of widening. Measured and left
+// out: steps of 64 keys with two score buffers in the same columns (products of 64
+// keys read the queries twice as often, 777 cycles instead of 514 per 128 keys: 587 us
+// at best); an issuer per query tile (613 us without turns, 552 with); a third or a
+// quarter of the exponentials as cubics on the FMA pipes (580, 571 us).
 #include "cached_attn_tc.cuh"
 
 namespace qia {
@@ -159,7 +171,8 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
   uint64_t* o_full = bars + 18;
   uint64_t* drain = bars + 19;
   uint64_t* q_full = bars + 20;       // softmax -> issuer
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  uint64_t* turn = bars + 21;         // [2][4] warp k of group i takes its exponentials
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = int(cluster_size()), split = int(cluster_rank());
@@ -179,6 +192,7 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
     mbar_init(smem_u32(o_full), 1);
     mbar_init(smem_u32(drain), 1);
     mbar_init(smem_u32(q_full), 4 * n_tiles);
+    for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&turn[i]), 1);
     fence_barrier_init();
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
@@ -310,7 +324,14 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
       if (!ok) break;
       tc_fence_after();
       softmax_tile<true>(t_s, t_o, reinterpret_cast<const TileInfo*>(smem + kSmemTail + (j % kScalarRing) * kInfoBytes), q_up,
-                   j == 0, st, &p_full[2 * w], lane);
+                   j == 0, st, &p_full[2 * w], lane,
+                   [&] {      // (group 0 first: its first wait is for the phase before the first)
+                     if (n_tiles > 1)
+                       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&turn[4 * w + (warp & 3)]), (j & 1) ^ (w ^ 1), err));
+                   },
+                   [&] {
+                     if (n_tiles > 1 && lane == 0) mbar_arrive(smem_u32(&turn[4 * (w ^ 1) + (warp & 3)]));
+                   });
     }
     const bool have = ok && n > 0 && __all_sync(0xffffffffu, mbar_wait(smem_u32(o_full), 0, err));
     tc_fence_after();
