@@ -24,8 +24,14 @@
 // Warps take 32-key steps of the CTA's slice in turn, each with a running
 // maximum and sum of its own; the CTA joins its warps in shared memory and the
 // CTAs of a cluster (which split the keys) join through distributed shared
-// memory, in rank order: one launch, no workspace, results that do not depend
+// memory, in a fixed order: one launch, no workspace, results that do not depend
 // on timing.
+//
+// On a B200, sixteen requests of 4097 to 16391 tokens, 32 / 8 heads, one token: 73 us,
+// 5.8 TB/s (89 % of the copy's rate). 32 heads over 4229 tokens: 11 to 12 us for 35
+// MB, of them 4.5 us launch, query, one fresh key and joining; the rest is latency,
+// with seven warps per SM. (Clusters of up to sixteen, eight warps per CTA and five
+// CTAs per SM were slower.)
 #include "cached_attn.cuh"
 #include "cluster.cuh"
 
@@ -584,26 +590,26 @@ int run_rows(const CachedAttn& p, int batch, int splits, cudaStream_t st) {
                         sizeof(RowsSmem<8 * NT, DEPTH>), splits, st, p);
 }
 
-// With few groups the device is not full, and a warp's own depth hides the
-// latency (three CTAs per SM); with many, one more CTA per SM does it better. On a
-// B200 (us, deep / shallow): 32 heads of one request, one row, 16384 tokens 29.5 / 31.9,
-// 333 5.95 / 5.95; sixteen requests of 8 K/V heads, four rows: 4229 31.6 / 30.6, 333
-// 7.8 / 8.2; sixteen rows: 4229 47.6 / 44.8.
-template <int NT>
-int launch_rows(const CachedAttn& p, int batch, cudaStream_t st) {
+}  // namespace
+
+// Up to eight rows: with few groups the device is not full, and a warp's own depth
+// hides the latency (three CTAs per SM); with many, one more CTA per SM does it
+// better. On a B200 (us, deep / shallow): 32 heads of one request, one row, 16384
+// tokens 29.2 / 31.6, 333 5.4 / 5.5; sixteen requests of 8 K/V heads, four rows: 333
+// 7.6 / 8.1, 4229 31.1 / 30.8, 16384 96.2 / 94.7. More rows leave no registers for
+// depth (32 heads, sixteen rows: 1111 tokens 11.7 / 10.9, 16384 44.7 / 42.6).
+int launch_cached_rows(const CachedAttn& p, int batch, cudaStream_t st) {
   const int64_t groups = int64_t(p.kv_heads) * batch;
   const int steps = (p.extent + kRowsStep - 1) / kRowsStep + (p.sk + kRowsStep - 1) / kRowsStep;
   RowsPlan deep, wide;
-  int rc = plan_rows<NT, 2>(groups, steps, &deep);
-  if (!rc) rc = plan_rows<NT, 1>(groups, steps, &wide);
+  if (int64_t(p.sq) * p.share > 8) {
+    const int rc = plan_rows<2, 1>(groups, steps, &wide);
+    return rc ? rc : run_rows<2, 1>(p, batch, wide.splits, st);
+  }
+  int rc = plan_rows<1, 2>(groups, steps, &deep);
+  if (!rc) rc = plan_rows<1, 1>(groups, steps, &wide);
   if (rc) return rc;
-  return deep.cost <= wide.cost ? run_rows<NT, 2>(p, batch, deep.splits, st) : run_rows<NT, 1>(p, batch, wide.splits, st);
-}
-
-}  // namespace
-
-int launch_cached_rows(const CachedAttn& p, int batch, cudaStream_t st) {
-  return int64_t(p.sq) * p.share <= 8 ? launch_rows<1>(p, batch, st) : launch_rows<2>(p, batch, st);
+  return deep.cost <= wide.cost ? run_rows<1, 2>(p, batch, deep.splits, st) : run_rows<1, 1>(p, batch, wide.splits, st);
 }
 
 }  // namespace qia
@@ -611,9 +617,9 @@ int launch_cached_rows(const CachedAttn& p, int batch, cudaStream_t st) {
 using namespace qia;
 
 // The rows that share a K/V head fill one 16-row tile. On a B200 (us, this form / the
-// 128-row tiles): 32 heads, one request, one row: 333 tokens 6.0 / 13.5, 16384 29.5 /
-// 65.9; sixteen rows: 16 tokens 16.4 / 14.7, 1111 17.6 / 17.2, 16384 58.9 / 66.4; four
-// requests of sixteen rows: 16 17.4 / 15.2, 4229 60 / 71.
+// larger ones): 32 heads, one request, one row: 16 tokens 4.5 / 10.9, 333 5.4 / 13.0,
+// 16384 29.2 / 66; sixteen rows: 16 9.0 / 11.5, 1111 10.9 / 19.1, 16384 42.6 / 66; four
+// requests of sixteen rows: 16 9.7 / 15.1, 4229 44.8 / 71.
 static bool use_rows(int64_t seq_q, int64_t share) { return seq_q * share <= 16; }
 
 extern "C" int64_t qia_cached_attention_workspace_bytes(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t heads,

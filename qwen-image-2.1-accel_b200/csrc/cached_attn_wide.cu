@@ -385,11 +385,11 @@ int make_rows_map(CUtensorMap* map, const void* base, int64_t rows) {
 // query tiles per request and K/V head on, several CTAs would convert the same keys.
 // Up to two, widening costs its bytes (5 per code, against 1) and saves the CTA's
 // conversion, so it is for few keys: up to 320 key tiles in all. On a B200 (us, widened /
-// in place): 32 heads of one request, 256 rows: 16 + 256 keys
-// (96 tiles) 15.8 / 19.5, 1024 + 256 (320) 25.2 / 24.9, 4229 + 256 (1152) 49.9 / 44.0; 8 K/V heads,
-// 40 rows of four: 1024 (72) 16.9 / 19.7, 4229 (280) 26.5 / 30.6, 8192 (520) 36.5 / 39.0; 128 heads of
-// four requests, 77 rows: 128 (256) 15.2 / 15.3,
-// 512 (640) 24.0 / 21.3, 8192 (8320) 237 / 123.
+// in place): 32 heads of one request, 256 rows: 16 + 256 keys (96 tiles) 15.6 / 19.5,
+// 1024 + 256 (320) 25.0 / 24.9, 4229 + 256 (1152) 49.4 / 44.2; 8 K/V heads, 40 rows of
+// four: 1024 + 40 (72) 16.8 / 19.7, 4229 (280) 26.3 / 30.6, 8192 (520) 35.7 / 39.1; 128
+// heads of four requests, 77 rows: 128 + 77 (256) 15.1 / 15.3, 512 (640) 23.6 / 21.5,
+// 8192 (8320) 232 / 123.
 bool cached_use_wide(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t kv_heads, int64_t share, int64_t extent) {
   const int64_t per = kTileRows / share;
   return (seq_q + per - 1) / per > 2 ||

@@ -3,9 +3,9 @@
 The reference keeps the prefix's K/V in bf16 (QwenImage21KVLayerCache,
 transformer_qwenimage21.py:56-74). Here a cached row (one token of one head)
 is 128 INT8 codes and an fp32 scale: half the memory, and half the bytes an
-attention over it streams. `cached_attention` multiplies the codes as they are
-(they are exact in the tensor cores' 16-bit types) and applies the scales to
-the scores; `kv_cache_read` gives bf16 rows to an attention of another kind.
+attention over it streams. `cached_attention` multiplies the codes as f16 rows,
+exact or scaled by powers of two; `kv_cache_read` gives bf16 rows to an attention
+of another kind.
 """
 from __future__ import annotations
 
@@ -204,7 +204,7 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
         return out
     size = _lib.load().qia_cached_attention_workspace_bytes(cache.batch, shape[1], fresh, shape[2], cache.kv_heads,
                                                             cache.extent)
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    ws = q.new_empty(size >> 1) if size else None       # (bf16 elements)
     _lib.call("qia_cached_attention", q.data_ptr(), k.data_ptr() if fresh else None, v.data_ptr() if fresh else None,
               *cache._buffers, None if key_valid is None else key_valid.data_ptr(), out.data_ptr(), cache.batch,
               shape[1], fresh, shape[2], cache.kv_heads, HEAD_DIM, cache.capacity, cache.extent,
