@@ -607,11 +607,12 @@ int qia_kv_cache_read(const void* k_codes, const void* v_codes,
  * the cached tokens, then the fresh ones), or NULL. Masked keys do not count
  * whatever they hold; a query without keys writes zeros. strides: elements, of
  * q, k, v, out (batch, seq, head each; multiples of 8). sm_scale <= 0:
- * 1/sqrt(128). Products of exact INT8 codes (cached) or bf16 rows (fresh),
- * fp32 scores, sums and accumulators; softmax weights are rounded once for the
- * second product. head_dim = 128, heads / kv_heads <= 128. workspace:
- * qia_cached_attention_workspace_bytes bytes of device memory, 128-byte
- * aligned (NULL when that is 0). */
+ * 1/sqrt(128). The products' operands are f16: up to 16 query rows per K/V head
+ * the INT8 codes as they are, above that cached and fresh rows scaled by powers
+ * of two (one rounding to eleven bits); fp32 scores, sums and accumulators;
+ * softmax weights are rounded once for the second product. head_dim = 128,
+ * heads / kv_heads <= 128. workspace: qia_cached_attention_workspace_bytes bytes
+ * of device memory, 128-byte aligned (NULL when that is 0). */
 int qia_cached_attention(const void* q, const void* k, const void* v,
                          const void* k_codes, const void* v_codes,
                          const void* k_scales, const void* v_scales,
