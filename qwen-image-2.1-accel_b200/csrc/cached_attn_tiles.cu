@@ -122,28 +122,15 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
     mbar_arrive(smem_u32(&info_full[j % kInfoRing]));
   };
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&k_full[i]), kWriters);
-      mbar_init(smem_u32(&v_full[i]), kWriters);
-      mbar_init(smem_u32(&k_empty[i]), 1);
-      mbar_init(smem_u32(&v_empty[i]), 1);
-      mbar_init(smem_u32(&s_full[i]), 1);
-    }
-    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&p_full[i]), 4);
-    for (int i = 0; i < kInfoRing; ++i) mbar_init(smem_u32(&info_full[i]), 2);
-    mbar_init(smem_u32(o_full), 1);
-    mbar_init(smem_u32(drain), 1);
-    mbar_init(smem_u32(fresh_done), 2);
-    mbar_init(smem_u32(q_full), 8);
-    for (int i = 0; i < kDuoUnits; ++i) {
-      mbar_init(smem_u32(&stage_full[i]), 1);
-      mbar_init(smem_u32(&stage_empty[i]), kWriters);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&factor_full[i]), 1);
-      mbar_init(smem_u32(&factor_empty[i]), 2 * kWriters);
-    }
+  // a barrier per thread (one thread for all of them took a microsecond)
+  if (threadIdx.x < 48) {
+    const int i = threadIdx.x;
+    const int arrivals = i < 4 || (i >= 28 && i < 35) || i == 20 ? kWriters      // k_full, v_full, stage_empty; q_full
+                         : i >= 14 && i < 18                     ? 4             // p_full
+                         : i == 37 || i == 38                    ? 2 * kWriters  // factor_empty
+                         : i >= 39                               ? 2             // fresh_done, info_full
+                                                                 : 1;
+    mbar_init(smem_u32(&bars[i]), uint32_t(arrivals));
     fence_barrier_init();
   }
   if (warp == 24) tmem_alloc(smem_u32(tmem_slot), 512);
