@@ -22,8 +22,8 @@
 // lora_shrink_kernel + lora_expand_kernel: many tokens per request, on tcgen05.
 // Both are bound by the bytes of x and of base and y, so a CTA is a stream of
 // TMA tiles with as much in flight as fits, and the products hide behind it (four
-// requests of 4096 tokens, 4096 -> 12288, rank 64: 170 us, 85 % of the copy's rate:
-// shrink 31 us, its bytes 21; expand 139, its bytes 123):
+// requests of 4096 tokens, 4096 -> 12288, rank 64: 168 us, 86 % of the copy's rate:
+// shrink 31 us, its bytes 21; expand the rest, its bytes 123):
 //   shrink  t = scale_i A_i x for 128 tokens, the contraction split over a
 //           cluster until the CTAs fill the device; partial sums are added
 //           through distributed shared memory in rank order; t is rounded to
@@ -356,11 +356,16 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
       int st = 0, issued = 0;
       uint32_t phase = 0;
       bool ok = true;
+      // x is read once: above 16 MB (an eighth of L2) it leaves L2 first, so that base
+      // and y stay. On a B200 (us, as usual / first): 4096 tokens of 12288 channels (101 MB)
+      // 40.6 / 36.9, of 4096 (34 MB) 29.0 / 27.7; 666 of 12288 (16 MB) 15.5 / 15.9, 800 of
+      // 4096 (7 MB) 15.5 / 16.0.
+      const uint64_t policy = l2_policy(int64_t(p.batch) * p.seq * p.in * 2 > (16 << 20));
       for (int i = 0; i < count; ++i) {
         if (!mbar_wait(smem_u32(&empty[st]), phase ^ 1, err)) { ok = false; break; }
         const uint32_t dst = smem_u32(smem + st * stage_bytes), bar = smem_u32(&full[st]);
         mbar_arrive_expect_tx(bar, uint32_t(kShrinkX + n * 128));
-        tma_load_3d(dst, &tm_x, bar, (first + i) * 64, s0, b);
+        tma_load_3d(dst, &tm_x, bar, (first + i) * 64, s0, b, policy);
         tma_load_3d(dst + kShrinkX, &tm_a, bar, (first + i) * 64, 0, id);
         ++issued;
         if (++st == stages) { st = 0; phase ^= 1; }
