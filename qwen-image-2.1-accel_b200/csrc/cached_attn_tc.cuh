@@ -366,7 +366,10 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, const T
   }
   float a, b;
   f2_unpack(f2_add(sum[0], sum[1]), a, b);
-  st.l = fmaf(fmaf(-missing, ex2_ftz(n1), a + b), num.z, st.l);
+  a += b;
+  // (only there: 2^n1 is at most 2^15 beside a positive score, infinite far below zero)
+  if (missing > 0.0f) a = fmaf(-missing, ex2_ftz(n1), a);
+  st.l = fmaf(a, num.z, st.l);
 }
 
 // A softmax warp's 32 rows of accumulators (a row per thread, 128 TMEM columns from

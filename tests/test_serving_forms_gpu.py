@@ -135,3 +135,25 @@ def test_adapter_forms_vs_64_bits(b, s, width, out, ranks, ids):
     again = base.clone()
     assert lora_add(x, again, w, idt, out=again) is again       # in place, the same bits
     assert torch.equal(again, got)
+
+
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("sq,kvh,length,fresh", [(1, 2, 40, 3), (12, 2, 0, 1), (50, 2, 1, 1), (300, 2, 150, 70),
+                                                 (40, 64, 700, 5), (150, 64, 700, 0)])
+def test_scores_of_one_sign_far_from_zero(sq, kvh, length, fresh, masked, sign):
+    """Every key scores the same, some 900 below or above zero: the output is
+    the mean of V, and no power of two of a maximum may reach the sums."""
+    from qwen_image_accel_b200.kernels.kv_cache import cached_attention
+    g = gen(24)
+    cache = make_cache(g, 2, kvh, max(length, 1) + 3, [length, 0 if fresh else length])
+    cache.k_codes.fill_(-127 if sign < 0 else 127)
+    cache.k_scales.fill_(40.0 / 127)
+    q = torch.full((2, sq, kvh, 128), 2.0, dtype=torch.bfloat16, device=DEV)
+    k, v = (torch.full((2, fresh, kvh, 128), sign * 40.0, dtype=torch.bfloat16, device=DEV),
+            rows(g, 2, fresh, kvh, 128)) if fresh else (None, None)
+    valid = None
+    if masked:
+        valid = torch.rand(2, cache.extent + fresh, device=DEV, generator=g) < 0.5
+        valid[:, -1] = True
+    assert_attention(cached_attention(q, cache, k, v, key_valid=valid), *attention64(q, cache, k, v, valid))
