@@ -159,15 +159,15 @@ inline TileGrid tile_grid(const CachedAttn& p) {
 }
 
 // A query tile into shared memory as f16, each row scaled by a power of two 2^e_i
-// (rows past the end are zeros), by THREADS threads (`t`; sixteen per row); 2^e_i
-// into scale[128]. Announced on q_full by every warp. The rows arrive where they
-// will stay, all in flight at once, and are converted in place, in short loops
-// (with the rows in registers and everything unrolled, a first CTA spent up to
-// 16000 cycles here, most of them waiting for its own instructions; now 5000 to
-// 9000, about 3400 of them the loads).
+// (rows past the end are zeros), by THREADS threads (`t`; sixteen per row), in two
+// steps: fetch_queries asks for the rows where they will stay, all at once, before
+// the block's barriers and TMEM are set up; convert_queries converts them in place,
+// with 2^e_i into scale[128], and announces them on q_full by every warp. Both are
+// short loops (with the rows in registers and everything unrolled, a first CTA spent
+// up to 16000 cycles here, most of them waiting for its own instructions).
 template <int THREADS>
-__device__ __forceinline__ void load_queries(const CachedAttn& p, const TileGrid& g, uint32_t slot, float* scale, int tile,
-                                             int t, int kvh, int b, uint64_t* q_full) {
+__device__ __forceinline__ void fetch_queries(const CachedAttn& p, const TileGrid& g, uint32_t slot, int tile, int t,
+                                              int kvh, int b) {
   constexpr int kRows = THREADS / 16, kLoads = kTileRows / kRows;
   static_assert(kRows % 8 == 0, "the swizzle of a thread's rows is the same");
   const int tile_rows = g.tokens_per_tile * p.share, row0 = t >> 4, piece = t & 15;
@@ -183,6 +183,13 @@ __device__ __forceinline__ void load_queries(const CachedAttn& p, const TileGrid
                  "r"(held ? 16 : 0)
                  : "memory");
   }
+}
+
+template <int THREADS>
+__device__ __forceinline__ void convert_queries(uint32_t slot, float* scale, int t, uint64_t* q_full) {
+  constexpr int kRows = THREADS / 16, kLoads = kTileRows / kRows;
+  const int row0 = t >> 4, piece = t & 15;
+  const uint32_t at = slot + tile_offset(row0, piece);
   asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
   for (int i = 0; i < kLoads; i += 8) {

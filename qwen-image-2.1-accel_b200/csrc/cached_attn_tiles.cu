@@ -122,9 +122,13 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
     mbar_arrive(smem_u32(&info_full[j % kInfoRing]));
   };
 
+  if (warp < 8) {
+    if (duo) fetch_queries<256>(p, tp, sbase + kSmemQ, 2 * pair, threadIdx.x, kvh, b);
+    else fetch_queries<128>(p, tp, sbase + kSmemQ + (warp >> 2) * kTileBytes, 2 * pair + (warp >> 2), threadIdx.x & 127, kvh, b);
+  }
   // a barrier per thread (one thread for all of them took a microsecond)
-  if (threadIdx.x < 48) {
-    const int i = threadIdx.x;
+  if (threadIdx.x >= 256 && threadIdx.x < 256 + 48) {
+    const int i = threadIdx.x - 256;
     const int arrivals = i < 4 || (i >= 28 && i < 35) || i == 20 ? kWriters      // k_full, v_full, stage_empty; q_full
                          : i >= 14 && i < 18                     ? 4             // p_full
                          : i == 37 || i == 38                    ? 2 * kWriters  // factor_empty
@@ -405,8 +409,8 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
     const uint32_t t_s = tmem + t_lane + uint32_t(128 * w), t_o = tmem + t_lane + uint32_t(256 + 128 * w);
     const int q_tile = duo ? 0 : w;
     float* scale = reinterpret_cast<float*>(smem + kSmemQScale) + q_tile * kTileRows;
-    if (duo) load_queries<256>(p, tp, sbase + kSmemQ, scale, 2 * pair, threadIdx.x, kvh, b, q_full);
-    else load_queries<128>(p, tp, sbase + kSmemQ + w * kTileBytes, scale, 2 * pair + w, threadIdx.x & 127, kvh, b, q_full);
+    if (duo) convert_queries<256>(sbase + kSmemQ, scale, threadIdx.x, q_full);
+    else convert_queries<128>(sbase + kSmemQ + w * kTileBytes, scale, threadIdx.x & 127, q_full);
     asm volatile("bar.sync 2, 256;" ::: "memory");       // (the rows' scales)
     const float q_up = scale[row];
     const int count = duo ? (n - w + 1) / 2 : n;       // key tiles of this group

@@ -185,7 +185,9 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
   const int per = (all_tiles + splits - 1) / splits;
   const int first = min(all_tiles, split * per), n = min(all_tiles, first + per) - first;   // this CTA's key tiles
 
-  if (threadIdx.x == 0) {
+  if (warp < 4 * n_tiles)
+    fetch_queries<128>(p, tp, sbase + kSmemQ + (warp >> 2) * kTileBytes, 2 * pair + (warp >> 2), threadIdx.x & 127, kvh, b);
+  if (threadIdx.x == 256) {
     for (int i = 0; i < 12; ++i) mbar_init(smem_u32(&bars[i]), 1);
     for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&s_full[i]), 1);
     for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&p_full[i]), 4);
@@ -197,7 +199,7 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
   }
-  if (warp == 8) tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == 9) tmem_alloc(smem_u32(tmem_slot), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -313,7 +315,7 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
     const uint32_t t_s = tmem + t_lane + uint32_t(128 * w), t_o = tmem + t_lane + uint32_t(256 + 128 * w);
     float* scale = reinterpret_cast<float*>(smem + kSmemQScale) + w * kTileRows;
     if (w < n_tiles)
-      load_queries<128>(p, tp, sbase + kSmemQ + w * kTileBytes, scale, 2 * pair + w, threadIdx.x & 127, kvh, b, q_full);
+      convert_queries<128>(sbase + kSmemQ + w * kTileBytes, scale, threadIdx.x & 127, q_full);
     bool ok = w < n_tiles;
     if (ok) asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");   // (the rows' scales)
     const float q_up = scale[row];
@@ -344,7 +346,7 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
