@@ -612,7 +612,8 @@ int qia_kv_cache_read(const void* k_codes, const void* v_codes,
  * of two (one rounding to eleven bits); fp32 scores, sums and accumulators;
  * softmax weights are rounded once for the second product. head_dim = 128,
  * heads / kv_heads <= 128. workspace: qia_cached_attention_workspace_bytes bytes
- * of device memory, 128-byte aligned (NULL when that is 0). */
+ * of device memory, 128-byte aligned (NULL when that is 0, as it is up to 16
+ * query rows per K/V head). */
 int qia_cached_attention(const void* q, const void* k, const void* v,
                          const void* k_codes, const void* v_codes,
                          const void* k_scales, const void* v_scales,
@@ -640,7 +641,7 @@ int64_t qia_cached_attention_workspace_bytes(int64_t batch, int64_t seq_q,
  * ranks[i] hold zeros. ranks, ids: int32, scales: f32, device memory. in,
  * out and r_pad multiples of 8, r_pad <= 128. workspace:
  * qia_lora_workspace_bytes bytes of device memory, 16-byte aligned (NULL when
- * that is 0). */
+ * that is 0, as it is for seq <= 8). */
 int qia_lora_add(const void* x, const void* base, void* y, const void* a,
                  const void* b, const void* ranks, const void* scales,
                  const void* ids, int64_t batch, int64_t seq,

@@ -202,8 +202,10 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
         raise ValueError(f"{who}: out must be like q")
     if not out.numel():
         return out
-    size = _lib.load().qia_cached_attention_workspace_bytes(cache.batch, shape[1], fresh, shape[2], cache.kv_heads,
-                                                            cache.extent)
+    size = 0
+    if shape[1] * shape[2] > 16 * cache.kv_heads:       # (up to 16 rows per K/V head need none)
+        size = _lib.load().qia_cached_attention_workspace_bytes(cache.batch, shape[1], fresh, shape[2], cache.kv_heads,
+                                                                cache.extent)
     ws = q.new_empty(size >> 1) if size else None       # (bf16 elements)
     _lib.call("qia_cached_attention", q.data_ptr(), k.data_ptr() if fresh else None, v.data_ptr() if fresh else None,
               *cache._buffers, None if key_valid is None else key_valid.data_ptr(), out.data_ptr(), cache.batch,

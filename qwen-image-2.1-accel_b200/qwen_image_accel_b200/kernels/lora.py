@@ -83,6 +83,7 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
     index = weights._index
     if x.get_device() != index or base.get_device() != index or ids.get_device() != index or out.get_device() != index:
         raise ValueError(f"{who}: the adapters are on {weights.device}, x, base, ids or out are not")
+    # (up to eight tokens per request need none)
     size = _lib.load().qia_lora_workspace_bytes(batch, seq, weights.r_pad) if seq > 8 else 0
     ws = x.new_empty(size >> 1) if size else None       # (bf16 elements)
     _lib.call("qia_lora_add", x.data_ptr(), base.data_ptr(), out.data_ptr(), *weights._buffers, ids.data_ptr(), batch,
