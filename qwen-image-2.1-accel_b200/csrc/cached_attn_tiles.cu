@@ -55,8 +55,13 @@ constexpr int kSmemML = kSmemQScale + 256 * 4;                      // m, l of 2
 constexpr int kSmemFactor = kSmemML + 2 * 256 * 4;                  // [2 tiles][K, V][128] scale 2^-e of a tile's keys
 constexpr int kSmemSlots = kSmemFactor + 2 * 256 * 4;               // [2 tiles][K, V][writer] maxima
 constexpr int kSmemBars = kSmemSlots + 2 * 2 * kWriters * 4;
-constexpr int kSmemStage = kSmemBars + 384;                         // codes in flight
+constexpr int kBars = 48;
+// the TMEM address, read after the setup barrier: nothing that is written from then
+// on (the codes in flight) may share its bytes
+constexpr int kSmemTmem = kSmemBars + kBars * 8;
+constexpr int kSmemStage = kSmemTmem + 128;                         // codes in flight
 constexpr int kSmemBytes = kSmemStage + kUnits * kUnitBytes + 1024;
+static_assert(kSmemTmem + 4 <= kSmemStage, "the TMEM address has a place of its own");
 static_assert(kSmemStage % 16 == 0 && kSmemBytes <= 227 * 1024, "shared memory");
 // registers of a softmax thread, a writer and any other: 256 x 112 + 512 x 56 + 128 x 48 = 63488 of the
 // 896 x 72 that the block starts with
@@ -84,7 +89,7 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
   uint64_t* factor_full = bars + 35;  // [2] factors of tile j % 2
   uint64_t* factor_empty = bars + 37; // [2]
   uint64_t* fresh_done = bars + 39;   // K and V writers are past the fresh tiles
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 48);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kSmemTmem);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = int(cluster_size()), split = int(cluster_rank());
@@ -127,7 +132,7 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
     else fetch_queries<128>(p, tp, sbase + kSmemQ + (warp >> 2) * kTileBytes, 2 * pair + (warp >> 2), threadIdx.x & 127, kvh, b);
   }
   // a barrier per thread (one thread for all of them took a microsecond)
-  if (threadIdx.x >= 256 && threadIdx.x < 256 + 48) {
+  if (threadIdx.x >= 256 && threadIdx.x < 256 + kBars) {
     const int i = threadIdx.x - 256;
     const int arrivals = i < 4 || (i >= 28 && i < 35) || i == 20 ? kWriters      // k_full, v_full, stage_empty; q_full
                          : i >= 14 && i < 18                     ? 4             // p_full

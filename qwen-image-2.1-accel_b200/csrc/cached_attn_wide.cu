@@ -40,7 +40,10 @@ constexpr int kThreads = 384;
 constexpr int kSmemQScale = kSmemTail + kScalarRing * kInfoBytes;   // 2^e_i of 256 rows
 constexpr int kSmemML = kSmemQScale + 256 * 4;                      // m, l of 256 rows (joining)
 constexpr int kSmemBars = kSmemML + 2 * 256 * 4;
+constexpr int kBars = 29;
+constexpr int kSmemTmem = kSmemBars + kBars * 8;                    // the TMEM address
 constexpr int kSmemBytes = kSmemBars + 256 + 1024;
+static_assert(kSmemTmem + 4 <= kSmemBars + 256 && kSmemBytes <= 227 * 1024, "shared memory");
 // registers of a softmax thread and of any other: 256 x 208 + 128 x 88 = 384 x 168, what the block starts with
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 struct Widened {
@@ -172,7 +175,7 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
   uint64_t* drain = bars + 19;
   uint64_t* q_full = bars + 20;       // softmax -> issuer
   uint64_t* turn = bars + 21;         // [2][4] warp k of group i takes its exponentials
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kSmemTmem);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = int(cluster_size()), split = int(cluster_rank());

@@ -306,6 +306,7 @@ __host__ __device__ constexpr int shrink_stages(int r_pad) {
   return 110 * 1024 / shrink_stage(r_pad) < 6 ? 110 * 1024 / shrink_stage(r_pad) : 6;
 }
 __host__ __device__ constexpr int shrink_smem(int r_pad) { return shrink_stages(r_pad) * shrink_stage(r_pad) + 256 + 1024; }
+static_assert((2 * 6 + 2) * 8 + 4 <= 256, "barriers of six stages and the TMEM address");
 static_assert(shrink_sums(kLoraMaxRank) <= shrink_stages(kLoraMaxRank) * shrink_stage(kLoraMaxRank) &&
                   shrink_sums(64) <= shrink_stages(64) * shrink_stage(64),
               "the sums reuse the stages");
@@ -449,6 +450,7 @@ constexpr int kExpandN = 128;
 constexpr int kExpandBase = 128 * kExpandN * 2;         // 32 KB: two 64-output panels
 __host__ __device__ constexpr int expand_panels(int r_pad) { return (r_pad + 63) / 64; }
 __host__ __device__ constexpr int expand_smem(int r_pad) { return kExpandBase + expand_panels(r_pad) * 32768 + 128 + 1024; }
+static_assert(5 * 8 + 4 <= 128, "barriers and the TMEM address");
 
 // grid (output tiles, token tiles, requests), 160 threads: warps 0-3 epilogue, 4 TMA and MMA
 __global__ void __launch_bounds__(160)
