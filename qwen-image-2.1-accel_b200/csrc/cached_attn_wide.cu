@@ -277,11 +277,14 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
         commit(drain);
         mbar_wait(smem_u32(drain), 0, ok ? err : nullptr, 100000000ull);
       }
-    } else if (warp == 9 && lane == 0 && n > 0) {
+    } else if (warp == 9 && lane == 0) {
       // ---------------------------------------------------------- TMA producer
       const int64_t bh = int64_t(b) * p.kv_heads + kvh;
       bool ok = true;
-      grid_wait();                           // the keys are widened
+      // the keys are widened. A CTA without key tiles waits too: this grid may not end
+      // before the one it depends on, since a launch of the remaining groups is
+      // ordered behind this grid alone
+      grid_wait();
       int issued = 0;
       for (int u = 0; u < 2 * n && ok; ++u) {
         const int j = u >> 1, st = j & 1;

@@ -1,0 +1,36 @@
+"""Calls of the serving operators that once answered wrongly, against plain
+64-bit code (bounds as in the operators' own tests unless stated)."""
+import pytest
+import torch
+
+from test_kv_cache_gpu import assert_attention, attention64, gen, make_cache, rows
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+
+
+# ------------------------------------------------------------- widened keys, more than one wave
+@pytest.mark.parametrize("b,h,lengths,sq,fresh", [
+    (20, 4, [0] * 19 + [5000], 300, 0),           # the whole first wave has no key at all
+    (20, 4, [0] * 18 + [1, 5000], 300, 0),
+    (1, 80, [900], 300, 0), (5, 16, [700, 0, 3, 129, 1300], 500, 40),
+])
+def test_the_groups_left_over_see_widened_keys(b, h, lengths, sq, fresh):
+    """160 groups of query tiles: a full wave, and twelve whose keys are split
+    in a launch of their own. The workspace holds NaN before each call."""
+    from qwen_image_accel_b200.kernels.kv_cache import cached_attention
+    g = gen(31)
+    cache = make_cache(g, b, h, max(lengths) + 3, lengths)
+    q = rows(g, b, sq, h, 128)
+    k, v = (rows(g, b, fresh, h, 128) for _ in range(2)) if fresh else (None, None)
+    ref = attention64(q, cache, k, v, None)
+    for _ in range(3):
+        junk = torch.full((1 << 28,), float("nan"), dtype=torch.bfloat16, device=DEV)
+        del junk                                  # (the allocator hands its memory to the workspace)
+        assert_attention(cached_attention(q, cache, k, v), *ref)
