@@ -27,9 +27,12 @@ class QuantizedKV:
 
     k_codes, v_codes: int8 [batch, kv_heads, capacity, 128]; k_scales,
     v_scales: float32 [batch, kv_heads, capacity]; lengths: int32 [batch] on
-    the device, the tokens each request holds. `extent` is the longest
-    request's length as the host knows it (the key columns of a mask); writes
-    through this class keep it up to date."""
+    the device, the tokens each request holds. The host counts them too, in one
+    list that a cache shares with its parts (select), so that a write through any
+    of them is known to all; `extent` is the longest request's count (the key
+    columns of a mask). What the host cannot count is set: `cache.extent = n`
+    says that each of its requests holds up to n tokens, e.g. the most that
+    replays of a captured append may reach."""
 
     def __init__(self, batch: int, kv_heads: int, capacity: int, device="cuda"):
         dev = torch.device(device)
@@ -39,17 +42,17 @@ class QuantizedKV:
                    torch.zeros(shape, dtype=torch.float32, device=dev),
                    torch.zeros(shape, dtype=torch.float32, device=dev),
                    torch.zeros(batch, dtype=torch.int32, device=dev),
-                   torch.zeros(batch, dtype=torch.int32, device=dev), 0, None)
+                   torch.zeros(batch, dtype=torch.int32, device=dev), 0)
 
     @classmethod
     def from_tensors(cls, k_codes, v_codes, k_scales, v_scales, lengths, extent: int) -> "QuantizedKV":
         """A cache around tensors of the class's layout (contiguous); no
         entry of `lengths` may exceed `extent`."""
         self = cls.__new__(cls)
-        self._bind(k_codes, v_codes, k_scales, v_scales, lengths, torch.zeros_like(lengths), int(extent), None)
+        self._bind(k_codes, v_codes, k_scales, v_scales, lengths, torch.zeros_like(lengths), int(extent))
         return self
 
-    def _bind(self, k_codes, v_codes, k_scales, v_scales, lengths, tickets, extent, parent):
+    def _bind(self, k_codes, v_codes, k_scales, v_scales, lengths, tickets, extent, held=None, first=0):
         _lib.require_cuda(k_codes, v_codes, k_scales, v_scales, lengths)
         if k_codes.ndim != 4 or k_codes.shape[-1] != HEAD_DIM:
             raise ValueError(f"QuantizedKV: codes must be [batch, kv_heads, capacity, 128], got {tuple(k_codes.shape)}")
@@ -63,8 +66,9 @@ class QuantizedKV:
         if not 0 <= extent <= capacity:
             raise ValueError(f"QuantizedKV: extent {extent} of capacity {capacity}")
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
-        self.lengths, self._tickets, self._parent = lengths, tickets, parent
-        self.batch, self.kv_heads, self.capacity, self.extent = batch, heads, capacity, extent
+        self.lengths, self._tickets = lengths, tickets
+        self.batch, self.kv_heads, self.capacity = batch, heads, capacity
+        self._held, self._first = [extent] * batch if held is None else held, first
         self.device, self._index = k_codes.device, k_codes.get_device()
         # the buffers' addresses, for the calls below
         self._buffers = tuple(t.data_ptr() for t in (k_codes, v_codes, k_scales, v_scales, lengths))
@@ -73,20 +77,23 @@ class QuantizedKV:
 
     def select(self, first: int, count: int = 1) -> "QuantizedKV":
         """Requests [first, first + count) of this cache, sharing its memory
-        (prefixes of different lengths are written one request at a time)."""
+        (prefixes of different lengths are written one request at a time). Its
+        extent is that of the requests it covers."""
         if first < 0 or count <= 0 or first + count > self.batch:
             raise ValueError(f"QuantizedKV.select: requests {first}+{count} of {self.batch}")
         part = QuantizedKV.__new__(QuantizedKV)
         s = slice(first, first + count)
         part._bind(self.k_codes[s], self.v_codes[s], self.k_scales[s], self.v_scales[s], self.lengths[s],
-                   self._tickets[s], self.extent, self)
+                   self._tickets[s], 0, self._held, self._first + first)
         return part
 
-    def _grow(self, extent: int, whole: bool) -> None:
-        """Record that requests hold up to `extent` tokens; `whole`: exactly so."""
-        self.extent = extent if whole else max(self.extent, extent)
-        if self._parent is not None:
-            self._parent._grow(extent, False)
+    @property
+    def extent(self) -> int:
+        return max(self._held[self._first:self._first + self.batch], default=0)
+
+    @extent.setter
+    def extent(self, tokens: int) -> None:
+        self._held[self._first:self._first + self.batch] = [tokens] * self.batch
 
 
 def _check_rows(who: str, cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -110,7 +117,7 @@ def kv_cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, start: 
     if start < 0 or start + seq > cache.capacity:
         raise ValueError(f"kv_cache_write: tokens {start}+{seq} of capacity {cache.capacity}")
     _write(cache, k, v, seq, start)
-    cache._grow(start + seq, True)
+    cache.extent = start + seq
 
 
 def kv_cache_append(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -118,10 +125,12 @@ def kv_cache_append(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> Non
     on the device, so a captured append replays)."""
     _check_rows("kv_cache_append", cache, k, v)
     seq = k.shape[1]
-    if cache.extent + seq > cache.capacity:
-        raise ValueError(f"kv_cache_append: {seq} tokens behind {cache.extent} of capacity {cache.capacity}")
+    extent = cache.extent
+    if extent + seq > cache.capacity:
+        raise ValueError(f"kv_cache_append: {seq} tokens behind {extent} of capacity {cache.capacity}")
     _write(cache, k, v, seq, -1)
-    cache._grow(cache.extent + seq, False)
+    for i in range(cache._first, cache._first + cache.batch):
+        cache._held[i] += seq
 
 
 def _write(cache, k, v, seq, start):
@@ -184,14 +193,14 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
         raise ValueError(f"{who}: scale={scale} must be positive")
     if (k is None) != (v is None):
         raise ValueError(f"{who}: k and v come together")
-    fresh, rows = 0, _NO_ROWS
+    extent, fresh, rows = cache.extent, 0, _NO_ROWS
     if k is not None:
         _check_rows(who, cache, k, v)
         fresh, rows = k.shape[1], k.stride()[:3] + v.stride()[:3]
     mask_stride = 0
     if key_valid is not None:
-        if key_valid.shape != (cache.batch, cache.extent + fresh) or key_valid.dtype != torch.bool:
-            raise ValueError(f"{who}: key_valid must be bool [{cache.batch}, {cache.extent + fresh}], got "
+        if key_valid.shape != (cache.batch, extent + fresh) or key_valid.dtype != torch.bool:
+            raise ValueError(f"{who}: key_valid must be bool [{cache.batch}, {extent + fresh}], got "
                              f"{key_valid.dtype} {tuple(key_valid.shape)}")
         if key_valid.stride(1) != 1 or key_valid.get_device() != cache._index:
             raise NotImplementedError(f"{who}: key_valid must have contiguous rows on the cache's device")
@@ -205,11 +214,11 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
     size = 0
     if shape[1] * shape[2] > 16 * cache.kv_heads:       # (up to 16 rows per K/V head need none)
         size = _lib.load().qia_cached_attention_workspace_bytes(cache.batch, shape[1], fresh, shape[2], cache.kv_heads,
-                                                                cache.extent)
+                                                                extent)
     ws = q.new_empty(size >> 1) if size else None       # (bf16 elements)
     _lib.call("qia_cached_attention", q.data_ptr(), k.data_ptr() if fresh else None, v.data_ptr() if fresh else None,
               *cache._buffers, None if key_valid is None else key_valid.data_ptr(), out.data_ptr(), cache.batch,
-              shape[1], fresh, shape[2], cache.kv_heads, HEAD_DIM, cache.capacity, cache.extent,
+              shape[1], fresh, shape[2], cache.kv_heads, HEAD_DIM, cache.capacity, extent,
               _strides12(*q_strides[:3], *rows, *out.stride()[:3]), mask_stride, 0.0 if scale is None else float(scale),
               None if ws is None else ws.data_ptr(), _lib.raw_stream(cache._index))
     return out

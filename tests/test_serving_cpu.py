@@ -1,0 +1,50 @@
+"""Host logic of the serving operators (no GPU: the launches are stubbed)."""
+import pytest
+import torch
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """kernels.kv_cache with CPU tensors and launches that do nothing."""
+    from qwen_image_accel_b200 import _lib
+    from qwen_image_accel_b200.kernels import kv_cache
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(_lib, "raw_stream", lambda index: 0)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: None)
+    return kv_cache
+
+
+def rows(batch, seq):
+    return torch.zeros(batch, seq, 2, 128, dtype=torch.bfloat16)
+
+
+def test_extent_is_shared_by_a_cache_and_its_parts(host):
+    cache = host.QuantizedKV(3, 2, 32, device="cpu")
+    first, pair, again = cache.select(0), cache.select(1, 2), cache.select(1, 2).select(0)
+    host.kv_cache_write(cache, rows(3, 10), rows(3, 10))
+    assert [c.extent for c in (cache, first, pair, again)] == [10, 10, 10, 10]
+    host.kv_cache_append(pair, rows(2, 5), rows(2, 5))
+    assert [c.extent for c in (cache, first, pair, again)] == [15, 10, 15, 15]
+    host.kv_cache_append(again, rows(1, 2), rows(1, 2))
+    assert [c.extent for c in (cache, first, pair, again, cache.select(2))] == [17, 10, 17, 17, 15]
+    with pytest.raises(ValueError, match="behind 17"):
+        host.kv_cache_append(cache, rows(3, 16), rows(3, 16))
+
+
+def test_extent_falls_when_every_longer_request_is_written_again(host):
+    cache = host.QuantizedKV(2, 2, 32, device="cpu")
+    host.kv_cache_write(cache, rows(2, 30), rows(2, 30))
+    for i, n in enumerate((4, 6)):
+        host.kv_cache_write(cache.select(i), rows(1, n), rows(1, n))
+    assert cache.extent == 6
+    host.kv_cache_append(cache, rows(2, 26), rows(2, 26))           # there is room
+    assert cache.extent == 32 and cache.select(0).extent == 30
+
+
+def test_extent_can_be_set_for_what_the_host_does_not_count(host):
+    cache = host.QuantizedKV(2, 2, 32, device="cpu")
+    part = cache.select(1)
+    cache.extent = 20
+    assert part.extent == 20
+    part.extent = 3
+    assert cache.extent == 20 and part.extent == 3

@@ -34,3 +34,22 @@ def test_the_groups_left_over_see_widened_keys(b, h, lengths, sq, fresh):
         junk = torch.full((1 << 28,), float("nan"), dtype=torch.bfloat16, device=DEV)
         del junk                                  # (the allocator hands its memory to the workspace)
         assert_attention(cached_attention(q, cache, k, v), *ref)
+
+
+# ------------------------------------------------------------- parts of a cache held across writes
+@pytest.mark.parametrize("sq", [1, 30, 300])
+def test_a_held_part_sees_writes_through_its_parent_and_through_other_parts(sq):
+    from qwen_image_accel_b200.kernels.kv_cache import (QuantizedKV, cached_attention, kv_cache_append, kv_cache_read,
+                                                        kv_cache_write)
+    g = gen(32)
+    cache = QuantizedKV(3, 2, 200)
+    part, other = cache.select(1), cache.select(1, 2)
+    kv_cache_write(cache, rows(g, 3, 90, 2, 128), rows(g, 3, 90, 2, 128))
+    kv_cache_append(other, rows(g, 2, 45, 2, 128), rows(g, 2, 45, 2, 128))
+    assert part.lengths.tolist() == [135] and kv_cache_read(part)[0].shape[1] == 135
+    q = rows(g, 1, sq, 2, 128)
+    assert_attention(cached_attention(q, part), *attention64(q, part, None, None, None))
+    kv_cache_append(part, rows(g, 1, 1, 2, 128), rows(g, 1, 1, 2, 128))
+    q = rows(g, 2, sq, 2, 128)
+    assert other.lengths.tolist() == [136, 135]
+    assert_attention(cached_attention(q, other), *attention64(q, other, None, None, None))
