@@ -389,7 +389,10 @@ cached_attn_rows_kernel(const __grid_constant__ CachedAttn p) {
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         m = __shfl_sync(0xffffffffu, m, 8 * (lane & 3));
-        if (lane >> 2 == j0 >> 2) pow2_scale(m, up[z], inv[z]);
+        if (lane >> 2 == j0 >> 2) {
+          pow2_scale(m, up[z], inv[z]);
+          if (m == 0) up[z] = 0.0f;        // (as of a cached zero row)
+        }
       }
     }
     float s[NT][2][4];

@@ -52,11 +52,14 @@ struct KeyScalars {
   float sk, lsv, rsv;   // c log2e ks, log2 vs, 1 / vs
 };
 
-// vs below 2^-90 is taken as 2^-90: sums of w / vs then stay in range.
+// vs below 2^-90 is taken as 2^-90: sums of w / vs then stay in range. A zero row
+// (scale 0) has zero codes, so any vs gives the same value: 2^-60, which leaves the
+// running maximum to the rows that count (with 1, f16 weights of rows with scales
+// below 2^-22 vanished beside it) and its own part of the sum above fp32's smallest
+// number beside rows with scales up to 2^50.
 __device__ __forceinline__ KeyScalars key_scalars(const CachedAttn& p, float ks, float vs, bool valid) {
   KeyScalars r;
-  // a zero row (scale 0) has zero codes: any vs gives the same value
-  const float v = vs == 0.0f ? 1.0f : fmaxf(vs, 8.077935669e-28f);
+  const float v = vs == 0.0f ? 8.673617380e-19f : fmaxf(vs, 8.077935669e-28f);
   r.sk = valid ? p.scale_log2 * ks : 0.0f;
   float lg, rc;                 // (relative errors below 2^-21)
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lg) : "f"(v));

@@ -53,3 +53,23 @@ def test_a_held_part_sees_writes_through_its_parent_and_through_other_parts(sq):
     q = rows(g, 2, sq, 2, 128)
     assert other.lengths.tolist() == [136, 135]
     assert_attention(cached_attention(q, other), *attention64(q, other, None, None, None))
+
+
+# ------------------------------------------------------------- zero V rows beside very small or large ones
+@pytest.mark.parametrize("sq", [1, 4, 16, 60, 300])
+@pytest.mark.parametrize("power", [-70, -40, -24, 0, 40, 46])
+def test_zero_rows_leave_the_weights_of_small_rows_alone(sq, power):
+    """A zero row has no scale of its own, so nothing may depend on the scales
+    of the rows around it."""
+    from qwen_image_accel_b200.kernels.kv_cache import cached_attention
+    g = gen(33)
+    cache = make_cache(g, 1, 2, 150, [150])
+    k, v = rows(g, 1, 20, 2, 128), rows(g, 1, 20, 2, 128) * 2.0 ** power
+    cache.v_scales.mul_(2.0 ** power)
+    zero = torch.arange(150, device=DEV) % 3 == 0
+    cache.v_codes[:, :, zero] = 0
+    cache.v_scales[:, :, zero] = 0
+    v[:, ::4] = 0
+    q = rows(g, 1, sq, 2, 128)
+    assert_attention(cached_attention(q, cache), *attention64(q, cache, None, None, None))
+    assert_attention(cached_attention(q, cache, k, v), *attention64(q, cache, k, v, None))
