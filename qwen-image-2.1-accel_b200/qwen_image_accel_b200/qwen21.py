@@ -348,9 +348,9 @@ class Block21:
         return out
 
     # ------------------------------------------------------------------ modes
-    def _joint_with_prefix(self, layer_cache, b: int, st: int, device):
+    def _joint_with_prefix(self, layer_cache, b: int, st: int, device, shared: bool = False):
         """Joint q/k/v buffers of p + st tokens with the cached prefix's K/V in
-        rows [0, p), and p."""
+        rows [0, p), and p. shared: a bf16 prefix of one sample may serve all."""
         if isinstance(layer_cache, QuantizedKVLayerCache):
             cache = layer_cache.quantized
             if cache is None:
@@ -358,8 +358,8 @@ class Block21:
             p, batch = cache.extent, cache.batch
         else:
             cached_k, cached_v = layer_cache.get()
-            p, batch = cached_k.shape[1], cached_k.shape[0]
-            if cached_v.shape != cached_k.shape:
+            p, batch = cached_k.shape[1], b if shared else cached_k.shape[0]
+            if cached_v.shape != cached_k.shape and not shared:
                 raise ValueError("cached decode: the cache does not match the batch")
         if batch != b:
             raise ValueError("cached decode: the cache does not match the batch")
@@ -422,14 +422,15 @@ class Block21:
                          key_valid: torch.Tensor | None = None) -> torch.Tensor:
         """The attention half of the cached decode on an already modulated
         input x [B, St, D] bf16: Q/K/V projections, QK-RMSNorm + RoPE behind the
-        cached prefix K/V, attention over [prefix, target] (Sage when the block
-        has it and nothing is masked, else SDPA), output projection -> bf16
-        [B, St, D]."""
+        cached prefix K/V (a bf16 prefix of batch 1 serves every sample),
+        attention over [prefix, target] (Sage when the block has it and nothing
+        is masked, else SDPA, or cached_attention over an INT8 prefix), output
+        projection -> bf16 [B, St, D]."""
         b, st, _ = x.shape
         if isinstance(layer_cache, QuantizedKVLayerCache) and not (self.sage and key_valid is None):
             return self._out_proj(self._attend_quantized(x.contiguous(), b, st, freqs, layer_cache.quantized,
                                                          key_valid))
-        p, oq, ok, ov = self._joint_with_prefix(layer_cache, b, st, x.device)
+        p, oq, ok, ov = self._joint_with_prefix(layer_cache, b, st, x.device, shared=True)
         self._qkv_into(x.contiguous(), b, st, freqs, oq, ok, ov, p)
         q = oq[:, p:]
         if self.sage and key_valid is None:

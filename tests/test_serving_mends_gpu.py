@@ -73,3 +73,25 @@ def test_zero_rows_leave_the_weights_of_small_rows_alone(sq, power):
     q = rows(g, 1, sq, 2, 128)
     assert_attention(cached_attention(q, cache), *attention64(q, cache, None, None, None))
     assert_attention(cached_attention(q, cache, k, v), *attention64(q, cache, k, v, None))
+
+
+# ------------------------------------------------------------- one prefix for several samples
+@pytest.mark.parametrize("profile", ["fused", "fused_sage"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attention_cached_takes_one_prefix_for_all_samples(profile, masked):
+    """A bf16 prefix of batch 1 serves a batch, like one that is stored once per sample."""
+    from test_block21_gpu import build, t_bf16
+    from qwen_image_accel_b200.qwen21 import KVLayerCache
+    blk, gold = build(profile)
+    ht = t_bf16(gold["h_target"]).cuda().repeat(2, 1, 1)
+    freqs = torch.view_as_complex(torch.from_numpy(gold["rope"]).contiguous()).cuda()[int(gold["prefix_len"]):]
+    k, v = t_bf16(gold["cached_k"]).cuda(), t_bf16(gold["cached_v"]).cuda()
+    valid = None
+    if masked:
+        valid = torch.ones(2, k.shape[1] + ht.shape[1], dtype=torch.bool, device=DEV)
+        valid[1, :3] = False
+    one, each = KVLayerCache(), KVLayerCache()
+    one.store(k, v)
+    each.store(k.repeat(2, 1, 1, 1), v.repeat(2, 1, 1, 1))
+    got = blk.attention_cached(ht, freqs.contiguous(), one, key_valid=valid)
+    assert torch.equal(got, blk.attention_cached(ht, freqs.contiguous(), each, key_valid=valid))
