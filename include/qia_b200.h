@@ -638,10 +638,10 @@ int64_t qia_cached_attention_workspace_bytes(int64_t batch, int64_t seq_q,
  * [batch, seq, out] bf16 (y may be base), strides: elements, (batch, seq) of
  * x, base, y, multiples of 8, rows contiguous. a: bf16 [adapters, r_pad, in],
  * b: bf16 [adapters, out, r_pad]; rows of A_i and columns of B_i past
- * ranks[i] hold zeros. ranks, ids: int32, scales: f32, device memory. in,
- * out and r_pad multiples of 8, r_pad <= 128. workspace:
- * qia_lora_workspace_bytes bytes of device memory, 16-byte aligned (NULL when
- * that is 0, as it is for seq <= 8). */
+ * ranks[i] hold zeros (rank 0: nothing is added). ranks, ids: int32, scales:
+ * f32, device memory. in, out and r_pad multiples of 8, r_pad <= 128.
+ * workspace: qia_lora_workspace_bytes bytes of device memory, 16-byte aligned
+ * (NULL when that is 0, as it is for seq <= 8). */
 int qia_lora_add(const void* x, const void* base, void* y, const void* a,
                  const void* b, const void* ranks, const void* scales,
                  const void* ids, int64_t batch, int64_t seq,

@@ -503,7 +503,8 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_consta
         const bool ok = mbar_wait(smem_u32(t_full), 0, err) && got_b;
         if (ok) {
           tc_fence_after();
-          const int steps = (min(__ldg(p.ranks + id), p.r_pad) + 15) / 16;
+          // (one step at least: t is zero past the rank, and the accumulator has to be written)
+          const int steps = max(1, (min(__ldg(p.ranks + id), p.r_pad) + 15) / 16);
           for (int k = 0; k < steps; ++k) {
             const uint64_t off = uint64_t(((k >> 2) * 16384 + (k & 3) * 32) >> 4);
             tc_mma_f16_ss(tmem, smem_desc_k_sw128(smem_u32(t_tile)) + off, smem_desc_k_sw128(smem_u32(b_tile)) + off,

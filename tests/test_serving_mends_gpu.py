@@ -95,3 +95,24 @@ def test_attention_cached_takes_one_prefix_for_all_samples(profile, masked):
     each.store(k.repeat(2, 1, 1, 1), v.repeat(2, 1, 1, 1))
     got = blk.attention_cached(ht, freqs.contiguous(), one, key_valid=valid)
     assert torch.equal(got, blk.attention_cached(ht, freqs.contiguous(), each, key_valid=valid))
+
+
+# ------------------------------------------------------------- adapters of rank 0
+@pytest.mark.parametrize("b,s", [(2, 1), (2, 8), (1, 60), (2, 300), (3, 1000)])
+@pytest.mark.parametrize("rank", [0, -1])
+def test_an_adapter_of_rank_zero_adds_nothing(b, s, rank):
+    """As a caller of the C entry may lay it out: zero rows and columns only."""
+    from qwen_image_accel_b200.kernels.lora import LoraWeights, lora_add
+    from test_lora_gpu import adapters, check, lora64, rand
+    g = gen(34)
+    items = adapters(g, 512, 1024, [40, 64])
+    w = LoraWeights(items)
+    x, base = rand(g, b, s, 512), rand(g, b, s, 1024)
+    ids = [i % 2 for i in range(b)]
+    idt = torch.tensor(ids, dtype=torch.int32, device=DEV)
+    used = lora_add(x, base, w, idt)                # (leaves its sums in the accumulators)
+    check(used, lora64(x, base, items, ids))
+    w.a[0], w.b[0], w.ranks[0] = 0, 0, rank
+    got = lora_add(x, base, w, idt)
+    for i, a in enumerate(ids):
+        assert torch.equal(got[i], used[i] if a else base[i])
