@@ -19,7 +19,8 @@ _strides6 = struct.Struct("6q").pack      # stride arguments (int64[]) as bytes
 
 class LoraWeights:
     """The adapters of one projection, laid out once: `adapters` is a list of
-    (A [rank, in], B [out, rank], scale), ranks 1 to 128 in any mix.
+    (A [rank, in], B [out, rank], scale), ranks to 128 in any mix (rank 0: an
+    adapter that adds nothing).
 
     a: bf16 [n, r_pad, in], b: bf16 [n, out, r_pad], zero-padded to the
     largest rank (a multiple of 8); ranks int32 [n], scales float32 [n]."""
@@ -34,11 +35,11 @@ class LoraWeights:
             if a.ndim != 2 or b.ndim != 2 or a.shape[1] != self.in_features or b.shape != (self.out_features, r):
                 raise ValueError(f"LoraWeights: A {tuple(a.shape)} and B {tuple(b.shape)} do not fit a "
                                  f"{self.in_features} -> {self.out_features} projection")
-        if self.in_features % 8 or self.out_features % 8 or not 1 <= min(ranks) <= max(ranks) <= MAX_RANK:
+        if self.in_features % 8 or self.out_features % 8 or max(ranks) > MAX_RANK:
             raise NotImplementedError(f"LoraWeights: {self.in_features} -> {self.out_features}, ranks {min(ranks)} to "
-                                      f"{max(ranks)} (features in multiples of 8, ranks 1 to {MAX_RANK})")
+                                      f"{max(ranks)} (features in multiples of 8, ranks to {MAX_RANK})")
         self.count = len(adapters)
-        self.r_pad = (max(ranks) + 7) // 8 * 8
+        self.r_pad = max(8, (max(ranks) + 7) // 8 * 8)
         self.a = torch.zeros(self.count, self.r_pad, self.in_features, dtype=torch.bfloat16, device=dev)
         self.b = torch.zeros(self.count, self.out_features, self.r_pad, dtype=torch.bfloat16, device=dev)
         for i, ((a, b, _), r) in enumerate(zip(adapters, ranks)):

@@ -190,7 +190,7 @@ class Qwen21Transformer:
                 some = next((h for h in held if h is not None), None)
                 if some is None:
                     continue
-                none = (torch.zeros(1, some[0].shape[1]), torch.zeros(some[1].shape[0], 1), 0.0)
+                none = (torch.zeros(0, some[0].shape[1]), torch.zeros(some[1].shape[0], 0), 0.0)
                 per[n] = LoraWeights([none if h is None else h for h in held], device=dev)
             blk.set_adapters(per)
 

@@ -116,3 +116,24 @@ def test_an_adapter_of_rank_zero_adds_nothing(b, s, rank):
     got = lora_add(x, base, w, idt)
     for i, a in enumerate(ids):
         assert torch.equal(got[i], used[i] if a else base[i])
+
+
+@pytest.mark.parametrize("s", [1, 300])
+def test_an_adapter_that_leaves_a_linear_out_does_nothing_there(s):
+    """Whatever the activations hold: infinities and NaN too."""
+    from qwen_image_accel_b200.kernels.lora import LoraWeights, lora_add
+    from test_lora_gpu import adapters, rand
+    from test_serving_gpu import adapter, build
+    model, shapes = build("fused")
+    model.load_adapters([adapter(shapes, 1), adapter(shapes, 2, skip=("attn.to_v",))])
+    w = model.blocks[0].adapters["attn.to_v"]
+    assert (w.in_features, w.out_features, w.count) == (512, 512, 2)
+    g = gen(35)
+    x, base = rand(g, 2, s, 512), rand(g, 2, s, 512)
+    x[1, 0, 7], x[1, s - 1, 9] = float("inf"), float("nan")
+    got = lora_add(x, base, w, torch.tensor([0, 1], dtype=torch.int32, device=DEV))
+    assert torch.equal(got[1], base[1]) and not torch.equal(got[0], base[0])
+    alone = LoraWeights([(torch.zeros(0, 512), torch.zeros(512, 0), 1.0)])
+    assert torch.equal(lora_add(x, base, alone, torch.zeros(2, dtype=torch.int32, device=DEV)), base)
+    with pytest.raises(ValueError, match="do not fit"):
+        LoraWeights(adapters(g, 512, 512, [8]) + [(torch.zeros(0, 512), torch.zeros(512, 1), 1.0)])
