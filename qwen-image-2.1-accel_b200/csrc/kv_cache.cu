@@ -224,7 +224,7 @@ extern "C" int qia_kv_cache_write(const void* k, const void* v, void* k_codes, v
   if (rc) return rc;
   const bool append = start < 0;
   if (append && !ticket) return set_error(QIA_ERR_INVALID, "%s: an append needs a ticket word", who);
-  if (!append && start + seq > capacity)
+  if (!append && start > capacity - seq)
     return set_error(QIA_ERR_INVALID, "%s: tokens %lld+%lld exceed the capacity %lld", who, (long long)start,
                      (long long)seq, (long long)capacity);
   if (seq == 0 && append) return QIA_OK;
@@ -246,7 +246,7 @@ extern "C" int qia_kv_cache_read(const void* k_codes, const void* v_codes, const
   const char* who = "qia_kv_cache_read";
   int rc = check_cache(who, k_codes, v_codes, k_scales, v_scales, lengths, batch, tokens, heads, capacity, head_dim);
   if (rc) return rc;
-  if (first < 0 || first + tokens > capacity)
+  if (first < 0 || first > capacity - tokens)
     return set_error(QIA_ERR_INVALID, "%s: tokens %lld+%lld of capacity %lld", who, (long long)first,
                      (long long)tokens, (long long)capacity);
   if (tokens == 0) return QIA_OK;

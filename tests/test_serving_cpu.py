@@ -48,3 +48,16 @@ def test_extent_can_be_set_for_what_the_host_does_not_count(host):
     assert part.extent == 20
     part.extent = 3
     assert cache.extent == 20 and part.extent == 3
+
+
+def test_token_positions_that_overflow_are_refused():
+    """The C entries, called past the Python checks: position + count beyond 64 bits."""
+    import ctypes
+    from qwen_image_accel_b200 import _lib
+    lib = _lib.load()
+    at, top = ctypes.c_void_p(4096), 2 ** 63 - 1
+    strides = (ctypes.c_int64 * 6)(*([1024] * 6))
+    rc = lib.qia_kv_cache_write(at, at, at, at, at, at, at, 1, 4, 1, 128, 8, top - 1, strides, None, None)
+    assert rc == 1 and b"capacity 8" in lib.qia_last_error_string()
+    rc = lib.qia_kv_cache_read(at, at, at, at, at, at, at, 1, top - 1, 4, 1, 128, 8, strides, None)
+    assert rc == 1 and b"capacity 8" in lib.qia_last_error_string()
