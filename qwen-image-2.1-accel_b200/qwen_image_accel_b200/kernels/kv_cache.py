@@ -96,6 +96,15 @@ class QuantizedKV:
         self._held[self._first:self._first + self.batch] = [tokens] * self.batch
 
 
+def _strides(t: torch.Tensor) -> tuple[int, int, int]:
+    """Batch, sequence and head strides; 0 for a dimension of size 1 whose
+    stride is odd (nothing is ever that far apart)."""
+    a, b, c, _ = t.stride()
+    if (a | b | c) & 7:
+        return tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], (a, b, c)))
+    return a, b, c
+
+
 def _check_rows(who: str, cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> None:
     _lib.require_cuda(k, v)
     shape = k.shape
@@ -136,7 +145,7 @@ def kv_cache_append(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> Non
 def _write(cache, k, v, seq, start):
     kc, vc, ks, vs, lengths = cache._buffers
     _lib.call("qia_kv_cache_write", k.data_ptr(), v.data_ptr(), kc, vc, ks, vs, lengths, cache.batch, seq,
-              cache.kv_heads, HEAD_DIM, cache.capacity, start, _strides6(*k.stride()[:3], *v.stride()[:3]),
+              cache.kv_heads, HEAD_DIM, cache.capacity, start, _strides6(*_strides(k), *_strides(v)),
               cache._ticket, _lib.raw_stream(cache._index))
 
 
@@ -161,7 +170,7 @@ def kv_cache_read(cache: QuantizedKV, first: int = 0, tokens: int | None = None,
         if out_k.shape != shape:
             raise ValueError(f"kv_cache_read: the outputs must be {shape}, got {tuple(out_k.shape)}")
     _lib.call("qia_kv_cache_read", *cache._buffers, out_k.data_ptr(), out_v.data_ptr(), cache.batch, first, tokens,
-              cache.kv_heads, HEAD_DIM, cache.capacity, _strides6(*out_k.stride()[:3], *out_v.stride()[:3]),
+              cache.kv_heads, HEAD_DIM, cache.capacity, _strides6(*_strides(out_k), *_strides(out_v)),
               _lib.raw_stream(cache._index))
     return out_k, out_v
 
@@ -184,8 +193,7 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
     if len(shape) != 4 or shape[0] != cache.batch or shape[3] != HEAD_DIM or shape[2] % cache.kv_heads:
         raise ValueError(f"{who}: q must be [{cache.batch}, seq, a multiple of {cache.kv_heads}, {HEAD_DIM}], got "
                          f"{tuple(shape)}")
-    q_strides = q.stride()
-    if q.dtype != torch.bfloat16 or q_strides[3] != 1:
+    if q.dtype != torch.bfloat16 or q.stride(3) != 1:
         raise NotImplementedError(f"{who}: q must be bf16 with contiguous rows")
     if q.get_device() != cache._index:
         raise ValueError(f"{who}: q and the cache are on different devices")
@@ -196,13 +204,13 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
     extent, fresh, rows = cache.extent, 0, _NO_ROWS
     if k is not None:
         _check_rows(who, cache, k, v)
-        fresh, rows = k.shape[1], k.stride()[:3] + v.stride()[:3]
+        fresh, rows = k.shape[1], _strides(k) + _strides(v)
     mask_stride = 0
     if key_valid is not None:
         if key_valid.shape != (cache.batch, extent + fresh) or key_valid.dtype != torch.bool:
             raise ValueError(f"{who}: key_valid must be bool [{cache.batch}, {extent + fresh}], got "
                              f"{key_valid.dtype} {tuple(key_valid.shape)}")
-        if key_valid.stride(1) != 1 or key_valid.get_device() != cache._index:
+        if key_valid.stride(1) != 1 and key_valid.shape[1] > 1 or key_valid.get_device() != cache._index:
             raise NotImplementedError(f"{who}: key_valid must have contiguous rows on the cache's device")
         mask_stride = key_valid.stride(0)
     if out is None:
@@ -219,6 +227,6 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
     _lib.call("qia_cached_attention", q.data_ptr(), k.data_ptr() if fresh else None, v.data_ptr() if fresh else None,
               *cache._buffers, None if key_valid is None else key_valid.data_ptr(), out.data_ptr(), cache.batch,
               shape[1], fresh, shape[2], cache.kv_heads, HEAD_DIM, cache.capacity, extent,
-              _strides12(*q_strides[:3], *rows, *out.stride()[:3]), mask_stride, 0.0 if scale is None else float(scale),
+              _strides12(*_strides(q), *rows, *_strides(out)), mask_stride, 0.0 if scale is None else float(scale),
               None if ws is None else ws.data_ptr(), _lib.raw_stream(cache._index))
     return out

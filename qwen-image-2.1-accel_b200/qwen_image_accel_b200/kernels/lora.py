@@ -17,6 +17,15 @@ MAX_RANK = 128
 _strides6 = struct.Struct("6q").pack      # stride arguments (int64[]) as bytes
 
 
+def _strides(t: torch.Tensor) -> tuple[int, int]:
+    """Batch and sequence strides; 0 for a dimension of size 1 whose stride is
+    odd (nothing is ever that far apart)."""
+    a, b, _ = t.stride()
+    if (a | b) & 7:
+        return tuple(0 if n == 1 else s for n, s in zip(t.shape[:2], (a, b)))
+    return a, b
+
+
 class LoraWeights:
     """The adapters of one projection, laid out once: `adapters` is a list of
     (A [rank, in], B [out, rank], scale), ranks to 128 in any mix (rank 0: an
@@ -65,8 +74,7 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
         raise ValueError(f"{who}: x {tuple(x.shape)} and base {tuple(base.shape)} do not fit a "
                          f"{weights.in_features} -> {weights.out_features} projection")
     batch, seq, _ = shape
-    x_strides, base_strides = x.stride(), base.stride()
-    if x.dtype != torch.bfloat16 or base.dtype != torch.bfloat16 or x_strides[2] != 1 or base_strides[2] != 1:
+    if x.dtype != torch.bfloat16 or base.dtype != torch.bfloat16 or x.stride(2) != 1 or base.stride(2) != 1:
         raise NotImplementedError(f"{who}: x and base must be bf16 with contiguous rows")
     if ids.shape != (batch,) or ids.dtype != torch.int32 or not ids.is_contiguous():
         raise ValueError(f"{who}: ids must be int32 [{batch}], got {ids.dtype} {tuple(ids.shape)}")
@@ -78,8 +86,7 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
         return out
     if out.data_ptr() == x.data_ptr():
         raise ValueError(f"{who}: out may be base, not x")
-    out_strides = out.stride()
-    if out_strides[2] != 1:
+    if out.stride(2) != 1:
         raise NotImplementedError(f"{who}: out must have contiguous rows")
     index = weights._index
     if x.get_device() != index or base.get_device() != index or ids.get_device() != index or out.get_device() != index:
@@ -89,6 +96,6 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
     ws = x.new_empty(size >> 1) if size else None       # (bf16 elements)
     _lib.call("qia_lora_add", x.data_ptr(), base.data_ptr(), out.data_ptr(), *weights._buffers, ids.data_ptr(), batch,
               seq, weights.in_features, weights.out_features, weights.count, weights.r_pad,
-              _strides6(*x_strides[:2], *base_strides[:2], *out_strides[:2]), None if ws is None else ws.data_ptr(),
+              _strides6(*_strides(x), *_strides(base), *_strides(out)), None if ws is None else ws.data_ptr(),
               _lib.raw_stream(index))
     return out

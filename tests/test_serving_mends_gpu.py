@@ -137,3 +137,38 @@ def test_an_adapter_that_leaves_a_linear_out_does_nothing_there(s):
     assert torch.equal(lora_add(x, base, alone, torch.zeros(2, dtype=torch.int32, device=DEV)), base)
     with pytest.raises(ValueError, match="do not fit"):
         LoraWeights(adapters(g, 512, 512, [8]) + [(torch.zeros(0, 512), torch.zeros(512, 1), 1.0)])
+
+
+# ------------------------------------------------------------- strides that nothing is apart by
+def odd(t, *dims):
+    """t with an odd stride in dimensions of size 1."""
+    strides = [13 if i in dims else s for i, s in enumerate(t.stride())]
+    assert all(t.shape[i] == 1 for i in dims)
+    return t.as_strided(t.shape, strides)
+
+
+@pytest.mark.parametrize("sq", [1, 40, 300])
+def test_odd_strides_of_dimensions_of_size_one(sq):
+    from qwen_image_accel_b200.kernels.kv_cache import QuantizedKV, cached_attention, kv_cache_read, kv_cache_write
+    from qwen_image_accel_b200.kernels.lora import LoraWeights, lora_add
+    from test_lora_gpu import adapters, check, lora64, rand
+    g = gen(36)
+    cache = QuantizedKV(1, 1, 1)
+    k, v = rows(g, 1, 1, 1, 128), rows(g, 1, 1, 1, 128)
+    kv_cache_write(cache, odd(k, 0, 1, 2), odd(v, 0, 1, 2))
+    ok, ov = torch.empty_like(k), torch.empty_like(v)
+    kv_cache_read(cache, out_k=odd(ok, 0, 1, 2), out_v=odd(ov, 0, 1))
+    assert all(torch.equal(a, b) for a, b in zip((ok, ov), kv_cache_read(cache)))
+    q = rows(g, 1, sq, 1, 128)
+    out = torch.empty_like(q)
+    cached_attention(odd(q, 0, 2), cache, odd(k, 0, 1, 2), odd(v, 0, 2), out=odd(out, 0, 2))
+    assert_attention(out, *attention64(q, cache, k, v, None))
+    mask = torch.ones(1, 2, dtype=torch.bool, device=DEV)[:, ::2]             # one column, stride 2
+    got = cached_attention(q, cache, key_valid=mask)
+    assert_attention(got, *attention64(q, cache, None, None, mask))
+    items = adapters(g, 64, 128, [8])
+    x, base = rand(g, 1, sq, 64), rand(g, 1, sq, 128)
+    ids = torch.zeros(1, dtype=torch.int32, device=DEV)
+    dims = (0, 1) if sq == 1 else (0,)
+    got = lora_add(odd(x, *dims), odd(base, *dims), LoraWeights(items), ids)
+    check(got, lora64(x, base, items, [0]))
