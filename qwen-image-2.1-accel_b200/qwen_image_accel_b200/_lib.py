@@ -179,6 +179,44 @@ def stream(device: torch.device | None = None):
 raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one element size share an element (exact: columns
+    of one buffer that lie beside each other do not)."""
+    at, other = a.data_ptr(), b.data_ptr()
+    if at > other:
+        a, b, at, other = b, a, other, at
+    size, end = a.element_size(), 1
+    for n, s in zip(a.shape, a.stride()):
+        end += (n - 1) * s
+    if at + end * size <= other or not a.numel() or not b.numel():
+        return False
+    # b's first element is at sum stride x of a minus the same of b, 0 <= x < size; with
+    # b's x counted from their ends every term is positive, and terms of one stride add up
+    target = (other - at) // size
+    most: dict[int, int] = {}
+    for n, s in zip(a.shape, a.stride()):
+        if n > 1 and s:
+            most[s] = most.get(s, 0) + n - 1
+    for n, s in zip(b.shape, b.stride()):
+        if n > 1 and s:
+            most[s] = most.get(s, 0) + n - 1
+            target += s * (n - 1)
+    rest = sum(s * m for s, m in most.items())
+    if not 0 <= target <= rest:
+        return False
+    terms = sorted(most.items(), reverse=True)
+
+    def reached(i: int, target: int, rest: int) -> bool:
+        if i == len(terms):
+            return target == 0
+        s, m = terms[i]
+        rest -= s * m
+        return any(reached(i + 1, target - s * x, rest)
+                   for x in range(max(0, -((rest - target) // s)), min(m, target // s) + 1))
+
+    return reached(0, target, rest)
+
+
 def require_cuda(*tensors: torch.Tensor | None) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:

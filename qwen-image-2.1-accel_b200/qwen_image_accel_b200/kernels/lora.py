@@ -66,7 +66,8 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
     """base [batch, seq, out] plus each request's adapter applied to x [batch,
     seq, in], both bf16 with contiguous rows; ids: int32 [batch] on the device,
     -1 for a request without an adapter. Returns a new bf16 tensor, or `out`,
-    which may be `base` itself."""
+    which may be `base` itself but may not share memory with x or lie otherwise
+    over base."""
     who = "lora_add"
     _lib.require_cuda(x, base, ids, out)
     shape = x.shape
@@ -78,14 +79,20 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
         raise NotImplementedError(f"{who}: x and base must be bf16 with contiguous rows")
     if ids.shape != (batch,) or ids.dtype != torch.int32 or not ids.is_contiguous():
         raise ValueError(f"{who}: ids must be int32 [{batch}], got {ids.dtype} {tuple(ids.shape)}")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(base)
     elif out.shape != base.shape or out.dtype != torch.bfloat16:
         raise ValueError(f"{who}: out must be like base")
     if not out.numel():
         return out
-    if out.data_ptr() == x.data_ptr():
-        raise ValueError(f"{who}: out may be base, not x")
+    if given:
+        if any(n > 1 and not s for n, s in zip(out.shape, out.stride())):
+            raise ValueError(f"{who}: several elements of out share memory")
+        if _lib.overlaps(out, x):
+            raise ValueError(f"{who}: out may be base, not x or a part of it")
+        if (out.data_ptr() != base.data_ptr() or out.stride() != base.stride()) and _lib.overlaps(out, base):
+            raise ValueError(f"{who}: out may be base, not overlap it")
     if out.stride(2) != 1:
         raise NotImplementedError(f"{who}: out must have contiguous rows")
     index = weights._index

@@ -61,3 +61,52 @@ def test_token_positions_that_overflow_are_refused():
     assert rc == 1 and b"capacity 8" in lib.qia_last_error_string()
     rc = lib.qia_kv_cache_read(at, at, at, at, at, at, at, 1, top - 1, 4, 1, 128, 8, strides, None)
     assert rc == 1 and b"capacity 8" in lib.qia_last_error_string()
+
+
+def test_overlaps_of_views():
+    """Views of one buffer, against the sets of their elements."""
+    import random
+    from qwen_image_accel_b200 import _lib
+    rng, buf = random.Random(1), torch.arange(400, dtype=torch.int16)
+
+    def view():
+        while True:
+            dims = rng.randint(1, 4)
+            shape = [rng.choice([1, 1, 2, 3, 5]) for _ in range(dims)]
+            stride = [rng.choice([0, 1, 2, 3, 4, 7, 8, 16, 30]) for _ in range(dims)]
+            first = rng.randint(0, 150)
+            if first + sum((n - 1) * s for n, s in zip(shape, stride)) < 400:
+                return buf.as_strided(shape, stride, first)
+
+    seen = set()
+    for _ in range(4000):
+        a, b = view(), view()
+        want = bool(set(a.flatten().tolist()) & set(b.flatten().tolist()))
+        assert _lib.overlaps(a, b) == want
+        seen.add(want)
+    assert seen == {True, False}
+    wide = torch.empty(4, 4096, 12288, dtype=torch.bfloat16, device="meta")
+    assert not _lib.overlaps(wide[:0], wide)
+
+
+def test_adapters_refuse_outputs_over_their_inputs(monkeypatch):
+    from qwen_image_accel_b200 import _lib
+    from qwen_image_accel_b200.kernels import lora
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(_lib, "raw_stream", lambda index: 0)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: None)
+    w = lora.LoraWeights([(torch.zeros(8, 64), torch.zeros(64, 8), 1.0)], device="cpu")
+    ids = torch.zeros(2, dtype=torch.int32)
+    buf = torch.zeros(2, 20, 256, dtype=torch.bfloat16)
+    x, base = buf[:, :9, :64], buf[:, :9, 64:128]
+    assert lora.lora_add(x, base, w, ids, out=base) is base                   # columns beside x
+    for out in (buf[:, 1:10, :64], buf[:, :9, 8:72], x):
+        with pytest.raises(ValueError, match="not x"):
+            lora.lora_add(x, base, w, ids, out=out)
+    for out in (buf[:, 1:10, 64:128], buf[:, :9, 72:136]):
+        with pytest.raises(ValueError, match="not overlap"):
+            lora.lora_add(x, base, w, ids, out=out)
+    shared = torch.zeros(1, 9, 64, dtype=torch.bfloat16).expand(2, -1, -1)
+    with pytest.raises(ValueError, match="share memory"):
+        lora.lora_add(x, shared, w, ids, out=shared)
+    assert lora.lora_add(x, shared, w, ids).shape == (2, 9, 64)
