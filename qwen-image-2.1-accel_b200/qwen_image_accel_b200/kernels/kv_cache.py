@@ -117,6 +117,11 @@ def _check_rows(who: str, cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) 
         raise ValueError(f"{who}: k, v and the cache are on different devices")
 
 
+def _check_output(who: str, out: torch.Tensor) -> None:
+    if any(n > 1 and not s for n, s in zip(out.shape, out.stride())):
+        raise ValueError(f"{who}: several elements of an output share memory")
+
+
 def kv_cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, start: int = 0) -> None:
     """Quantise k, v [batch, seq, kv_heads, 128] bf16 (any strides that are
     multiples of 8, rows contiguous) into tokens [start, start + seq) of every
@@ -169,6 +174,10 @@ def kv_cache_read(cache: QuantizedKV, first: int = 0, tokens: int | None = None,
         _check_rows("kv_cache_read", cache, out_k, out_v)
         if out_k.shape != shape:
             raise ValueError(f"kv_cache_read: the outputs must be {shape}, got {tuple(out_k.shape)}")
+        _check_output("kv_cache_read", out_k)
+        _check_output("kv_cache_read", out_v)
+        if _lib.overlaps(out_k, out_v):
+            raise ValueError("kv_cache_read: the outputs overlap")
     _lib.call("qia_kv_cache_read", *cache._buffers, out_k.data_ptr(), out_v.data_ptr(), cache.batch, first, tokens,
               cache.kv_heads, HEAD_DIM, cache.capacity, _strides6(*_strides(out_k), *_strides(out_v)),
               _lib.raw_stream(cache._index))
@@ -186,7 +195,8 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
     [batch, fresh, kv_heads, 128] or None; key_valid: bool [batch, cache.extent
     + fresh], False where a key takes no part (whatever it holds). Cached
     tokens past a request's length never take part. A query without any key
-    gives zeros. scale defaults to 1/sqrt(128). Returns bf16 like q."""
+    gives zeros. scale defaults to 1/sqrt(128). Returns bf16 like q, or `out`,
+    which may be q itself."""
     who = "cached_attention"
     _lib.require_cuda(q, key_valid)
     shape = q.shape
@@ -217,6 +227,11 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
         out = torch.empty_like(q)
     elif out.shape != shape or out.dtype != torch.bfloat16 or out.stride(3) != 1 or out.get_device() != cache._index:
         raise ValueError(f"{who}: out must be like q")
+    else:
+        _check_output(who, out)
+        if (out.data_ptr() != q.data_ptr() or out.stride() != q.stride()) and _lib.overlaps(out, q) or (
+                fresh and (_lib.overlaps(out, k) or _lib.overlaps(out, v))):
+            raise ValueError(f"{who}: out may be q, not overlap it, k or v")
     if not out.numel():
         return out
     size = 0

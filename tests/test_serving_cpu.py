@@ -110,3 +110,25 @@ def test_adapters_refuse_outputs_over_their_inputs(monkeypatch):
     with pytest.raises(ValueError, match="share memory"):
         lora.lora_add(x, shared, w, ids, out=shared)
     assert lora.lora_add(x, shared, w, ids).shape == (2, 9, 64)
+
+
+def test_attention_and_read_back_refuse_outputs_over_their_inputs(host, monkeypatch):
+    from qwen_image_accel_b200 import _lib
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: None)
+    cache = host.QuantizedKV(2, 2, 32, device="cpu")
+    host.kv_cache_write(cache, rows(2, 8), rows(2, 8))
+    buf = torch.zeros(2, 12, 2, 4 * 128, dtype=torch.bfloat16)
+    q, k, v = (buf[:, :5, :, 128 * i:128 * (i + 1)] for i in range(3))
+    assert host.cached_attention(q, cache, k, v, out=q) is q
+    assert host.cached_attention(q, cache, k, v, out=buf[:, :5, :, 384:]).shape == q.shape
+    for out in (k, v, buf[:, 1:6, :, 128:256], buf[:, 1:6, :, :128], buf[:, :5, :, 8:136]):
+        with pytest.raises(ValueError, match="not overlap"):
+            host.cached_attention(q, cache, k, v, out=out)
+    one = rows(2, 1).expand(-1, 5, -1, -1)
+    with pytest.raises(ValueError, match="share memory"):
+        host.cached_attention(q, cache, k, v, out=one)
+    with pytest.raises(ValueError, match="share memory"):
+        host.kv_cache_read(cache, tokens=5, out_k=one, out_v=rows(2, 5))
+    with pytest.raises(ValueError, match="overlap"):
+        host.kv_cache_read(cache, tokens=5, out_k=k, out_v=buf[:, 2:7, :, 128:256])
+    host.kv_cache_read(cache, tokens=5, out_k=k, out_v=v)

@@ -172,3 +172,15 @@ def test_odd_strides_of_dimensions_of_size_one(sq):
     dims = (0, 1) if sq == 1 else (0,)
     got = lora_add(odd(x, *dims), odd(base, *dims), LoraWeights(items), ids)
     check(got, lora64(x, base, items, [0]))
+
+
+@pytest.mark.parametrize("b,sq,h,kvh,n,fresh", [(2, 1, 8, 4, 700, 1), (1, 16, 4, 4, 300, 0), (2, 60, 4, 2, 300, 60),
+                                                (2, 60, 90, 90, 300, 60), (2, 700, 4, 4, 300, 90)])
+def test_attention_written_over_its_queries(b, sq, h, kvh, n, fresh):
+    from qwen_image_accel_b200.kernels.kv_cache import cached_attention
+    g = gen(37)
+    cache = make_cache(g, b, kvh, n, [n] * b)
+    q = rows(g, b, sq, h, 128)
+    k, v = (rows(g, b, fresh, kvh, 128) for _ in range(2)) if fresh else (None, None)
+    want = cached_attention(q, cache, k, v)
+    assert cached_attention(q, cache, k, v, out=q) is q and torch.equal(q, want)
