@@ -17,7 +17,7 @@ copied in whenever a different KV cache object (a new request) arrives. The
 modulation vectors are computed inside the graph, so each replay sees the new
 timestep. The returned tensor is the graph's static output: it is overwritten
 by the next replay. Serial use only (one request at a time), as for the
-reference.
+reference. An INT8 prefix cache (KVCache(quantized=True)) is refused.
 """
 from __future__ import annotations
 
@@ -25,7 +25,7 @@ from collections import OrderedDict
 
 import torch
 
-from ..qwen21 import KVLayerCache, modulation_values
+from ..qwen21 import KVLayerCache, QuantizedKVLayerCache, modulation_values
 from .decode import _key_valid, bound_blocks
 
 
@@ -95,6 +95,9 @@ def install_cuda_graph(transformer, max_graphs: int = 1) -> None:
         kv_cache = step.get("kv_cache")
         if kv_cache is None:
             raise RuntimeError("the graph replay needs the model's kv_cache argument")
+        if isinstance(kv_cache.get_layer(0), QuantizedKVLayerCache):
+            raise NotImplementedError("the graph replay keeps a bf16 prefix cache of its own; decode over an INT8 "
+                                      "KVCache without install_cuda_graph")
         h, mod, rope = kwargs["hidden_states"], kwargs["modulation"], kwargs["rotary_emb"]
         mask = kwargs.get("attention_mask")
         key = (tuple(h.shape), tuple(mod.shape), tuple(rope.shape), h.dtype, tuple(kv_cache.get_layer(0).k.shape),

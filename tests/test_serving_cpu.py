@@ -132,3 +132,28 @@ def test_attention_and_read_back_refuse_outputs_over_their_inputs(host, monkeypa
     with pytest.raises(ValueError, match="overlap"):
         host.kv_cache_read(cache, tokens=5, out_k=k, out_v=buf[:, 2:7, :, 128:256])
     host.kv_cache_read(cache, tokens=5, out_k=k, out_v=v)
+
+
+def test_step_graph_refuses_an_int8_cache():
+    from qwen_image_accel_b200.optimizations import cuda_graph, decode
+    from qwen_image_accel_b200.qwen21 import KVCache
+
+    class Block(torch.nn.Module):
+        def forward(self, hidden_states, **kwargs):
+            return hidden_states
+
+    class Model(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.transformer_blocks = [Block(), Block()]
+
+        def forward(self, kv_cache=None, **kwargs):
+            return self.transformer_blocks[0].forward(**kwargs)
+
+    model = Model()
+    setattr(model, decode._STATE, {"bound": [None, None]})
+    cuda_graph.install_cuda_graph(model)
+    h = torch.zeros(1, 4, 8)
+    step = {"hidden_states": h, "modulation": h, "rotary_emb": h, "kv_cache_mode": "cached"}
+    with pytest.raises(NotImplementedError, match="INT8"):
+        model(kv_cache=KVCache(2, quantized=True), **step)
