@@ -175,8 +175,9 @@ def stream(device: torch.device | None = None):
 
 
 # handle of the current stream of a device index, without the Stream object
-# around it (2.4 us of a small op's call)
-raw_stream = torch._C._cuda_getCurrentRawStream
+# around it (2.4 us of a small op's call); None in a torch without CUDA, which can
+# import this package but calls nothing
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:

@@ -157,3 +157,14 @@ def test_step_graph_refuses_an_int8_cache():
     step = {"hidden_states": h, "modulation": h, "rotary_emb": h, "kv_cache_mode": "cached"}
     with pytest.raises(NotImplementedError, match="INT8"):
         model(kv_cache=KVCache(2, quantized=True), **step)
+
+
+def test_the_package_imports_in_a_torch_without_cuda():
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = ("import torch\ndel torch._C._cuda_getCurrentRawStream\n"
+            "import qwen_image_accel_b200.kernels.lora, qwen_image_accel_b200.qwen21_model\n")
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
+                          cwd=Path(__file__).resolve().parents[1] / "qwen-image-2.1-accel_b200")
+    assert done.returncode == 0, done.stderr[-500:]
