@@ -43,6 +43,7 @@ class QuantizedKV:
                    torch.zeros(shape, dtype=torch.float32, device=dev),
                    torch.zeros(batch, dtype=torch.int32, device=dev),
                    torch.zeros(batch, dtype=torch.int32, device=dev), 0)
+        self._count(0)
 
     @classmethod
     def from_tensors(cls, k_codes, v_codes, k_scales, v_scales, lengths, extent: int) -> "QuantizedKV":
@@ -68,7 +69,8 @@ class QuantizedKV:
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
         self.lengths, self._tickets = lengths, tickets
         self.batch, self.kv_heads, self.capacity = batch, heads, capacity
-        self._held, self._first = [extent] * batch if held is None else held, first
+        # per request: the most that it may hold, and whether it holds just that
+        self._held, self._first = [(extent, False)] * batch if held is None else held, first
         self.device, self._index = k_codes.device, k_codes.get_device()
         # the buffers' addresses, for the calls below
         self._buffers = tuple(t.data_ptr() for t in (k_codes, v_codes, k_scales, v_scales, lengths))
@@ -89,11 +91,25 @@ class QuantizedKV:
 
     @property
     def extent(self) -> int:
-        return max(self._held[self._first:self._first + self.batch], default=0)
+        return max(self._held[self._first:self._first + self.batch], default=(0, True))[0]
 
     @extent.setter
     def extent(self, tokens: int) -> None:
-        self._held[self._first:self._first + self.batch] = [tokens] * self.batch
+        self._held[self._first:self._first + self.batch] = [(tokens, False)] * self.batch
+
+    @property
+    def uniform(self) -> bool:
+        """Whether every request is known to hold `extent` tokens, as after one
+        write to all of them (not after `extent` was set, from_tensors included)."""
+        held = set(self._held[self._first:self._first + self.batch])
+        return len(held) <= 1 and all(known for _, known in held)
+
+    def _count(self, tokens: int, behind: bool = False) -> None:
+        """Each request holds `tokens` tokens, or that many more. What a captured
+        call will write at its replays is not known."""
+        known = not (torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing())
+        part = slice(self._first, self._first + self.batch)
+        self._held[part] = [(n + tokens, k and known) if behind else (tokens, known) for n, k in self._held[part]]
 
 
 def _strides(t: torch.Tensor) -> tuple[int, int, int]:
@@ -131,7 +147,7 @@ def kv_cache_write(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor, start: 
     if start < 0 or start + seq > cache.capacity:
         raise ValueError(f"kv_cache_write: tokens {start}+{seq} of capacity {cache.capacity}")
     _write(cache, k, v, seq, start)
-    cache.extent = start + seq
+    cache._count(start + seq)
 
 
 def kv_cache_append(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -143,8 +159,7 @@ def kv_cache_append(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> Non
     if extent + seq > cache.capacity:
         raise ValueError(f"kv_cache_append: {seq} tokens behind {extent} of capacity {cache.capacity}")
     _write(cache, k, v, seq, -1)
-    for i in range(cache._first, cache._first + cache.batch):
-        cache._held[i] += seq
+    cache._count(seq, behind=True)
 
 
 def _write(cache, k, v, seq, start):

@@ -103,8 +103,9 @@ class KVLayerCache:
 
 class QuantizedKVLayerCache:
     """KVLayerCache in INT8: a prefix is quantised as it is stored and takes
-    half the memory. `quantized` is the cache that the attention reads; get()
-    reads bf16 rows back for anything else."""
+    half the memory. `quantized` is the cache that the attention reads (one
+    whose requests differ in length may be put there); get() reads bf16 rows
+    back for anything else, zeros past a request's length."""
 
     def __init__(self):
         self.quantized: QuantizedKV | None = None
@@ -371,6 +372,14 @@ class Block21:
             ov[:, :p].copy_(cached_v)
         return p, oq, ok, ov
 
+    def _sage_over(self, layer_cache, key_valid) -> bool:
+        """Whether the decode runs on the Sage attention: it takes no mask, and
+        so no prefix whose requests differ in length."""
+        if not self.sage or key_valid is not None:
+            return False
+        cache = layer_cache.quantized if isinstance(layer_cache, QuantizedKVLayerCache) else None
+        return cache is None or cache.uniform
+
     def _attend_quantized(self, x, b, st, freqs, cache: QuantizedKV | None, key_valid, ids=None):
         """bf16 attention of the target tokens (LN output x) over [INT8 prefix,
         target], without a joint K/V copy."""
@@ -393,7 +402,7 @@ class Block21:
         b, st, _ = h.shape
         h = h.contiguous()
         ids = adapter_ids if self.adapters else None
-        sage = self.sage and key_valid is None
+        sage = self._sage_over(layer_cache, key_valid)
         # adapters multiply the bf16 activation: the LN output then stays bf16
         x = self._normalized(h, s1, self.qkv_mx and ids is None)
         if isinstance(layer_cache, QuantizedKVLayerCache) and not sage:
@@ -427,13 +436,14 @@ class Block21:
         is masked, else SDPA, or cached_attention over an INT8 prefix), output
         projection -> bf16 [B, St, D]."""
         b, st, _ = x.shape
-        if isinstance(layer_cache, QuantizedKVLayerCache) and not (self.sage and key_valid is None):
+        sage = self._sage_over(layer_cache, key_valid)
+        if isinstance(layer_cache, QuantizedKVLayerCache) and not sage:
             return self._out_proj(self._attend_quantized(x.contiguous(), b, st, freqs, layer_cache.quantized,
                                                          key_valid))
         p, oq, ok, ov = self._joint_with_prefix(layer_cache, b, st, x.device, shared=True)
         self._qkv_into(x.contiguous(), b, st, freqs, oq, ok, ov, p)
         q = oq[:, p:]
-        if self.sage and key_valid is None:
+        if sage:
             attn = sage_attention(q, ok, ov)
         else:
             mask = None if key_valid is None else key_valid[:, None, None, :]

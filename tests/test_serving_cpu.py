@@ -168,3 +168,22 @@ def test_the_package_imports_in_a_torch_without_cuda():
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
                           cwd=Path(__file__).resolve().parents[1] / "qwen-image-2.1-accel_b200")
     assert done.returncode == 0, done.stderr[-500:]
+
+
+def test_uniform_lengths_are_those_the_host_counted(host):
+    cache = host.QuantizedKV(2, 2, 32, device="cpu")
+    part = cache.select(1)
+    assert cache.uniform
+    host.kv_cache_write(cache, rows(2, 10), rows(2, 10))
+    host.kv_cache_append(cache, rows(2, 1), rows(2, 1))
+    assert cache.uniform and part.uniform
+    host.kv_cache_append(part, rows(1, 1), rows(1, 1))
+    assert not cache.uniform and part.uniform
+    host.kv_cache_append(cache.select(0), rows(1, 1), rows(1, 1))
+    assert cache.uniform
+    part.extent = 12
+    assert not cache.uniform and not part.uniform and cache.extent == 12
+    host.kv_cache_write(cache, rows(2, 3), rows(2, 3))
+    assert cache.uniform
+    same = host.QuantizedKV.from_tensors(cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales, cache.lengths, 3)
+    assert not same.uniform and same.extent == 3

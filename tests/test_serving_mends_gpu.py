@@ -184,3 +184,28 @@ def test_attention_written_over_its_queries(b, sq, h, kvh, n, fresh):
     k, v = (rows(g, b, fresh, kvh, 128) for _ in range(2)) if fresh else (None, None)
     want = cached_attention(q, cache, k, v)
     assert cached_attention(q, cache, k, v, out=q) is q and torch.equal(q, want)
+
+
+# ------------------------------------------------------------- prefixes of different lengths
+@pytest.mark.parametrize("profile", ["fused", "fused_sage", "mxfp8_sage"])
+def test_a_block_leaves_out_what_a_shorter_request_does_not_hold(profile):
+    """Without a mask, the requests' lengths are the mask (the Sage attention
+    took the rows past them as keys of zeros)."""
+    from test_block21_gpu import build, t_bf16
+    from qwen_image_accel_b200.kernels.kv_cache import QuantizedKV, kv_cache_write
+    from qwen_image_accel_b200.qwen21 import QuantizedKVLayerCache, modulation_values
+    blk, gold = build(profile)
+    ht = t_bf16(gold["h_target"]).cuda().repeat(2, 1, 1)
+    mod = t_bf16(gold["modulation"]).cuda()
+    vals = modulation_values(torch.cat([mod[:1], mod[:1], mod[1:]]))
+    p = int(gold["prefix_len"])
+    freqs = torch.view_as_complex(torch.from_numpy(gold["rope"]).contiguous()).cuda()[p:].contiguous()
+    k, v = t_bf16(gold["cached_k"]).cuda(), t_bf16(gold["cached_v"]).cuda()
+    layer = QuantizedKVLayerCache()
+    layer.quantized = QuantizedKV(2, k.shape[2], p)
+    kv_cache_write(layer.quantized.select(0), k, v)
+    kv_cache_write(layer.quantized.select(1), k[:, :p // 3], v[:, :p // 3])
+    valid = torch.ones(2, p + ht.shape[1], dtype=torch.bool, device=DEV)
+    valid[1, p // 3:p] = False
+    assert torch.equal(blk.forward_cached(ht, vals, freqs, layer), blk.forward_cached(ht, vals, freqs, layer, valid))
+    assert torch.equal(blk.attention_cached(ht, freqs, layer), blk.attention_cached(ht, freqs, layer, valid))
