@@ -105,11 +105,14 @@ class QuantizedKV:
         return len(held) <= 1 and all(known for _, known in held)
 
     def _count(self, tokens: int, behind: bool = False) -> None:
-        """Each request holds `tokens` tokens, or that many more. What a captured
-        call will write at its replays is not known."""
-        known = not (torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing())
+        """Each request holds `tokens` tokens, or that many more (how often a
+        captured append will be replayed is not known)."""
         part = slice(self._first, self._first + self.batch)
-        self._held[part] = [(n + tokens, k and known) if behind else (tokens, known) for n, k in self._held[part]]
+        if behind:
+            known = not (torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing())
+            self._held[part] = [(n + tokens, k and known) for n, k in self._held[part]]
+        else:
+            self._held[part] = [(tokens, True)] * self.batch
 
 
 def _strides(t: torch.Tensor) -> tuple[int, int, int]:

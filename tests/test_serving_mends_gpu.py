@@ -209,3 +209,38 @@ def test_a_block_leaves_out_what_a_shorter_request_does_not_hold(profile):
     valid[1, p // 3:p] = False
     assert torch.equal(blk.forward_cached(ht, vals, freqs, layer), blk.forward_cached(ht, vals, freqs, layer, valid))
     assert torch.equal(blk.attention_cached(ht, freqs, layer), blk.attention_cached(ht, freqs, layer, valid))
+
+
+def test_a_captured_store_and_decode_equal_the_eager_ones():
+    """A store inside the graph keeps the block on the Sage attention; a
+    captured append leaves it (the host cannot count its replays)."""
+    from test_block21_gpu import build, t_bf16
+    from qwen_image_accel_b200.kernels.kv_cache import kv_cache_append
+    from qwen_image_accel_b200.qwen21 import QuantizedKVLayerCache, modulation_values
+    blk, gold = build("fused_sage")
+    ht, mod = t_bf16(gold["h_target"]).cuda(), t_bf16(gold["modulation"]).cuda()
+    vals, p = modulation_values(mod), int(gold["prefix_len"])
+    freqs = torch.view_as_complex(torch.from_numpy(gold["rope"]).contiguous()).cuda()[p:].contiguous()
+    k, v = t_bf16(gold["cached_k"]).cuda(), t_bf16(gold["cached_v"]).cuda()
+    layer = QuantizedKVLayerCache()
+
+    def step():
+        layer.store(k, v)
+        return blk.forward_cached(ht, vals, freqs, layer)
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    assert torch.equal(got, want) and layer.quantized.uniform
+    layer.quantized.extent = p - 1
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kv_cache_append(layer.quantized, k[:, :1], v[:, :1])
+    assert layer.quantized.extent == p and not layer.quantized.uniform
