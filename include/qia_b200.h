@@ -650,8 +650,14 @@ int qia_lora_add(const void* x, const void* base, void* y, const void* a,
                  void* stream);
 int64_t qia_lora_workspace_bytes(int64_t batch, int64_t seq, int64_t r_pad);
 
+/* Kernels that the four operators above (qia_kv_cache_write, qia_kv_cache_read,
+ * qia_cached_attention, qia_lora_add) have queued in this process: their calls
+ * choose forms of none to three kernels. Read only. */
+extern int64_t qia_launches;
+
 /* Reads and clears the device-side error word of the current device (set when
- * a bounded wait inside a tensor-core kernel gave up). Synchronises the device. */
+ * a bounded wait inside a tensor-core kernel gave up, or by what an entry says
+ * it records there). Synchronises the device. */
 int qia_device_error(int* code);
 
 #ifdef __cplusplus

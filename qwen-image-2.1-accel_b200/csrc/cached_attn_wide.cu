@@ -434,6 +434,7 @@ int launch_cached_wide(const CachedAttn& p, int batch, void* workspace, cudaStre
     cached_widen_kernel<<<dim3(unsigned(wd.tiles), unsigned(p.kv_heads), unsigned(batch)), 256, 0, st>>>(p, wd);
     rc = check_launch("cached_widen_kernel");
     if (rc) return rc;
+    count_launch();
   }
   static std::atomic<int> resident[17];
   return launch_waves(
@@ -462,6 +463,7 @@ int launch_cached_wide(const CachedAttn& p, int batch, void* workspace, cudaStre
           cudaGetLastError();
           return set_error(QIA_ERR_CUDA, "cached_attn_wide_kernel: %s", cudaGetErrorString(e));
         }
+        count_launch();
         return int(QIA_OK);
       });
 }

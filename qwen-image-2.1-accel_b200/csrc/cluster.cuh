@@ -127,6 +127,7 @@ int launch_cluster(const char* what, void (*kernel)(KArgs...), dim3 grid, int th
     cudaGetLastError();
     return set_error(QIA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   }
+  count_launch();
   return QIA_OK;
 }
 

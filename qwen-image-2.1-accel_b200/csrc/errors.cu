@@ -23,6 +23,14 @@ int check_launch(const char* what) {
   return QIA_OK;
 }
 
+}  // namespace qia
+
+int64_t qia_launches = 0;
+
+namespace qia {
+
+void count_launch() { __atomic_fetch_add(&qia_launches, int64_t(1), __ATOMIC_RELAXED); }
+
 int sm_count() {
   static int cached[64] = {0};
   int dev = 0;

@@ -236,7 +236,9 @@ extern "C" int qia_kv_cache_write(const void* k, const void* v, void* k_codes, v
   kv_write_kernel<<<grid, 256, 0, as_stream(stream)>>>(
       rows, make_cache(k_codes, v_codes, k_scales, v_scales, lengths, capacity, heads), int(batch), int(seq),
       append ? 0 : int(start), append, (unsigned*)ticket, device_error_word());
-  return check_launch(who);
+  rc = check_launch(who);
+  if (!rc) count_launch();
+  return rc;
 }
 
 extern "C" int qia_kv_cache_read(const void* k_codes, const void* v_codes, const void* k_scales, const void* v_scales,
@@ -261,5 +263,7 @@ extern "C" int qia_kv_cache_read(const void* k_codes, const void* v_codes, const
   kv_read_kernel<<<grid, 256, 0, as_stream(stream)>>>(
       make_cache((void*)k_codes, (void*)v_codes, (void*)k_scales, (void*)v_scales, (void*)lengths, capacity, heads),
       rows, int(first), int(tokens), wide);
-  return check_launch(who);
+  rc = check_launch(who);
+  if (!rc) count_launch();
+  return rc;
 }

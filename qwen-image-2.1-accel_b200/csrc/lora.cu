@@ -636,6 +636,7 @@ int launch_tiles(const Lora& p, void* workspace, cudaStream_t st) {
     cudaGetLastError();
     return set_error(QIA_ERR_CUDA, "lora_expand_kernel: %s", cudaGetErrorString(e));
   }
+  count_launch();
   return QIA_OK;
 }
 

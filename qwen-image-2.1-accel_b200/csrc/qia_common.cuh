@@ -23,6 +23,8 @@ int set_error(int code, const char* fmt, ...);
 
 // Checks the launch that was just queued; maps a CUDA error to QIA_ERR_CUDA.
 int check_launch(const char* what);
+// Adds one to qia_launches: a kernel of a serving operator was queued.
+void count_launch();
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 

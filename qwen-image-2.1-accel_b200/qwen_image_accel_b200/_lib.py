@@ -101,6 +101,7 @@ RAW_SIGNATURES: dict[str, tuple] = {
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+_launches: ctypes.c_int64 | None = None      # qia_launches of the loaded library
 
 
 class QiaError(RuntimeError):
@@ -112,7 +113,7 @@ class QiaError(RuntimeError):
 
 
 def load() -> ctypes.CDLL:
-    global _lib
+    global _lib, _launches
     if _lib is not None:
         return _lib
     with _lock:
@@ -132,6 +133,7 @@ def load() -> ctypes.CDLL:
                 fn = getattr(lib, name)
                 fn.argtypes = args
                 fn.restype = res
+            _launches = ctypes.c_int64.in_dll(lib, "qia_launches")
             _lib = lib
     return _lib
 
@@ -140,11 +142,14 @@ def declared_symbols() -> list[str]:
     return ["qia_last_error_string", "qia_abi_version", *SIGNATURES, *RAW_SIGNATURES]
 
 
-# kernels each entry point queues (for launch accounting); default 1
+# kernels each entry point queues (for launch accounting); default 1, None where the
+# library counts them itself
 KERNELS_PER_CALL = {"qia_sage_attention": 4, "qia_sage_attention_split": 4, "qia_sage_quantize": 3,
                     "qia_sage_attention_split_mx": 4, "qia_sage_quantize_joint": 3, "qia_sage_attention_joint_mx": 4,
                     "qia_sage_attention_noalloc": 4, "qia_sage_attention_prefill": 4,
-                    "qia_device_error": 0}
+                    "qia_device_error": 0,
+                    **dict.fromkeys(("qia_kv_cache_write", "qia_kv_cache_read", "qia_cached_attention",
+                                     "qia_lora_add"))}
 launch_count = 0
 
 
@@ -152,8 +157,14 @@ def call(name: str, *args) -> None:
     """Invoke a qia_* entry point and raise QiaError on a non-zero status."""
     global launch_count
     lib = _lib or load()
-    launch_count += KERNELS_PER_CALL.get(name, 1)
-    rc = getattr(lib, name)(*args)
+    kernels = KERNELS_PER_CALL.get(name, 1)
+    if kernels is None:
+        before = _launches.value
+        rc = getattr(lib, name)(*args)
+        launch_count += _launches.value - before
+    else:
+        launch_count += kernels
+        rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.qia_last_error_string().decode(errors="replace")
         raise QiaError(name, rc, msg)

@@ -244,3 +244,41 @@ def test_a_captured_store_and_decode_equal_the_eager_ones():
     with torch.cuda.graph(graph):
         kv_cache_append(layer.quantized, k[:, :1], v[:, :1])
     assert layer.quantized.extent == p and not layer.quantized.uniform
+
+
+# ------------------------------------------------------------- launch accounting
+def test_launches_are_counted_by_form():
+    from qwen_image_accel_b200 import _lib
+    from qwen_image_accel_b200.kernels.kv_cache import (QuantizedKV, cached_attention, kv_cache_append, kv_cache_read,
+                                                        kv_cache_write)
+    from qwen_image_accel_b200.kernels.lora import LoraWeights, lora_add
+    from test_lora_gpu import adapters, rand
+    g = gen(38)
+
+    def kernels(call):
+        before = _lib.launch_count
+        call()
+        return _lib.launch_count - before
+
+    small = QuantizedKV(1, 2, 64)
+    x = rows(g, 1, 8, 2, 128)
+    assert kernels(lambda: kv_cache_write(small, x, x)) == 1
+    assert kernels(lambda: kv_cache_append(small, x[:, :0], x[:, :0])) == 0
+    assert kernels(lambda: kv_cache_read(small)) == 1
+
+    def attend(b, h, n, sq):
+        cache, q = make_cache(g, b, h, n, [n] * b), rows(g, b, sq, h, 128)
+        return kernels(lambda: cached_attention(q, cache))
+
+    assert attend(1, 2, 64, 4) == 1               # one 16-row tile
+    assert attend(3, 40, 500, 77) == 1            # converted in place
+    assert attend(1, 2, 64, 77) == 2              # widened, attended
+    assert attend(1, 80, 900, 300) == 3           # and a remainder of twelve groups
+    w = LoraWeights(adapters(g, 512, 1024, [64]))
+
+    def adapt(b, s):
+        x, base = rand(g, b, s, 512), rand(g, b, s, 1024)
+        ids = torch.zeros(b, dtype=torch.int32, device=DEV)
+        return kernels(lambda: lora_add(x, base, w, ids))
+
+    assert adapt(2, 1) == 1 and adapt(2, 1000) == 2
