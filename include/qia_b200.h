@@ -641,7 +641,12 @@ int64_t qia_cached_attention_workspace_bytes(int64_t batch, int64_t seq_q,
  * ranks[i] hold zeros (rank 0: nothing is added). ranks, ids: int32, scales:
  * f32, device memory. in, out and r_pad multiples of 8, r_pad <= 128.
  * workspace: qia_lora_workspace_bytes bytes of device memory, 16-byte aligned
- * (NULL when that is 0, as it is for seq <= 8). */
+ * (NULL when that is 0, as it is for seq <= 8).
+ * fp32 sums, one rounding of y. scales[i] A_i x goes into the second product as
+ * two bf16 parts (2^-17 of it) where a token's weights are read for eight tokens
+ * at most, always so for seq <= 8, and as one (2^-9) in the form for many tokens.
+ * The form is chosen by sizes, batch included, so a request's last bits may
+ * depend on how many others it is served with. */
 int qia_lora_add(const void* x, const void* base, void* y, const void* a,
                  const void* b, const void* ranks, const void* scales,
                  const void* ids, int64_t batch, int64_t seq,

@@ -28,7 +28,8 @@
 //           cluster until the CTAs fill the device; partial sums are added
 //           through distributed shared memory in rank order; t is rounded to
 //           bf16 once (the operand type of the second product: at most 2^-9 of
-//           each |t_r B_r|, below the rounding of y where |B t| <= |y|);
+//           each |t_r B_r|, below the rounding of y where |B t| <= |y|; the token
+//           form keeps two parts, so precision goes with the form);
 //   expand  y = base + B_i t for 128 tokens x 128 outputs: base arrives by TMA,
 //           is added to the accumulator in place in shared memory and leaves by
 //           a TMA store. Launched as a dependent of shrink: its base and B tiles

@@ -67,7 +67,12 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
     seq, in], both bf16 with contiguous rows; ids: int32 [batch] on the device,
     -1 for a request without an adapter. Returns a new bf16 tensor, or `out`,
     which may be `base` itself but may not share memory with x or lie otherwise
-    over base."""
+    over base.
+
+    Sums are fp32. Up to 8 tokens per request the scaled A x is kept to 2^-17,
+    beyond that to one bf16 rounding (2^-9) wherever the form for many tokens is
+    the faster one. That depends on all sizes, the batch's too, so a request's
+    last bits may differ with the number of requests beside it."""
     who = "lora_add"
     _lib.require_cuda(x, base, ids, out)
     shape = x.shape
