@@ -609,9 +609,12 @@ int qia_kv_cache_read(const void* k_codes, const void* v_codes,
  * q, k, v, out (batch, seq, head each; multiples of 8). sm_scale <= 0:
  * 1/sqrt(128). The products' operands are f16: up to 16 query rows per K/V head
  * the INT8 codes as they are, above that cached and fresh rows scaled by powers
- * of two (one rounding to eleven bits); fp32 scores, sums and accumulators;
- * softmax weights are rounded once for the second product. head_dim = 128,
- * heads / kv_heads <= 128. workspace: qia_cached_attention_workspace_bytes bytes
+ * of two. There a cached element is code x scale with the scale kept to 15 bits,
+ * then rounded to eleven (2^-15 + 2^-11 of it; rows read back to bf16 lose 2^-8),
+ * and a score is off by up to that part of sum |q_d k_d| sm_scale, which shows in
+ * scores of some tens and more; with up to 16 rows the codes are exact. fp32 scores, sums and accumulators; softmax weights
+ * are rounded once, to f16, for the second product. There is no causal limit.
+ * head_dim = 128, heads / kv_heads <= 128. workspace: qia_cached_attention_workspace_bytes bytes
  * of device memory, 128-byte aligned (NULL when that is 0, as it is up to 16
  * query rows per K/V head). */
 int qia_cached_attention(const void* q, const void* k, const void* v,
@@ -644,7 +647,7 @@ int64_t qia_cached_attention_workspace_bytes(int64_t batch, int64_t seq_q,
  * (NULL when that is 0, as it is for seq <= 8).
  * fp32 sums, one rounding of y. scales[i] A_i x goes into the second product as
  * two bf16 parts (2^-17 of it) where a token's weights are read for eight tokens
- * at most, always so for seq <= 8, and as one (2^-9) in the form for many tokens.
+ * at most, always so for seq <= 8, and as one (2^-8) in the form for many tokens.
  * The form is chosen by sizes, batch included, so a request's last bits may
  * depend on how many others it is served with. */
 int qia_lora_add(const void* x, const void* base, void* y, const void* a,

@@ -78,7 +78,7 @@ __device__ __forceinline__ uint32_t cvt_f16x2(float lo, float hi) {
   return r;
 }
 
-// A key's factor, kept to 15 bits (2^-16 of the scale, a sixteenth of the f16
+// A key's factor, kept to 15 bits (2^-15 of the scale, a sixteenth of the f16
 // rounding): its products with the offset below and with a code are then exact.
 __device__ __forceinline__ float code_factor(float x) {
   return x == x ? __uint_as_float((__float_as_uint(x) + 256u) & 0xfffffe00u) : x;

@@ -27,7 +27,7 @@
 //   shrink  t = scale_i A_i x for 128 tokens, the contraction split over a
 //           cluster until the CTAs fill the device; partial sums are added
 //           through distributed shared memory in rank order; t is rounded to
-//           bf16 once (the operand type of the second product: at most 2^-9 of
+//           bf16 once (the operand type of the second product: at most 2^-8 of
 //           each |t_r B_r|, below the rounding of y where |B t| <= |y|; the token
 //           form keeps two parts, so precision goes with the form);
 //   expand  y = base + B_i t for 128 tokens x 128 outputs: base arrives by TMA,

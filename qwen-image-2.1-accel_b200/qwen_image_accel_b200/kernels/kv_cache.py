@@ -206,7 +206,7 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
                      v: torch.Tensor | None = None, key_valid: torch.Tensor | None = None,
                      scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(scale q K^T) V over [cached prefix, fresh k / v], unmasked but
-    for key_valid.
+    for key_valid (no causal limit: a query sees every fresh key).
 
     q: bf16 [batch, seq, heads, 128], heads a multiple of the cache's K/V
     heads (query head h reads K/V head h // (heads // kv_heads)); k, v: bf16

@@ -70,7 +70,7 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
     over base.
 
     Sums are fp32. Up to 8 tokens per request the scaled A x is kept to 2^-17,
-    beyond that to one bf16 rounding (2^-9) wherever the form for many tokens is
+    beyond that to one bf16 rounding (2^-8) wherever the form for many tokens is
     the faster one. That depends on all sizes, the batch's too, so a request's
     last bits may differ with the number of requests beside it."""
     who = "lora_add"
