@@ -612,11 +612,12 @@ int qia_kv_cache_read(const void* k_codes, const void* v_codes,
  * of two. There a cached element is code x scale with the scale kept to 15 bits,
  * then rounded to eleven (2^-15 + 2^-11 of it; rows read back to bf16 lose 2^-8),
  * and a score is off by up to that part of sum |q_d k_d| sm_scale, which shows in
- * scores of some tens and more; with up to 16 rows the codes are exact. fp32 scores, sums and accumulators; softmax weights
- * are rounded once, to f16, for the second product. There is no causal limit.
- * head_dim = 128, heads / kv_heads <= 128. workspace: qia_cached_attention_workspace_bytes bytes
- * of device memory, 128-byte aligned (NULL when that is 0, as it is up to 16
- * query rows per K/V head). */
+ * scores of some tens and more; with up to 16 rows the codes are exact. fp32
+ * scores, sums and accumulators; softmax weights are rounded once, to f16, for
+ * the second product. There is no causal limit. head_dim = 128, heads / kv_heads
+ * <= 128. workspace: qia_cached_attention_workspace_bytes bytes of device memory,
+ * 128-byte aligned (NULL when that is 0, as it is up to 16 query rows per K/V
+ * head). */
 int qia_cached_attention(const void* q, const void* k, const void* v,
                          const void* k_codes, const void* v_codes,
                          const void* k_scales, const void* v_scales,

@@ -191,6 +191,13 @@ def stream(device: torch.device | None = None):
 raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def used_strides(strides, *shapes) -> list[int]:
+    """The leading strides of tensors (one after another, as many of each as its
+    entry of `shapes` has sizes) with 0 for dimensions of size 1: nothing is ever
+    that far apart, so what a view has there need not be a multiple of anything."""
+    return [0 if n == 1 else s for n, s in zip((n for shape in shapes for n in shape), strides)]
+
+
 def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors of one element size share an element (exact: columns
     of one buffer that lie beside each other do not)."""

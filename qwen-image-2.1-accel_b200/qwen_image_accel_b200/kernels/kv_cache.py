@@ -22,6 +22,14 @@ _strides12 = struct.Struct("12q").pack
 _NO_ROWS = (0,) * 6
 
 
+class _Held:
+    """What the host knows of a cache's requests: per request, the most tokens
+    that it may hold and whether it holds just that; `changes` counts updates."""
+
+    def __init__(self, extent: int, batch: int):
+        self.counts, self.changes = [(extent, False)] * batch, 0
+
+
 class QuantizedKV:
     """K and V of up to `capacity` tokens of each of `batch` requests.
 
@@ -69,8 +77,8 @@ class QuantizedKV:
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
         self.lengths, self._tickets = lengths, tickets
         self.batch, self.kv_heads, self.capacity = batch, heads, capacity
-        # per request: the most that it may hold, and whether it holds just that
-        self._held, self._first = [(extent, False)] * batch if held is None else held, first
+        self._held, self._first = _Held(extent, batch) if held is None else held, first
+        self._seen, self._extent = -1, 0
         self.device, self._index = k_codes.device, k_codes.get_device()
         # the buffers' addresses, for the calls below
         self._buffers = tuple(t.data_ptr() for t in (k_codes, v_codes, k_scales, v_scales, lengths))
@@ -91,37 +99,45 @@ class QuantizedKV:
 
     @property
     def extent(self) -> int:
-        return max(self._held[self._first:self._first + self.batch], default=(0, True))[0]
+        held = self._held
+        if self._seen != held.changes:
+            self._extent = max(held.counts[self._first:self._first + self.batch], default=(0, True))[0]
+            self._seen = held.changes
+        return self._extent
 
     @extent.setter
     def extent(self, tokens: int) -> None:
-        self._held[self._first:self._first + self.batch] = [(tokens, False)] * self.batch
+        self._hold([(tokens, False)] * self.batch)
+
+    def _hold(self, counts: list) -> None:
+        self._held.counts[self._first:self._first + self.batch] = counts
+        self._held.changes += 1
 
     @property
     def uniform(self) -> bool:
         """Whether every request is known to hold `extent` tokens, as after one
         write to all of them (not after `extent` was set, from_tensors included)."""
-        held = set(self._held[self._first:self._first + self.batch])
+        held = set(self._held.counts[self._first:self._first + self.batch])
         return len(held) <= 1 and all(known for _, known in held)
 
     def _count(self, tokens: int, behind: bool = False) -> None:
         """Each request holds `tokens` tokens, or that many more (how often a
         captured append will be replayed is not known)."""
-        part = slice(self._first, self._first + self.batch)
         if behind:
             known = not (torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing())
-            self._held[part] = [(n + tokens, k and known) for n, k in self._held[part]]
+            counts = self._held.counts[self._first:self._first + self.batch]
+            self._hold([(n + tokens, k and known) for n, k in counts])
         else:
-            self._held[part] = [(tokens, True)] * self.batch
+            self._hold([(tokens, True)] * self.batch)
 
 
-def _strides(t: torch.Tensor) -> tuple[int, int, int]:
-    """Batch, sequence and head strides; 0 for a dimension of size 1 whose
-    stride is odd (nothing is ever that far apart)."""
-    a, b, c, _ = t.stride()
-    if (a | b | c) & 7:
-        return tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], (a, b, c)))
-    return a, b, c
+def _strides(a: torch.Tensor, b: torch.Tensor) -> tuple:
+    """Batch, sequence and head strides of a, then of b."""
+    i, j, k, _ = a.stride()
+    m, n, o, _ = b.stride()
+    if (i | j | k | m | n | o) & 7:
+        return tuple(_lib.used_strides((i, j, k, m, n, o), a.shape[:3], b.shape[:3]))
+    return i, j, k, m, n, o
 
 
 def _check_rows(who: str, cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -137,7 +153,8 @@ def _check_rows(who: str, cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) 
 
 
 def _check_output(who: str, out: torch.Tensor) -> None:
-    if any(n > 1 and not s for n, s in zip(out.shape, out.stride())):
+    strides = out.stride()
+    if 0 in strides and any(n > 1 and not s for n, s in zip(out.shape, strides)):
         raise ValueError(f"{who}: several elements of an output share memory")
 
 
@@ -168,7 +185,7 @@ def kv_cache_append(cache: QuantizedKV, k: torch.Tensor, v: torch.Tensor) -> Non
 def _write(cache, k, v, seq, start):
     kc, vc, ks, vs, lengths = cache._buffers
     _lib.call("qia_kv_cache_write", k.data_ptr(), v.data_ptr(), kc, vc, ks, vs, lengths, cache.batch, seq,
-              cache.kv_heads, HEAD_DIM, cache.capacity, start, _strides6(*_strides(k), *_strides(v)),
+              cache.kv_heads, HEAD_DIM, cache.capacity, start, _strides6(*_strides(k, v)),
               cache._ticket, _lib.raw_stream(cache._index))
 
 
@@ -197,7 +214,7 @@ def kv_cache_read(cache: QuantizedKV, first: int = 0, tokens: int | None = None,
         if _lib.overlaps(out_k, out_v):
             raise ValueError("kv_cache_read: the outputs overlap")
     _lib.call("qia_kv_cache_read", *cache._buffers, out_k.data_ptr(), out_v.data_ptr(), cache.batch, first, tokens,
-              cache.kv_heads, HEAD_DIM, cache.capacity, _strides6(*_strides(out_k), *_strides(out_v)),
+              cache.kv_heads, HEAD_DIM, cache.capacity, _strides6(*_strides(out_k, out_v)),
               _lib.raw_stream(cache._index))
     return out_k, out_v
 
@@ -232,7 +249,7 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
     extent, fresh, rows = cache.extent, 0, _NO_ROWS
     if k is not None:
         _check_rows(who, cache, k, v)
-        fresh, rows = k.shape[1], _strides(k) + _strides(v)
+        fresh, rows = k.shape[1], _strides(k, v)
     mask_stride = 0
     if key_valid is not None:
         if key_valid.shape != (cache.batch, extent + fresh) or key_valid.dtype != torch.bool:
@@ -257,9 +274,10 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKV, k: torch.Tensor | None
         size = _lib.load().qia_cached_attention_workspace_bytes(cache.batch, shape[1], fresh, shape[2], cache.kv_heads,
                                                                 extent)
     ws = q.new_empty(size >> 1) if size else None       # (bf16 elements)
+    outer = _strides(q, out)
     _lib.call("qia_cached_attention", q.data_ptr(), k.data_ptr() if fresh else None, v.data_ptr() if fresh else None,
               *cache._buffers, None if key_valid is None else key_valid.data_ptr(), out.data_ptr(), cache.batch,
               shape[1], fresh, shape[2], cache.kv_heads, HEAD_DIM, cache.capacity, extent,
-              _strides12(*_strides(q), *rows, *_strides(out)), mask_stride, 0.0 if scale is None else float(scale),
+              _strides12(*outer[:3], *rows, *outer[3:]), mask_stride, 0.0 if scale is None else float(scale),
               None if ws is None else ws.data_ptr(), _lib.raw_stream(cache._index))
     return out

@@ -17,15 +17,6 @@ MAX_RANK = 128
 _strides6 = struct.Struct("6q").pack      # stride arguments (int64[]) as bytes
 
 
-def _strides(t: torch.Tensor) -> tuple[int, int]:
-    """Batch and sequence strides; 0 for a dimension of size 1 whose stride is
-    odd (nothing is ever that far apart)."""
-    a, b, _ = t.stride()
-    if (a | b) & 7:
-        return tuple(0 if n == 1 else s for n, s in zip(t.shape[:2], (a, b)))
-    return a, b
-
-
 class LoraWeights:
     """The adapters of one projection, laid out once: `adapters` is a list of
     (A [rank, in], B [out, rank], scale), ranks to 128 in any mix (rank 0: an
@@ -80,7 +71,9 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
         raise ValueError(f"{who}: x {tuple(x.shape)} and base {tuple(base.shape)} do not fit a "
                          f"{weights.in_features} -> {weights.out_features} projection")
     batch, seq, _ = shape
-    if x.dtype != torch.bfloat16 or base.dtype != torch.bfloat16 or x.stride(2) != 1 or base.stride(2) != 1:
+    x_batch, x_row, x_unit = x.stride()
+    base_batch, base_row, base_unit = base.stride()
+    if x.dtype != torch.bfloat16 or base.dtype != torch.bfloat16 or x_unit != 1 or base_unit != 1:
         raise NotImplementedError(f"{who}: x and base must be bf16 with contiguous rows")
     if ids.shape != (batch,) or ids.dtype != torch.int32 or not ids.is_contiguous():
         raise ValueError(f"{who}: ids must be int32 [{batch}], got {ids.dtype} {tuple(ids.shape)}")
@@ -91,14 +84,16 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
         raise ValueError(f"{who}: out must be like base")
     if not out.numel():
         return out
+    out_batch, out_row, out_unit = strides = out.stride()
     if given:
-        if any(n > 1 and not s for n, s in zip(out.shape, out.stride())):
+        if 0 in strides and any(n > 1 and not s for n, s in zip(out.shape, strides)):
             raise ValueError(f"{who}: several elements of out share memory")
         if _lib.overlaps(out, x):
             raise ValueError(f"{who}: out may be base, not x or a part of it")
-        if (out.data_ptr() != base.data_ptr() or out.stride() != base.stride()) and _lib.overlaps(out, base):
+        if out is not base and (out.data_ptr() != base.data_ptr() or strides != base.stride()) and \
+                _lib.overlaps(out, base):
             raise ValueError(f"{who}: out may be base, not overlap it")
-    if out.stride(2) != 1:
+    if out_unit != 1:
         raise NotImplementedError(f"{who}: out must have contiguous rows")
     index = weights._index
     if x.get_device() != index or base.get_device() != index or ids.get_device() != index or out.get_device() != index:
@@ -106,8 +101,11 @@ def lora_add(x: torch.Tensor, base: torch.Tensor, weights: LoraWeights, ids: tor
     # (up to eight tokens per request need none)
     size = _lib.load().qia_lora_workspace_bytes(batch, seq, weights.r_pad) if seq > 8 else 0
     ws = x.new_empty(size >> 1) if size else None       # (bf16 elements)
+    rows = x_batch, x_row, base_batch, base_row, out_batch, out_row
+    if (x_batch | x_row | base_batch | base_row | out_batch | out_row) & 7:
+        rows = _lib.used_strides(rows, shape[:2], shape[:2], shape[:2])
     _lib.call("qia_lora_add", x.data_ptr(), base.data_ptr(), out.data_ptr(), *weights._buffers, ids.data_ptr(), batch,
               seq, weights.in_features, weights.out_features, weights.count, weights.r_pad,
-              _strides6(*_strides(x), *_strides(base), *_strides(out)), None if ws is None else ws.data_ptr(),
+              _strides6(*rows), None if ws is None else ws.data_ptr(),
               _lib.raw_stream(index))
     return out
