@@ -199,8 +199,10 @@ cached_attn_wide_kernel(const __grid_constant__ CachedAttn p, const __grid_const
     mbar_init(smem_u32(q_full), 4 * n_tiles);
     for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&turn[i]), 1);
     fence_barrier_init();
-    prefetch_tmap(&tm_k);
-    prefetch_tmap(&tm_v);
+    if (wd.tiles) {                        // (a call without keys has no maps)
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+    }
   }
   if (warp == 9) tmem_alloc(smem_u32(tmem_slot), 512);
   tc_fence_before();
@@ -415,7 +417,7 @@ int launch_cached_wide(const CachedAttn& p, int batch, void* workspace, cudaStre
   if (rc) return rc;
   TileGrid g = tile_grid(p);
   const int64_t groups = int64_t(g.pairs) * p.kv_heads * batch, heads = int64_t(batch) * p.kv_heads;
-  Widened wd;
+  Widened wd = {};
   wd.cached_cap = (p.extent + 127) / 128;
   wd.tiles = wd.cached_cap + (p.sk + 127) / 128;
   const int64_t rows = heads * wd.tiles * 128;

@@ -282,3 +282,18 @@ def test_launches_are_counted_by_form():
         return kernels(lambda: lora_add(x, base, w, ids))
 
     assert adapt(2, 1) == 1 and adapt(2, 1000) == 2
+
+
+# ------------------------------------------------------------- no keys at all
+@pytest.mark.parametrize("sq", [1, 16, 17, 100, 300])
+def test_attention_over_an_empty_cache_and_no_fresh_keys(sq):
+    from qwen_image_accel_b200 import _lib
+    from qwen_image_accel_b200.kernels.kv_cache import QuantizedKV, cached_attention
+    g = gen(39)
+    cache = QuantizedKV(3, 60, 40)
+    q = rows(g, 3, sq, 60, 128)
+    out = torch.full_like(q, float("nan"))
+    assert not cached_attention(q, cache, out=out).any()
+    none, mask = q[:, :0], torch.zeros(3, 0, dtype=torch.bool, device=DEV)
+    assert not cached_attention(q, cache, none, none, key_valid=mask).any()
+    assert _lib.device_error() == 0
