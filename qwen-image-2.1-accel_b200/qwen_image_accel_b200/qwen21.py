@@ -114,7 +114,7 @@ class QuantizedKVLayerCache:
         b, n, h, _ = k.shape
         c = self.quantized
         if c is None or c.batch != b or c.kv_heads != h or c.capacity < n or c.device != k.device:
-            c = self.quantized = QuantizedKV(b, h, n, device=k.device)
+            c = self.quantized = QuantizedKV(b, h, max(n, 1), device=k.device)
         kv_cache_write(c, k, v)
 
     def get(self) -> tuple[torch.Tensor, torch.Tensor]:

@@ -297,3 +297,20 @@ def test_attention_over_an_empty_cache_and_no_fresh_keys(sq):
     none, mask = q[:, :0], torch.zeros(3, 0, dtype=torch.bool, device=DEV)
     assert not cached_attention(q, cache, none, none, key_valid=mask).any()
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("profile", ["fused", "fused_sage"])
+def test_an_empty_prefix_is_stored_and_decoded_like_a_bf16_one(profile):
+    from test_block21_gpu import build, psnr, t_bf16
+    from qwen_image_accel_b200.qwen21 import KVLayerCache, QuantizedKVLayerCache, modulation_values
+    blk, gold = build(profile)
+    ht, mod = t_bf16(gold["h_target"]).cuda(), t_bf16(gold["modulation"]).cuda()
+    freqs = torch.view_as_complex(torch.from_numpy(gold["rope"]).contiguous()).cuda()[int(gold["prefix_len"]):]
+    k = t_bf16(gold["cached_k"]).cuda()[:, :0]
+    outs = []
+    for layer in (KVLayerCache(), QuantizedKVLayerCache()):
+        layer.store(k, k)
+        assert layer.get()[0].shape == k.shape
+        outs.append(blk.forward_cached(ht, modulation_values(mod), freqs.contiguous(), layer))
+    # no cached row, so nothing of INT8: the same attention (Sage), or two roundings to bf16 of one (the weights, 40 dB at least)
+    assert torch.equal(*outs) if profile == "fused_sage" else psnr(*outs) >= 40
