@@ -55,11 +55,11 @@ constexpr int kSmemML = kSmemQScale + 256 * 4;                      // m, l of 2
 constexpr int kSmemFactor = kSmemML + 2 * 256 * 4;                  // [2 tiles][K, V][128] scale 2^-e of a tile's keys
 constexpr int kSmemSlots = kSmemFactor + 2 * 256 * 4;               // [2 tiles][K, V][writer] maxima
 constexpr int kSmemBars = kSmemSlots + 2 * 2 * kWriters * 4;
-constexpr int kBars = 48;
+constexpr int kBars = 55;
 // the TMEM address, read after the setup barrier: nothing that is written from then
 // on (the codes in flight) may share its bytes
 constexpr int kSmemTmem = kSmemBars + kBars * 8;
-constexpr int kSmemStage = kSmemTmem + 128;                         // codes in flight
+constexpr int kSmemStage = kSmemBars + 512;                         // codes in flight
 constexpr int kSmemBytes = kSmemStage + kUnits * kUnitBytes + 1024;
 static_assert(kSmemTmem + 4 <= kSmemStage, "the TMEM address has a place of its own");
 static_assert(kSmemStage % 16 == 0 && kSmemBytes <= 227 * 1024, "shared memory");
@@ -84,7 +84,12 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
   uint64_t* o_full = bars + 18;
   uint64_t* drain = bars + 19;
   uint64_t* q_full = bars + 20;       // softmax -> issuer
-  uint64_t* stage_full = bars + 21;   // [7] bulk copies -> operand writers
+  // bulk copies -> operand writers, [7] for K and for V: a parity wait only tells the
+  // phase from the one before, so a team's barriers count its own uses of a unit alone
+  // (with one barrier per unit, a team could take the other's copy, still on its way,
+  // for its own)
+  uint64_t* stage_full_k = bars + 21;
+  uint64_t* stage_full_v = bars + 48;
   uint64_t* stage_empty = bars + 28;  // [7] operand writers -> bulk copies
   uint64_t* factor_full = bars + 35;  // [2] factors of tile j % 2
   uint64_t* factor_empty = bars + 37; // [2]
@@ -137,7 +142,7 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
     const int arrivals = i < 4 || (i >= 28 && i < 35) || i == 20 ? kWriters      // k_full, v_full, stage_empty; q_full
                          : i >= 14 && i < 18                     ? 4             // p_full
                          : i == 37 || i == 38                    ? 2 * kWriters  // factor_empty
-                         : i >= 39                               ? 2             // fresh_done, info_full
+                         : i >= 39 && i < 48                     ? 2             // fresh_done, info_full
                                                                  : 1;
     mbar_init(smem_u32(&bars[i]), uint32_t(arrivals));
     fence_barrier_init();
@@ -247,15 +252,18 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
         ok = mbar_wait(smem_u32(&stage_empty[st]), phase ^ 1, err);
         if (!ok) break;
         const int k0 = (first + (u >> 2)) * kTileRows + (u & 1) * kUnitKeys, rows = max(0, min(len - k0, kUnitKeys));
-        mbar_arrive_expect_tx(smem_u32(&stage_full[st]), uint32_t(rows * kCaD));
+        const uint32_t full = smem_u32(((u & 2) ? stage_full_v : stage_full_k) + st);
+        mbar_arrive_expect_tx(full, uint32_t(rows * kCaD));
         if (rows > 0)
-          bulk_load(unit_at(st), ((u & 2) ? p.vc : p.kc) + (head_row + k0) * kCaD, uint32_t(rows * kCaD),
-                    smem_u32(&stage_full[st]));
+          bulk_load(unit_at(st), ((u & 2) ? p.vc : p.kc) + (head_row + k0) * kCaD, uint32_t(rows * kCaD), full);
         if (++st == units) { st = 0; phase ^= 1; }
       }
       if (!ok)   // let queued copies land before the shared memory is released
-        for (int i = max(0, u - units); i < u; ++i)
-          mbar_wait(smem_u32(&stage_full[i % units]), uint32_t((i / units) & 1), nullptr, 100000000ull);
+        for (int i = max(0, u - units); i < u; ++i) {
+          uint32_t uses = 0;                   // of the unit by that team before
+          for (int k = i % units; k < i; k += units) uses += ((k ^ i) & 2) == 0;
+          mbar_wait(smem_u32(((i & 2) ? stage_full_v : stage_full_k) + i % units), uses & 1, nullptr, 100000000ull);
+        }
     } else if (warp == 26) {
       // ---------------------------------------- numbers and factors of cached tiles
       // (keys lane + 32 i; the next tile's scales are requested before this one's are used)
@@ -371,16 +379,18 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
     const int row0 = 8 * writer + (lane >> 4);
     const uint32_t code_at = uint32_t(row0 * kCaD + piece * 8);
     const float* factors = reinterpret_cast<const float*>(smem + kSmemFactor) + z * 128 + row0;
+    uint64_t* stage_full = z ? stage_full_v : stage_full_k;
     int st = 2 * z;
-    uint32_t phase = 0;
+    uint32_t phases = 0;                     // bit st: of the team's next use of that unit
 #pragma unroll 1
     for (int u = 0; u < 2 * cached_n; ++u) {
       const int i0 = u >> 1, j = fresh_n + i0, h = u & 1;
       if (h == 0)
         ok = ok && mbar_wait(smem_u32(&factor_full[i0 & 1]), (i0 >> 1) & 1, err) &&
              mbar_wait(smem_u32(&empty[j & 1]), ((j >> 1) & 1) ^ 1, err);
-      ok = ok && mbar_wait(smem_u32(&stage_full[st]), phase, err);
+      ok = ok && mbar_wait(smem_u32(&stage_full[st]), (phases >> st) & 1, err);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      phases ^= 1u << st;
       const uint32_t from = unit_at(st) + code_at;
       uint2 codes[4];
       float a[4];
@@ -404,7 +414,7 @@ cached_attn_tiles_kernel(const __grid_constant__ CachedAttn p, const __grid_cons
       }
       if (h == 1) publish(j);
       st += h ? 3 : 1;                       // (the other operand's units lie between)
-      if (st >= units) { st -= units; phase ^= 1; }
+      if (st >= units) st -= units;
     }
   } else {
     // ----------------------------------------------------------------- softmax

@@ -314,3 +314,22 @@ def test_an_empty_prefix_is_stored_and_decoded_like_a_bf16_one(profile):
         outs.append(blk.forward_cached(ht, modulation_values(mod), freqs.contiguous(), layer))
     # no cached row, so nothing of INT8: the same attention (Sage), or two roundings to bf16 of one (the weights, 40 dB at least)
     assert torch.equal(*outs) if profile == "fused_sage" else psnr(*outs) >= 40
+
+
+# ------------------------------------------------------------- codes in flight for two teams
+@pytest.mark.parametrize("b,h,n,sq", [(3, 40, 600, 77), (2, 80, 900, 200), (1, 8, 5300, 60), (1, 8, 5300, 256)])
+def test_many_calls_with_cold_codes_give_the_same_bits(b, h, n, sq):
+    """Copies of K and V that land late and in another order: L2 holds other
+    data before each call."""
+    from qwen_image_accel_b200 import _lib
+    from qwen_image_accel_b200.kernels.kv_cache import cached_attention
+    g = gen(40)
+    cache = make_cache(g, b, h, n, [n] * b)
+    q = rows(g, b, sq, h, 128)
+    flush = torch.empty(1 << 27, dtype=torch.int16, device=DEV)
+    want = cached_attention(q, cache)
+    assert_attention(want, *attention64(q, cache, None, None, None))
+    for i in range(100):
+        flush.fill_(i)
+        assert torch.equal(cached_attention(q, cache), want)
+    assert _lib.device_error() == 0
