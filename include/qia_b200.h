@@ -614,7 +614,8 @@ int qia_kv_cache_read(const void* k_codes, const void* v_codes,
  * and a score is off by up to that part of sum |q_d k_d| sm_scale, which shows in
  * scores of some tens and more; with up to 16 rows the codes are exact. fp32
  * scores, sums and accumulators; softmax weights are rounded once, to f16, for
- * the second product. There is no causal limit. head_dim = 128, heads / kv_heads
+ * the second product (keys whose weight times V scale is 2^-33 of a row's largest
+ * may vanish). There is no causal limit. head_dim = 128, heads / kv_heads
  * <= 128. workspace: qia_cached_attention_workspace_bytes bytes of device memory,
  * 128-byte aligned (NULL when that is 0, as it is up to 16 query rows per K/V
  * head). */

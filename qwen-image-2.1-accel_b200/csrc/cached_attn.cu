@@ -28,8 +28,8 @@
 // on timing.
 //
 // On a B200, sixteen requests of 4097 to 16391 tokens, 32 / 8 heads, one token: 73 us,
-// 5.8 TB/s (89 % of the copy's rate). 32 heads over 4229 tokens: 11 to 12 us for 35
-// MB, of them 4.5 us launch, query, one fresh key and joining; the rest is latency,
+// 5.8 TB/s (89 % of the copy's rate). 32 heads over 4229 tokens: 12.6 us for 35
+// MB, of them 4.8 us launch, query, one fresh key and joining; the rest is latency,
 // with seven warps per SM. (Clusters of up to sixteen and five CTAs per SM were
 // slower, eight warps per CTA no faster.)
 #include "cached_attn.cuh"

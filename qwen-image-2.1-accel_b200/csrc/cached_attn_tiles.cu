@@ -36,7 +36,7 @@
 // tile: 3100 cycles per 128 keys, 2.4 TB/s of codes); with two, the softmax, which
 // sees every tile. Both are instruction issue: seven warps per scheduler, nine
 // instructions per four codes. Four requests of 77 rows, 32 heads, on a B200: 8192
-// cached tokens 117 us, 1024 25 us, 16 13 us (seven writer warps, each with its own
+// cached tokens 117 to 122 us, 1024 25 us, 16 12 us (seven writer warps, each with its own
 // copies and factors in unrolled code: 150, 28 and 13 us; eight in one team: 155,
 // 30 and 15 us; pieces of the scores read ahead while others are used: 119, 25 and
 // 14 us).

@@ -19,8 +19,8 @@
 //
 // The warps of the two groups that share a scheduler take their exponentials in
 // turn: both at once, each runs at half the unit's rate and then both wait for the
-// tensor cores (4096 rows over 8325 keys, 32 heads: 559 us without turns, 530 to 547
-// with).
+// tensor cores (4096 rows over 8325 keys, 32 heads: 559 us without turns on a card
+// that took 530 to 547 with them; 528 to 558 over several cards).
 //
 // What bounds it: the chain scores, softmax, weights, product of each query tile. Per
 // key tile and SM the tensor cores need 2050 cycles for both, the exponentials 2048;
